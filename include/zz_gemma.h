@@ -99,6 +99,15 @@ int zz_stack_prefill_dev(int stack, float *d_H, int S, int *d_tok, void *stream)
 int zz_stack_decode_dev(int stack, int *d_tok, int n, float *d_logits, int use_graph,
                         void *stream);
 
+/* Beam search from one token: n steps of W beams (1 <= W <= 16) through the blocks and the
+ * head, selected by zz_beam_step_dev (zz_beam.h) on the head's logits. d_seq [W][n + 1]
+ * receives the beams' tokens, d_tok[0] first, the best beam first; d_score [W] their
+ * accumulated log-probabilities. A beam that took `eos` (no token is -1) is finished and
+ * repeats it. Tokens never leave the device. A call that needs more room than any
+ * before allocates the search's rows and waits for the device; d_tok lies outside d_seq. */
+int zz_stack_beam_dev(int stack, const int *d_tok, int W, int n, int eos, int *d_seq, float *d_score,
+                      void *stream);
+
 /* zz_head_use_flash on the stack's head. */
 int zz_stack_use_flash(int stack, int on);
 

@@ -1,0 +1,307 @@
+"""8-bit rows and the fp8 product on the GPU against their 64-bit forms (zzref8.py)."""
+import numpy as np
+import pytest
+import torch
+
+import zzref8 as R
+import zunzuncito_amd as zz
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16 = torch.float32, torch.bfloat16
+KIND = {F32: zz.ZZ_F32, BF16: zz.ZZ_BF16}
+
+
+@pytest.fixture(autouse=True, scope="module")
+def _up():
+    zz.init()
+
+
+def stream():
+    return torch.cuda.current_stream().cuda_stream
+
+
+def inputs(S, D, dtype, seed, wide=1):
+    g = torch.Generator().manual_seed(seed)
+    col = 1 + 30 * (torch.rand(D * wide, generator=g) < 0.02)
+    x = (torch.randn(S, D * wide, generator=g) * col).to(dtype)
+    res = (3 * torch.randn(S, D * wide, generator=g) * col).to(dtype)
+    return x, res, 1 + 0.3 * torch.randn(D, generator=g)
+
+
+def buffers(S, D):
+    nb = R.blocks(D)
+    # a row behind the last one, and a guard, that have to stay as they are
+    return (torch.full((S + 1, nb * 128), 0x55, dtype=torch.uint8, device="cuda"),
+            torch.full((nb * S + 3,), -7.0, device="cuda"))
+
+
+def taken(q, s, S, D):
+    torch.cuda.synchronize()
+    assert bool((q[S] == 0x55).all()) and bool((s[-3:] == -7.0).all())
+    return q[:S].cpu(), s[:-3].view(-1, S).cpu()
+
+
+# one element, a block less one, a block, block edges, every number of groups a thread holds,
+# odd widths (rows that no vector load fits), the largest
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("S, D", [(1, 1), (3, 7), (1, 127), (2, 128), (5, 129), (1, 2816), (4, 2048), (3, 2049),
+                                  (2, 4095), (65, 1088), (1, 8192), (2, 8191), (130, 64)])
+def test_add_norm(dtype, S, D):
+    print("case", S, D, dtype, flush=True)
+    x, res, w = inputs(S, D, dtype, 100 + S + D)
+    X, Rs, Wt = x.cuda(), res.cuda(), w.cuda()
+    for use_res, use_w, store in ((True, True, True), (False, True, False), (True, False, False)):
+        q, s = buffers(S, D)
+        sm = torch.full((S + 1, D), -5.0, dtype=dtype, device="cuda")
+        zz.add_norm_fp8_dev(X.data_ptr(), Rs.data_ptr() if use_res else 0, sm.data_ptr() if store else 0,
+                            Wt.data_ptr() if use_w else 0, S, D, 1e-6, q.data_ptr(), s.data_ptr(), KIND[dtype],
+                            stream=stream())
+        qh, sh = taken(q, s, S, D)
+        h, y = R.norm_rows(x, res if use_res else None, w if use_w else None, float(np.float32(1e-6)))
+        R.check_rows(y, qh, sh, R.norm_delta(D))
+        if store:
+            got = sm[:S].cpu()
+            assert torch.equal(got, torch.from_numpy(h).float().to(dtype))     # h is f32's own: one rounding
+        assert bool((sm[S if store else 0:] == -5.0).all())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("D, ldx, off", [(2816, 5632, 0), (200, 203, 0), (256, 512, 1), (129, 160, 3)])
+def test_add_norm_strides_and_in_place(dtype, D, ldx, off):
+    """Rows apart, a start that no vector load fits, sum stored over res and over x."""
+    S = 9
+    g = torch.Generator().manual_seed(D)
+    xb = torch.randn(S * ldx + off, generator=g).to(dtype)
+    rb = torch.randn(S * ldx + off, generator=g).to(dtype)
+    w = 1 + 0.1 * torch.randn(D, generator=g)
+    for over in ("x", "res"):
+        X, Rs, Wt = xb.cuda(), rb.cuda(), w.cuda()
+        esz = X.element_size()
+        px, pr = X.data_ptr() + off * esz, Rs.data_ptr() + off * esz
+        q, s = buffers(S, D)
+        zz.add_norm_fp8_dev(px, pr, px if over == "x" else pr, Wt.data_ptr(), S, D, 1e-5, q.data_ptr(), s.data_ptr(),
+                            KIND[dtype], ldx=ldx, ldr=ldx, lds=ldx, stream=stream())
+        qh, sh = taken(q, s, S, D)
+        x = xb[off:].view(S, ldx)[:, :D]
+        r = rb[off:].view(S, ldx)[:, :D]
+        h, y = R.norm_rows(x, r, w, float(np.float32(1e-5)))
+        R.check_rows(y, qh, sh, R.norm_delta(D))
+        want = (xb if over == "x" else rb).clone()
+        want[off:].view(S, ldx)[:, :D] = torch.from_numpy(h).float().to(dtype)
+        assert torch.equal((X if over == "x" else Rs).cpu(), want)             # and nothing between the rows
+        assert torch.equal((Rs if over == "x" else X).cpu(), rb if over == "x" else xb)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("S, D, ldx", [(1, 1, 1), (7, 130, 130), (33, 2112, 4224), (2, 20000, 20000), (1000, 64, 67),
+                                       (5, 1088, 1088)])
+def test_rows(dtype, S, D, ldx):
+    g = torch.Generator().manual_seed(S * D)
+    xb = (torch.randn(S * ldx, generator=g) * torch.exp(3 * torch.randn(S * ldx, generator=g))).to(dtype)
+    X = xb.cuda()
+    q, s = buffers(S, D)
+    zz.rows_fp8_dev(X.data_ptr(), S, D, q.data_ptr(), s.data_ptr(), KIND[dtype], ldx=ldx, stream=stream())
+    qh, sh = taken(q, s, S, D)
+    R.check_rows(xb.view(S, ldx)[:, :D].double().numpy(), qh, sh, 0.0)
+
+
+def test_rows_at_the_edges():
+    """Zero blocks, values below the floor, the largest finite ones, subnormal codes; a NaN
+    and an infinity stay in their rows."""
+    x = torch.zeros(8, 256)
+    x[1, :] = 2.0 ** -130
+    x[2, :128] = torch.finfo(F32).max
+    x[3, 0], x[3, 1:] = 448.0, torch.linspace(2.0 ** -11, 2.0 ** -5, 255)
+    x[6] = 1.0
+    clean = x.double().numpy()
+    x[4, 5] = float("nan")
+    x[5, 9] = float("inf")
+    X = x.cuda()
+    q, s = buffers(8, 256)
+    zz.rows_fp8_dev(X.data_ptr(), 8, 256, q.data_ptr(), s.data_ptr(), stream=stream())
+    qh, sh = taken(q, s, 8, 256)
+    keep = [0, 1, 2, 3, 6, 7]
+    R.check_rows(clean[keep], qh[keep], sh[:, keep], 0.0)
+    v = R.e4m3_value(qh.numpy())
+    assert np.isnan(v[4, 5]) and not np.isnan(np.delete(v[4], 5)).any()
+    assert torch.isinf(sh[0, 5]) and np.isnan(v[5, 9]) and not np.isnan(v[5, 128:]).any()
+
+
+def coded(shape, seed, lo=0, hi=256):
+    """Codes of every finite kind."""
+    r = np.random.default_rng(seed)
+    c = r.integers(lo, hi, shape).astype(np.uint8)
+    return np.where((c & 127) == 127, 3, c).astype(np.uint8)
+
+
+def case(S, O, I, seed):
+    r = np.random.default_rng(seed)
+    xq = np.zeros((S, R.blocks(I) * 128), np.uint8)
+    xq[:, :I] = coded((S, I), seed)
+    xs = np.exp(r.normal(-5, 1, (R.blocks(I), S))).astype(np.float32)
+    wq = coded((O, I), seed + 1)
+    ws = np.exp(r.normal(-8, 1, (R.blocks(O), R.blocks(I)))).astype(np.float32)
+    return xq, xs, wq, ws
+
+
+# one of everything, ragged tiles in each direction, block edges of the matrix's scales, and
+# sizes on both sides of each choice between kernels
+SHAPES = [(1, 1, 1), (1, 16, 128), (2, 17, 129), (1, 2816, 2112), (3, 1000, 1088), (16, 129, 300), (17, 128, 2816),
+          (21, 1000, 1088), (33, 257, 511), (64, 704, 2816), (65, 2112, 640), (100, 130, 1000), (128, 256, 256),
+          (200, 1500, 700), (256, 512, 128), (300, 257, 1025), (513, 640, 2816), (700, 2816, 704), (1025, 300, 130)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("S, O, I", SHAPES)
+def test_product(dtype, S, O, I):
+    print("case", S, O, I, dtype, flush=True)
+    xq, xs, wq, ws = case(S, O, I, S + O + I)
+    m = zz.Fp8Matrix(O, I)
+    try:
+        m.upload(wq, ws)
+        Q, Sc = torch.from_numpy(xq).cuda(), torch.from_numpy(xs).cuda()
+        y = torch.full((S + 1, O), -3.0, dtype=dtype, device="cuda")
+        m.matmul_dev(Q.data_ptr(), Sc.data_ptr(), S, y.data_ptr(), KIND[dtype], stream=stream())
+        torch.cuda.synchronize()
+        assert bool((y[S] == -3.0).all())
+        want, mag = R.product(xq, xs, wq, ws, O, I)
+        got = y[:S].double().cpu().numpy()
+        off = np.abs(got - want)
+        assert np.all(off <= R.product_bound(mag, want, I, dtype)), (off / np.maximum(mag, 1e-300)).max()
+        again = torch.empty_like(y[:S])
+        m.matmul_dev(Q.data_ptr(), Sc.data_ptr(), S, again.data_ptr(), KIND[dtype], stream=stream())
+        torch.cuda.synchronize()
+        assert torch.equal(again, y[:S])
+    finally:
+        m.close()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("S, ldy, off", [(5, 133, 0), (40, 200, 1), (300, 136, 0), (300, 131, 3)])
+def test_product_strides(dtype, S, ldy, off):
+    O, I = 130, 200
+    xq, xs, wq, ws = case(S, O, I, 5)
+    m = zz.Fp8Matrix(O, I)
+    try:
+        D = [torch.from_numpy(a).cuda() for a in (xq, xs, wq, ws)]
+        torch.cuda.synchronize()
+        m.upload_dev(D[2].data_ptr(), D[3].data_ptr())
+        y = torch.full((S * ldy + off,), -3.0, dtype=dtype, device="cuda")
+        m.matmul_dev(D[0].data_ptr(), D[1].data_ptr(), S, y.data_ptr() + off * y.element_size(), KIND[dtype], ldy=ldy,
+                     stream=stream())
+        v = y[off:].view(S, ldy).double().cpu().numpy()
+        want, mag = R.product(xq, xs, wq, ws, O, I)
+        assert np.all(np.abs(v[:, :O] - want) <= R.product_bound(mag, want, I, dtype))
+        assert np.all(v[:, O:] == -3.0) and bool((y[:off] == -3.0).all())
+    finally:
+        m.close()
+
+
+def test_product_edges():
+    """Row independence (a NaN row, an infinite scale), the largest codes, a second upload, a
+    matrix without weights, and the host form."""
+    S, O, I = 37, 140, 260
+    xq, xs, wq, ws = case(S, O, I, 77)
+    m = zz.Fp8Matrix(O, I)
+    try:
+        Q, Sc = torch.from_numpy(xq).cuda(), torch.from_numpy(xs).cuda()
+        y = torch.full((S, O), -3.0, device="cuda")
+        with pytest.raises(RuntimeError, match="no weights"):
+            m.matmul_dev(Q.data_ptr(), Sc.data_ptr(), S, y.data_ptr(), stream=stream())
+        with pytest.raises(RuntimeError, match="no weights"):
+            m.matmul(np.ones((2, I), np.float32))
+        m.upload(wq, ws)
+        with pytest.raises(RuntimeError, match="closer"):
+            m.matmul_dev(Q.data_ptr(), Sc.data_ptr(), S, y.data_ptr(), ldy=O - 1, stream=stream())
+        with pytest.raises(RuntimeError, match="overlaps"):
+            m.matmul_dev(Q.data_ptr(), Sc.data_ptr(), S, Q.data_ptr(), stream=stream())
+        torch.cuda.synchronize()
+        assert bool((y == -3.0).all())
+        m.matmul_dev(Q.data_ptr(), Sc.data_ptr(), S, y.data_ptr(), stream=stream())
+        Q2, Sc2 = Q.clone(), Sc.clone()
+        Q2[3, 7] = 0x7F
+        Sc2[1, 20] = float("inf")
+        y2 = torch.empty_like(y)
+        m.matmul_dev(Q2.data_ptr(), Sc2.data_ptr(), S, y2.data_ptr(), stream=stream())
+        torch.cuda.synchronize()
+        other = [t for t in range(S) if t not in (3, 20)]
+        assert torch.equal(y2[other], y[other]) and bool(y2[3].isnan().all()) and not bool(y2[20].isfinite().any())
+        # 448 * 448 * I, exact in f32's 24 bits for one block
+        full = np.full((O, I), 0x7E, np.uint8)
+        m.upload(full, np.ones_like(ws))
+        Q.fill_(0)
+        Q[:, :I] = 0x7E
+        Sc.fill_(1.0)
+        m.matmul_dev(Q.data_ptr(), Sc.data_ptr(), S, y.data_ptr(), stream=stream())
+        torch.cuda.synchronize()
+        assert bool((y == 448.0 * 448.0 * I).all())
+        # the host form is the two device calls
+        m.upload(wq, ws)
+        x = np.random.default_rng(1).normal(size=(S, I)).astype(np.float32)
+        X = torch.from_numpy(x).cuda()
+        zz.rows_fp8_dev(X.data_ptr(), S, I, Q.data_ptr(), Sc.data_ptr(), stream=stream())
+        m.matmul_dev(Q.data_ptr(), Sc.data_ptr(), S, y.data_ptr(), stream=stream())
+        torch.cuda.synchronize()
+        assert np.array_equal(m.matmul(x), y.cpu().numpy())
+    finally:
+        m.close()
+
+
+def test_two_matrices_streams_and_graphs():
+    """Matrices beside each other on two streams, and a captured chain (norm, product, rows,
+    product) replayed with eager work between: every replay is the eager result."""
+    S, D, M = 19, 320, 200
+    a, b = zz.Fp8Matrix(M, D), zz.Fp8Matrix(D, M)
+    try:
+        _, _, wa, sa = case(1, M, D, 3)
+        _, _, wb, sb = case(1, D, M, 4)
+        a.upload(wa, sa)
+        b.upload(wb, sb)
+        g = torch.Generator(device="cuda").manual_seed(6)
+        w = torch.ones(D, device="cuda")
+
+        class Run:
+            def __init__(self):
+                self.x = torch.empty(S, D, device="cuda")
+                self.res = torch.empty(S, D, device="cuda")
+                self.q, self.s = torch.empty(S, 384, dtype=torch.uint8, device="cuda"), torch.empty(3, S, device="cuda")
+                self.h = torch.empty(S, M, dtype=BF16, device="cuda")
+                self.q2, self.s2 = torch.empty(S, 256, dtype=torch.uint8, device="cuda"), torch.empty(2, S, device="cuda")
+                self.sum, self.y = torch.empty(S, D, device="cuda"), torch.empty(S, D, device="cuda")
+
+            def __call__(self):
+                st = stream()
+                zz.add_norm_fp8_dev(self.x.data_ptr(), self.res.data_ptr(), self.sum.data_ptr(), w.data_ptr(), S, D,
+                                    1e-6, self.q.data_ptr(), self.s.data_ptr(), stream=st)
+                a.matmul_dev(self.q.data_ptr(), self.s.data_ptr(), S, self.h.data_ptr(), zz.ZZ_BF16, stream=st)
+                zz.rows_fp8_dev(self.h.data_ptr(), S, M, self.q2.data_ptr(), self.s2.data_ptr(), zz.ZZ_BF16, stream=st)
+                b.matmul_dev(self.q2.data_ptr(), self.s2.data_ptr(), S, self.y.data_ptr(), stream=st)
+
+        one, two, eager = Run(), Run(), Run()
+        graphs = []
+        torch.cuda.synchronize()
+        for r in (one, two):
+            gr = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(gr):
+                r()
+            graphs.append(gr)
+        side = [torch.cuda.Stream(), torch.cuda.Stream()]
+        for k in range(4):
+            for r in (one, two):
+                r.x.normal_(generator=g)
+                r.res.normal_(generator=g)
+            torch.cuda.synchronize()
+            for st, gr in zip(side, graphs):
+                with torch.cuda.stream(st):
+                    gr.replay()
+            torch.cuda.synchronize()
+            for r in (one, two):
+                eager.x.copy_(r.x)
+                eager.res.copy_(r.res)
+                eager()
+                torch.cuda.synchronize()
+                assert torch.equal(eager.y, r.y) and torch.equal(eager.sum, r.sum), k
+    finally:
+        a.close()
+        b.close()

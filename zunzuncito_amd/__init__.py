@@ -2,8 +2,9 @@
 
 The product is libzzmoe.so (HIP, gfx950), whose C ABI is include/zz_gpu.h (the
 engines' gpu.h, same symbols), include/zz_moe.h (the whole MoE block with
-experts resident in HBM) and include/zz_gemma.h (gemma's feed-forward block and
-tied embedding / lm_head around it). This module is a thin ctypes binding of that ABI for
+experts resident in HBM), include/zz_gemma.h (gemma's feed-forward block and
+tied embedding / lm_head around it), include/zz_fp8.h (8-bit floating-point rows
+and matrices) and include/zz_beam.h (beam search's step). This module is a thin ctypes binding of that ABI for
 Python callers, tests and the benchmark. There is no CPU fallback here: when the
 library is missing or no gfx950 device is present, calls raise.
 """
@@ -18,9 +19,11 @@ LIB_PATH = os.path.join(PKG_DIR, "libzzmoe.so")
 GPU_FMT_Q40, GPU_FMT_Q80, GPU_FMT_TQ2, GPU_FMT_Q4A = 1, 2, 3, 4
 ZZ_GATE_SOFTMAX_PES, ZZ_GATE_SIGMOID_BIAS, ZZ_GATE_SOFTMAX_TOPK, ZZ_GATE_DENSE = 0, 1, 2, 3
 ZZ_GATE_GROUPED = 4
+ZZ_F32, ZZ_BF16 = 0, 1
+ZZ_BEAM_MAXW, ZZ_BEAM_MAXV = 16, 524288
 ZZ_ACT_GEGLU_TANH, ZZ_ACT_SWIGLU, ZZ_ACT_SWIGLU_CLAMP = 0, 1, 2
 
-# Every symbol include/zz_gpu.h and include/zz_moe.h declare.
+# Every symbol the headers in include/ declare.
 ABI_SYMBOLS = (
     "gpu_init", "gpu_shutdown", "gpu_ready", "gpu_name", "gpu_map", "gpu_q40_matmul",
     "gpu_matmul", "zz_moe_layer_create", "zz_moe_layer_destroy", "zz_moe_record_bytes",
@@ -35,6 +38,9 @@ ABI_SYMBOLS = (
     "zz_stack_destroy", "zz_stack_prefill_dev", "zz_stack_decode_dev", "zz_moe_load_experts",
     "zz_gemma_stack_load", "zz_head_flash", "zz_head_use_flash", "zz_head_flash_replays",
     "zz_stack_use_flash", "zz_moe_forward_dev_noalloc", "zz_router_expf", "zz_gpu_map_refreshes", "zz_moe_dots",
+    "zz_fp8_row_bytes", "zz_add_norm_fp8_dev", "zz_rows_fp8_dev", "zz_fp8_create", "zz_fp8_destroy",
+    "zz_fp8_upload", "zz_fp8_upload_dev", "zz_fp8_matmul_dev", "zz_fp8_matmul",
+    "zz_beam_ws_bytes", "zz_beam_step_dev", "zz_beam_reorder_dev", "zz_stack_beam_dev",
 )
 KERNELS = ("prep", "logits", "topk", "dispatch", "ffn_up", "ffn_down", "combine", "dec_route",
            "dec_down")
@@ -135,6 +141,22 @@ def lib():
     L.zz_head_use_flash.argtypes = [C.c_int, C.c_int]
     L.zz_head_flash_replays.argtypes = [C.POINTER(C.c_uint)]
     L.zz_stack_use_flash.argtypes = [C.c_int, C.c_int]
+    p, i, l = C.c_void_p, C.c_int, C.c_int64
+    L.zz_fp8_row_bytes.restype = l
+    L.zz_fp8_row_bytes.argtypes = [l]
+    L.zz_add_norm_fp8_dev.argtypes = [i, p, l, p, l, p, l, p, C.c_float, i, i, p, p, p]
+    L.zz_rows_fp8_dev.argtypes = [i, p, l, i, i, p, p, p]
+    L.zz_fp8_create.argtypes = [i, i]
+    L.zz_fp8_destroy.argtypes = [i]
+    L.zz_fp8_upload.argtypes = [i, _u8p, _f32p]
+    L.zz_fp8_upload_dev.argtypes = [i, p, p]
+    L.zz_fp8_matmul_dev.argtypes = [i, p, p, i, i, p, l, p]
+    L.zz_fp8_matmul.argtypes = [i, _f32p, _f32p, i]
+    L.zz_beam_ws_bytes.restype = l
+    L.zz_beam_ws_bytes.argtypes = [i, i, i]
+    L.zz_beam_step_dev.argtypes = [i, p, l, i, i, i, p, p, i, i, p, p, p, p, p, C.c_size_t, p]
+    L.zz_beam_reorder_dev.argtypes = [p, p, p, i, i, l, l, l, l, p]
+    L.zz_stack_beam_dev.argtypes = [i, p, i, i, i, p, p, p]
     _lib = L
     return L
 
@@ -455,7 +477,100 @@ class Stack:
                                          1 if graph else 0, C.c_void_p(stream or None)):
             raise RuntimeError(f"zz_stack_decode_dev declined: {last_error()}")
 
+    def beam_dev(self, d_tok, W, n, d_seq, d_score, eos=-1, stream=0):
+        """Beam search of n steps from d_tok[0] (zz_stack_beam_dev): d_seq [W, n + 1] int32,
+        d_score [W] f32."""
+        if not lib().zz_stack_beam_dev(self.id, d_tok, W, n, eos, d_seq, d_score, stream or None):
+            raise RuntimeError(f"zz_stack_beam_dev declined: {last_error()}")
+
     def close(self):
         if self.id >= 0:
             lib().zz_stack_destroy(self.id)
             self.id = -1
+
+
+def fp8_row_bytes(D):
+    """Bytes of one row of D e4m3 codes: D up to whole blocks of 128."""
+    return lib().zz_fp8_row_bytes(D)
+
+
+def add_norm_fp8_dev(d_x, d_res, d_sum, d_w, S, D, eps, d_q, d_s, dtype=ZZ_F32, ldx=0, ldr=0, lds=0, stream=0):
+    """x + res, its RMS norm and the e4m3 rows of that (zz_add_norm_fp8_dev); device
+    pointers as ints, 0 for none (res, sum, w)."""
+    if not lib().zz_add_norm_fp8_dev(dtype, d_x or None, ldx, d_res or None, ldr, d_sum or None, lds, d_w or None,
+                                     eps, S, D, d_q or None, d_s or None, stream or None):
+        raise RuntimeError(f"zz_add_norm_fp8_dev declined: {last_error()}")
+
+
+def rows_fp8_dev(d_x, S, D, d_q, d_s, dtype=ZZ_F32, ldx=0, stream=0):
+    """The e4m3 rows of x (zz_rows_fp8_dev): codes [S, fp8_row_bytes(D)], scales
+    [ceil(D/128), S]."""
+    if not lib().zz_rows_fp8_dev(dtype, d_x or None, ldx, S, D, d_q or None, d_s or None, stream or None):
+        raise RuntimeError(f"zz_rows_fp8_dev declined: {last_error()}")
+
+
+class Fp8Matrix:
+    """A resident e4m3 matrix [O, I] with a scale per 128 x 128 block (zz_fp8_create)."""
+
+    def __init__(self, O, I):
+        self.O, self.I = O, I
+        self.id = lib().zz_fp8_create(O, I)
+        if self.id < 0:
+            raise RuntimeError(f"zz_fp8_create declined: {last_error()}")
+
+    def upload(self, codes, scales):
+        """Host codes uint8 [O, I] and scales f32 [ceil(O/128), ceil(I/128)]."""
+        codes = np.ascontiguousarray(codes, np.uint8)
+        scales = np.ascontiguousarray(scales, np.float32)
+        if codes.shape != (self.O, self.I) or scales.shape != (-(-self.O // 128), -(-self.I // 128)):
+            raise ValueError("codes [O, I] and scales [ceil(O/128), ceil(I/128)]")
+        if not lib().zz_fp8_upload(self.id, _p(codes, _u8p), _p(scales, _f32p)):
+            raise RuntimeError(f"zz_fp8_upload declined: {last_error()}")
+
+    def upload_dev(self, d_codes, d_scales):
+        if not lib().zz_fp8_upload_dev(self.id, d_codes or None, d_scales or None):
+            raise RuntimeError(f"zz_fp8_upload_dev declined: {last_error()}")
+
+    def matmul_dev(self, d_q, d_s, S, d_y, dtype=ZZ_F32, ldy=0, stream=0):
+        """y [S, O] of e4m3 rows [S, I] (zz_fp8_matmul_dev)."""
+        if not lib().zz_fp8_matmul_dev(self.id, d_q or None, d_s or None, S, dtype, d_y or None, ldy, stream or None):
+            raise RuntimeError(f"zz_fp8_matmul_dev declined: {last_error()}")
+
+    def matmul(self, x):
+        """Host x [S, I] f32, rounded to e4m3 rows, times the matrix; y [S, O]."""
+        x = np.ascontiguousarray(x, np.float32)
+        if x.ndim != 2 or x.shape[1] != self.I:
+            raise ValueError("x [S, I]")
+        y = np.zeros((x.shape[0], self.O), np.float32)
+        if not lib().zz_fp8_matmul(self.id, _p(x, _f32p), _p(y, _f32p), x.shape[0]):
+            raise RuntimeError(f"zz_fp8_matmul declined: {last_error()}")
+        return y
+
+    def close(self):
+        if self.id >= 0:
+            lib().zz_fp8_destroy(self.id)
+            self.id = -1
+
+
+def beam_ws_bytes(N, W, V):
+    """Workspace bytes of one beam_step_dev of these sizes."""
+    n = lib().zz_beam_ws_bytes(N, W, V)
+    if n < 0:
+        raise RuntimeError("zz_beam_ws_bytes declined: 1 <= W <= 16, 1 <= V <= 524288, N * W <= 65535")
+    return n
+
+
+def beam_step_dev(d_logits, N, W, V, d_score, d_score_out, d_parent, d_token, d_ws, ws_bytes, d_done=0,
+                  d_done_out=0, eos=-1, pad=0, dtype=ZZ_F32, ldl=0, stream=0):
+    """One step of beam search over logits [N*W, V] (zz_beam_step_dev)."""
+    if not lib().zz_beam_step_dev(dtype, d_logits or None, ldl, N, W, V, d_score or None, d_done or None, eos, pad,
+                                  d_score_out or None, d_parent or None, d_token or None, d_done_out or None,
+                                  d_ws or None, ws_bytes, stream or None):
+        raise RuntimeError(f"zz_beam_step_dev declined: {last_error()}")
+
+
+def beam_reorder_dev(d_dst, d_src, d_parent, N, W, outer=1, outer_stride=0, row_stride=0, row_bytes=0, stream=0):
+    """The beams' states in their parents' order (zz_beam_reorder_dev); d_dst may be d_src."""
+    if not lib().zz_beam_reorder_dev(d_dst or None, d_src or None, d_parent or None, N, W, outer, outer_stride,
+                                     row_stride, row_bytes, stream or None):
+        raise RuntimeError(f"zz_beam_reorder_dev declined: {last_error()}")

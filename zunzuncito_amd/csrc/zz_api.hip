@@ -1036,11 +1036,13 @@ extern "C" int zz_moe_stats(unsigned *c) {
 extern "C" const char *zz_last_error(void) { return g_err; }
 
 void zz_gemma_shutdown();   // zz_gemma.hip
+void zz_fp8_shutdown();     // zz_fp8.hip
 
 extern "C" void gpu_shutdown(void) {
     if (!g_ready) return;
     (void)hipStreamSynchronize(g_stream);
     zz_gemma_shutdown();
+    zz_fp8_shutdown();
     for (Layer *&L : g_layers) { free_layer(L); L = nullptr; }
     g_layers.clear();
     g_maps.clear([](const ZzRange &m) { (void)hipFree(m.dev); });

@@ -1,0 +1,93 @@
+// zz_fp8_dev.h -- what the 8-bit floating-point kernels share (zz_fp8_rows.hip,
+// zz_fp8_mma.hip) and their launchers.
+#pragma once
+#include "zz_common.h"
+
+#define ZZ_F8B 128                  // elements under one scale
+#define ZZ_F8MAX 448.0f             // largest e4m3 value
+#define ZZ_F8FLOOR 0x1p-100f        // a block's largest magnitude counts as at least this
+
+// element types of the unquantised side, as in include/zz_fp8.h
+struct zz_bf16 { uint16_t u; };
+
+__device__ __forceinline__ float zz_f32_of(float v) { return v; }
+__device__ __forceinline__ float zz_f32_of(zz_bf16 v) { return __uint_as_float((unsigned)v.u << 16); }
+
+// f32 -> bf16 bits, round to nearest even; a NaN stays one
+__device__ __forceinline__ unsigned zz_bf16_bits(float f) {
+    const unsigned u = __float_as_uint(f);
+    const unsigned r = (u + 0x7fffu + ((u >> 16) & 1u)) >> 16;
+    return (u & 0x7fffffffu) > 0x7f800000u ? (u >> 16) | 0x40u : r;
+}
+__device__ __forceinline__ void zz_put(float *p, float v) { *p = v; }
+__device__ __forceinline__ void zz_put(zz_bf16 *p, float v) { p->u = (uint16_t)zz_bf16_bits(v); }
+
+// n (<= 8) consecutive elements as f32, zero behind them. VEC: all 8 lie inside, at 16 bytes
+template <bool VEC, typename T>
+__device__ __forceinline__ void zz_get8(float (&v)[8], const T *p, int n) {
+    if (VEC && n >= 8) {
+        if constexpr (sizeof(T) == 4) {
+            const float4 a = *(const float4 *)p, b = *(const float4 *)(p + 4);
+            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+            v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+        } else {
+            const uint4 a = *(const uint4 *)p;
+            const unsigned w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                v[2 * j] = __uint_as_float(w[j] << 16);
+                v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+            }
+        }
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; j++) v[j] = j < n ? zz_f32_of(p[j]) : 0.0f;
+}
+template <bool VEC, typename T>
+__device__ __forceinline__ void zz_put8(T *p, const float (&v)[8], int n) {
+    if (VEC && n >= 8) {
+        if constexpr (sizeof(T) == 4) {
+            *(float4 *)p = make_float4(v[0], v[1], v[2], v[3]);
+            *(float4 *)(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
+        } else {
+            unsigned w[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) w[j] = zz_bf16_bits(v[2 * j]) | zz_bf16_bits(v[2 * j + 1]) << 16;
+            *(uint4 *)p = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; j++)
+        if (j < n) zz_put(p + j, v[j]);
+}
+
+struct ZzF8RowsArgs {
+    const void *x, *res;        // res, sum, w may be null
+    void *sum;
+    const float *w;
+    int64_t ldx, ldr, lds;      // elements
+    float eps;
+    int S, D, vec;              // vec: every full group of 8 lies at 16 bytes
+    uint8_t *q;                 // [S][nb * 128]
+    float *s;                   // [nb][S]
+};
+int zz_launch_add_norm_fp8(int dtype, const ZzF8RowsArgs &a, hipStream_t st);
+int zz_launch_rows_fp8(int dtype, const ZzF8RowsArgs &a, hipStream_t st);
+
+// A resident matrix: codes in 16-row groups, [O/16][nb][2][64 lanes][16 B], lane 16q + r of
+// half h holding row r's columns 64h + 16q .. + 15 of the block: what the lane's operands of
+// the block's four matrix-core steps are made of (step j: bytes 8 (j & 1) .. + 7 of half
+// j / 2). The steps' columns are in an order of their own, which the activation rows follow
+// and a dot product does not see. Rows from O and columns from I on are zero.
+struct ZzF8Mat {
+    int O, I;
+    const uint8_t *w;
+    const float *ws;            // [ceil(O/128)][nb]
+};
+__host__ __device__ __forceinline__ int zz_f8_nb(int n) { return (n + ZZ_F8B - 1) / ZZ_F8B; }
+
+int zz_launch_fp8_pack(const uint8_t *codes, int O, int I, uint8_t *dst, hipStream_t st);
+int zz_launch_fp8_matmul(const ZzF8Mat &m, const uint8_t *q, const float *s, int S, int dtype, void *y,
+                         int64_t ldy, hipStream_t st);

@@ -1,0 +1,123 @@
+// zz_fp8_rows.hip -- activation rows to e4m3 codes with an f32 scale per 128 elements
+// (include/zz_fp8.h), with the residual's addition and the RMS norm before it or without.
+//
+//   h = x + res;  r = 1 / sqrt(sum(h^2) / D + eps);  y = (h * r) * w
+//   per 128: a = max(max|y|, 2^-100), scale = a / 448, code = e4m3(y * (448 / a))
+// y * (448 / a) differs from y / scale by two roundings of f32, far below a code's step;
+// |y| <= a keeps it under 448 * (1 + 2^-22), which rounds to 448.
+//
+// A thread holds 8 consecutive elements: 16 lanes are one block, so its maximum is four DPP
+// steps and a code group one 8-byte store.
+#include "zz_fp8_dev.h"
+
+// 16 lanes' 8 values each -> their codes (two words) and the block's scale
+__device__ __forceinline__ uint2 zz_f8_block(const float (&y)[8], float *scale) {
+    float a = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; j++) a = fmaxf(a, fabsf(y[j]));
+    a = fmaxf(zz_group_max<16>(a), ZZ_F8FLOOR);
+    const float inv = ZZ_F8MAX / a;
+    *scale = a / ZZ_F8MAX;
+    int c[2];
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        int w = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * k] * inv, y[4 * k + 1] * inv, 0, false);
+        c[k] = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * k + 2] * inv, y[4 * k + 3] * inv, w, true);
+    }
+    return make_uint2((unsigned)c[0], (unsigned)c[1]);
+}
+
+// One workgroup per row, NU groups of 8 per thread held in registers between the sum of
+// squares and the codes: x and res are read once, sum and codes written once.
+template <typename T, int NU, bool VEC>
+__global__ __launch_bounds__(256) void zz_add_norm_fp8_kernel(ZzF8RowsArgs a) {
+    __shared__ double red[4];
+    const int row = blockIdx.x, tid = threadIdx.x, D = a.D, nb = zz_f8_nb(D);
+    const T *x = (const T *)a.x + row * a.ldx;
+    const T *res = a.res ? (const T *)a.res + row * a.ldr : nullptr;
+    T *sum = a.sum ? (T *)a.sum + row * a.lds : nullptr;
+    float h[NU][8];
+    float ss = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NU; i++) {
+        const int e = 8 * (i * 256 + tid);
+        zz_get8<VEC>(h[i], x + e, D - e);
+        if (res) {
+            float t[8];
+            zz_get8<VEC>(t, res + e, D - e);
+#pragma unroll
+            for (int j = 0; j < 8; j++) h[i][j] += t[j];
+        }
+#pragma unroll
+        for (int j = 0; j < 8; j++) ss = fmaf(h[i][j], h[i][j], ss);
+        if (sum && e < D) zz_put8<VEC>(sum + e, h[i], D - e);
+    }
+    // a thread's at most 32 squares in f32, the threads' sums in double
+    double t = zz_wave_sum((double)ss);
+    if ((tid & 63) == 0) red[tid >> 6] = t;
+    __syncthreads();
+    t = (red[0] + red[1]) + (red[2] + red[3]);
+    const float r = 1.0f / sqrtf((float)(t / D) + a.eps);
+#pragma unroll
+    for (int i = 0; i < NU; i++) {
+        const int e = 8 * (i * 256 + tid);
+        float w[8];
+        if (a.w) {
+            zz_get8<VEC>(w, a.w + e, D - e);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; j++) w[j] = 1.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; j++) h[i][j] = (h[i][j] * r) * w[j];
+        float sc;
+        const uint2 c = zz_f8_block(h[i], &sc);
+        if (e < nb * ZZ_F8B) {
+            *(uint2 *)(a.q + (size_t)row * nb * ZZ_F8B + e) = c;
+            if ((tid & 15) == 0) a.s[(size_t)(e / ZZ_F8B) * a.S + row] = sc;
+        }
+    }
+}
+
+// Blocks of rows without a norm: 16 lanes per block, 16 blocks per workgroup.
+template <typename T, bool VEC>
+__global__ __launch_bounds__(256) void zz_rows_fp8_kernel(ZzF8RowsArgs a) {
+    const int nb = zz_f8_nb(a.D), total = a.S * nb;
+    const int id = blockIdx.x * 16 + (threadIdx.x >> 4), m = threadIdx.x & 15;
+    const int at = id < total ? id : total - 1, row = at / nb, b = at - row * nb;
+    const int e = b * ZZ_F8B + 8 * m;
+    float v[8];
+    zz_get8<VEC>(v, (const T *)a.x + row * a.ldx + e, a.D - e);
+    float sc;
+    const uint2 c = zz_f8_block(v, &sc);
+    if (id >= total) return;
+    *(uint2 *)(a.q + (size_t)row * nb * ZZ_F8B + e) = c;
+    if (m == 0) a.s[(size_t)b * a.S + row] = sc;
+}
+
+template <typename T, bool VEC>
+static void launch_norm(const ZzF8RowsArgs &a, hipStream_t st) {
+    const int u = (zz_f8_nb(a.D) * 16 + 255) / 256;
+    const dim3 g(a.S), b(256);
+    if (u <= 1) hipLaunchKernelGGL((zz_add_norm_fp8_kernel<T, 1, VEC>), g, b, 0, st, a);
+    else if (u <= 2) hipLaunchKernelGGL((zz_add_norm_fp8_kernel<T, 2, VEC>), g, b, 0, st, a);
+    else hipLaunchKernelGGL((zz_add_norm_fp8_kernel<T, 4, VEC>), g, b, 0, st, a);
+}
+
+int zz_launch_add_norm_fp8(int dtype, const ZzF8RowsArgs &a, hipStream_t st) {
+    if (dtype == 0) a.vec ? launch_norm<float, true>(a, st) : launch_norm<float, false>(a, st);
+    else a.vec ? launch_norm<zz_bf16, true>(a, st) : launch_norm<zz_bf16, false>(a, st);
+    return hipGetLastError() == hipSuccess;
+}
+
+int zz_launch_rows_fp8(int dtype, const ZzF8RowsArgs &a, hipStream_t st) {
+    const dim3 g((unsigned)(((int64_t)a.S * zz_f8_nb(a.D) + 15) / 16)), b(256);
+    if (dtype == 0) {
+        if (a.vec) hipLaunchKernelGGL((zz_rows_fp8_kernel<float, true>), g, b, 0, st, a);
+        else hipLaunchKernelGGL((zz_rows_fp8_kernel<float, false>), g, b, 0, st, a);
+    } else {
+        if (a.vec) hipLaunchKernelGGL((zz_rows_fp8_kernel<zz_bf16, true>), g, b, 0, st, a);
+        else hipLaunchKernelGGL((zz_rows_fp8_kernel<zz_bf16, false>), g, b, 0, st, a);
+    }
+    return hipGetLastError() == hipSuccess;
+}

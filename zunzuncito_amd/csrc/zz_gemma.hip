@@ -10,6 +10,7 @@
 #include "zz_dot_dev.h"
 #include "zz_route_dev.h"
 #include "../../include/zz_gemma.h"
+#include "../../include/zz_beam.h"
 
 #include <math.h>
 #include <stdlib.h>
@@ -588,6 +589,8 @@ struct Stack {
     hipGraphExec_t exec = nullptr;  // one decode step, captured on first use
     unsigned long long gen = 0;     // zz_lib_mem_gen() the graph was captured at
     unsigned long long warm = 0;    // zz_lib_mem_gen() after the last eager step
+    char *beam = nullptr;           // a search's rows (zz_stack_beam_dev), one allocation
+    size_t beam_cap = 0;
     // what a container load created for this stack, destroyed with it
     std::vector<int> own_layers, own_blocks;
     int own_head = -1;
@@ -604,7 +607,7 @@ static void free_stack(Stack *k, bool owned = false) {
     }
     if (k->exec) (void)hipGraphExecDestroy(k->exec);
     if (k->graph) (void)hipGraphDestroy(k->graph);
-    void *ps[] = {k->h, k->alt, k->logits, k->cur};
+    void *ps[] = {k->h, k->alt, k->logits, k->cur, k->beam};
     for (void *p : ps)
         if (p) (void)hipFree(p);
     delete k;
@@ -780,6 +783,69 @@ extern "C" int zz_stack_decode_dev(int id, int *d_tok, int n, float *d_logits, i
     }
     if (d_logits && n > 0)
         ZZ_CHECK(hipMemcpyAsync(d_logits, k->logits, sizeof(float) * k->V, hipMemcpyDeviceToDevice, st));
+    return 1;
+}
+
+// ------------------------------------------------------------------ beam search
+// the search before its first step: beam 0 live at 0, the others at minus infinity
+__global__ __launch_bounds__(64) void zz_beam_begin_kernel(const int *first, int W, int64_t ld, int *seq, int *cur,
+                                                           float *score, uint8_t *done, int eos) {
+    const int w = threadIdx.x, t = first[0];
+    if (w >= W) return;
+    seq[w * ld] = t;
+    cur[w] = t;
+    score[w] = w == 0 ? 0.0f : -INFINITY;
+    done[w] = eos >= 0 && t == eos;
+}
+
+// the chosen tokens behind the histories, which the parents' order was given before
+__global__ __launch_bounds__(64) void zz_beam_append_kernel(const int *token, int W, int64_t ld, int at, int *seq,
+                                                            int *cur) {
+    const int w = threadIdx.x;
+    if (w >= W) return;
+    seq[w * ld + at] = token[w];
+    cur[w] = token[w];
+}
+
+extern "C" int zz_stack_beam_dev(int id, const int *d_tok, int W, int n, int eos, int *d_seq, float *d_score,
+                                 void *stream) {
+    Stack *k = get_stack(id);
+    if (!k || !d_tok || !d_seq || !d_score || W < 1 || W > ZZ_BEAM_MAXW || n < 0 || n > 1 << 24)
+        ZZ_FAIL("zz_stack_beam_dev: bad arguments (1 <= W <= %d, 0 <= n <= 2^24)", ZZ_BEAM_MAXW);
+    const int64_t wsb = zz_beam_ws_bytes(1, W, k->V);
+    if (wsb < 0) ZZ_FAIL("zz_stack_beam_dev: a vocabulary of %d is declined", k->V);
+    const int64_t ld = (int64_t)n + 1;
+    hipStream_t st = stream ? (hipStream_t)stream : zz_lib_stream();
+    // [rows W x D | logits W x V | tokens, parents, chosen, finished: 16 each | workspace]
+    const size_t rows = sizeof(float) * (size_t)W * k->D, lg = sizeof(float) * (size_t)W * k->V;
+    const size_t need = rows + lg + 256 + (size_t)wsb;
+    if (need > k->beam_cap) {
+        ZZ_CHECK(hipDeviceSynchronize());
+        if (k->beam) (void)hipFree(k->beam);
+        k->beam = nullptr;
+        k->beam_cap = 0;
+        zz_lib_mem_bump();
+        ZZ_CHECK(hipMalloc(&k->beam, need));
+        k->beam_cap = need;
+    }
+    float *h = (float *)k->beam, *logits = (float *)(k->beam + rows);
+    int *cur = (int *)(k->beam + rows + lg), *parent = cur + 16, *token = parent + 16;
+    uint8_t *done = (uint8_t *)(token + 16);
+    char *ws = (char *)(done + 64);
+    hipLaunchKernelGGL(zz_beam_begin_kernel, dim3(1), dim3(64), 0, st, d_tok, W, ld, d_seq, cur, d_score, done, eos);
+    for (int i = 0; i < n; i++) {
+        if (!zz_head_embed_dev(k->head, cur, W, h, st) || !stack_blocks(k, h, W, st)) return 0;
+        for (int w = 0; w < W; w += ZZ_DEC_MAXS) {
+            const int m = W - w < ZZ_DEC_MAXS ? W - w : ZZ_DEC_MAXS;
+            if (!zz_head_logits_dev(k->head, h + (size_t)w * k->D, m, logits + (size_t)w * k->V, nullptr, st)) return 0;
+        }
+        if (!zz_beam_step_dev(ZZ_F32, logits, 0, 1, W, k->V, d_score, done, eos, eos >= 0 ? eos : 0, d_score, parent,
+                              token, done, ws, (size_t)wsb, st))
+            return 0;
+        if (!zz_beam_reorder_dev(d_seq, d_seq, parent, 1, W, 1, 0, 4 * ld, 4 * ((int64_t)i + 1), st)) return 0;
+        hipLaunchKernelGGL(zz_beam_append_kernel, dim3(1), dim3(64), 0, st, token, W, ld, i + 1, d_seq, cur);
+    }
+    if (hipGetLastError() != hipSuccess) ZZ_FAIL("zz_stack_beam_dev: launch failed");
     return 1;
 }
 
