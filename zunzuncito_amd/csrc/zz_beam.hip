@@ -39,10 +39,22 @@ __device__ __forceinline__ double zz_unord64(zz_u64 u) {
     return __longlong_as_double((long long)((u >> 63) ? (u & 0x7fffffffffffffffull) : ~u));
 }
 // a candidate: the larger key is the better one; 0 is none (no float's bits order to 0)
-__device__ __forceinline__ zz_u64 zz_beam_key(float v, int t) { return ((zz_u64)zz_ord32(v) << 32) | (0xffffffffu - (unsigned)t); }
+// (minus zero is zero)
+__device__ __forceinline__ zz_u64 zz_beam_key(float v, int t) {
+    return ((zz_u64)zz_ord32(v + 0.0f) << 32) | (0xffffffffu - (unsigned)t);
+}
 
+// the wave's largest key: the upper words first, the lower ones only where several lanes share
+// the upper word (equal logits)
 __device__ __forceinline__ zz_u64 zz_wave_max64(zz_u64 v) {
-    return zz_group_reduce<64>(v, [](zz_u64 a, zz_u64 b) { return a > b ? a : b; });
+    const unsigned hi = (unsigned)(v >> 32), lo = (unsigned)v;
+    auto mx = [](unsigned a, unsigned b) { return a > b ? a : b; };
+    const unsigned H = zz_group_reduce<64>(hi, mx);
+    const zz_u64 at = __ballot(hi == H);
+    unsigned L;
+    if (__popcll(at) == 1) L = (unsigned)__builtin_amdgcn_readlane((int)lo, __ffsll((long long)at) - 1);
+    else L = zz_group_reduce<64>(hi == H ? lo : 0u, mx);
+    return ((zz_u64)H << 32) | L;
 }
 
 struct ZzBeamArgs {
@@ -56,9 +68,6 @@ struct ZzBeamArgs {
     uint8_t *done_out;              // may be null
     zz_u64 *ws;                     // [N*W][chunks][W + 1]: keys, then (maximum, sum)
 };
-
-// a logit as the step counts it: NaN is minus infinity, minus zero is zero
-__device__ __forceinline__ float zz_beam_logit(float v) { return v == v ? v + 0.0f : -INFINITY; }
 
 // NV pieces of 16 bytes a thread, piece i * 256 + tid of the chunk counted from the row's first
 // token: the sum's order does not depend on where the row lies, so equal rows have equal
@@ -102,31 +111,70 @@ __global__ __launch_bounds__(256) void zz_beam_part_kernel(ZzBeamArgs a) {
     float lm = -INFINITY;
 #pragma unroll
     for (int k = 0; k < NE; k++) {
-        v[k] = zz_beam_logit(v[k]);
+        v[k] = fmaxf(v[k], -INFINITY);                   // a NaN counts as minus infinity
         lm = fmaxf(lm, v[k]);
     }
     const float m = zz_wave_max(lm);
     float s = 0.0f;
+    if (fabsf(m) < 16384.0f) {
+        // 2^(v log2(e) - c), c = m log2(e) rounded; what c's rounding left is a common factor
+        const float c = m * ZZ_LOG2E, off = fmaf(m, ZZ_LOG2E, -c);
 #pragma unroll
-    for (int k = 0; k < NE; k++) {
-        // at an infinite maximum the difference would be NaN; padding is minus infinity and
-        // counts where the whole row is, whose sum is not used
-        const float e = v[k] == m ? 1.0f : __builtin_amdgcn_exp2f((v[k] - m) * ZZ_LOG2E);
-        s += e;
+        for (int k = 0; k < NE; k++) s += __builtin_amdgcn_exp2f(fmaf(v[k], ZZ_LOG2E, -c));
+        s *= __builtin_amdgcn_exp2f(-off);
+    } else if (fabsf(m) != INFINITY) {
+#pragma unroll
+        for (int k = 0; k < NE; k++) s += __builtin_amdgcn_exp2f((v[k] - m) * ZZ_LOG2E);
+    } else {
+        // the infinite logits share the probability; at minus infinity the sum is not used
+#pragma unroll
+        for (int k = 0; k < NE; k++) s += v[k] == m ? 1.0f : 0.0f;
     }
     s = zz_wave_sum(s);
-    // W rounds of the wave's largest remaining key
-    zz_u64 prev = ~0ull;
-    for (int k = 0; k < W; k++) {
-        zz_u64 b = 0;
+    // The W-th largest of the lanes' maxima: at least W logits reach it, and the W best do. What
+    // reaches it is a few more than W, unless many are equal.
+    float left = lm, line = m;
+    for (int k = 1; k < W; k++) {
+        const zz_u64 at = __ballot(left == line);
+        if (l == __ffsll((long long)at) - 1) left = -INFINITY;
+        line = zz_wave_max(left);
+    }
+    if (l < W) best[w][l] = 0;
+    cand[w][l] = 0;
+    int total = line == -INFINITY ? 65 : 0;              // padding would be among them
+    if (total == 0) {
 #pragma unroll
-        for (int j = 0; j < NE; j++) {
-            const int t = tok(j);
-            const zz_u64 key = t < 0 ? 0 : zz_beam_key(v[j], t);
-            if (key < prev && key > b) b = key;
+        for (int k = 0; k < NE; k++) {
+            const zz_u64 at = __ballot(v[k] >= line);
+            if (at) {
+                const int o = total + __builtin_amdgcn_mbcnt_hi((unsigned)(at >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)at, 0));
+                if (v[k] >= line && o < 64) cand[w][o] = zz_beam_key(v[k], tok(k));
+                total += __popcll(at);
+            }
         }
-        prev = zz_wave_max64(b);
-        if (l == 0) best[w][k] = prev;
+    }
+    if (total <= 64) {
+        // a candidate a lane: its place is the number of better ones
+        const zz_u64 key = cand[w][l];
+        int rank = 0;
+        for (int j = 0; j < total; j += 8)
+#pragma unroll
+            for (int i = 0; i < 8; i++) rank += cand[w][j + i] > key;
+        if (l < total && rank < W) best[w][rank] = key;
+    } else {
+        // W rounds of the wave's largest remaining key
+        zz_u64 prev = ~0ull;
+        for (int k = 0; k < W; k++) {
+            zz_u64 b = 0;
+#pragma unroll
+            for (int j = 0; j < NE; j++) {
+                const int t = tok(j);
+                const zz_u64 key = t < 0 ? 0 : zz_beam_key(v[j], t);
+                if (key < prev && key > b) b = key;
+            }
+            prev = zz_wave_max64(b);
+            if (l == 0) best[w][k] = prev;
+        }
     }
     if (l == 0) { wm[w] = m; wsum[w] = s; }
     __syncthreads();
@@ -135,7 +183,9 @@ __global__ __launch_bounds__(256) void zz_beam_part_kernel(ZzBeamArgs a) {
     const zz_u64 key = l < 4 * W ? best[l / W][l % W] : 0;
     cand[0][l] = key;
     int rank = 0;
-    for (int j = 0; j < 4 * W; j++) rank += cand[0][j] > key || (cand[0][j] == key && j < l);
+    for (int j = 0; j < 4 * W; j += 4)
+#pragma unroll
+        for (int i = 0; i < 4; i++) rank += cand[0][j + i] > key || (cand[0][j + i] == key && j + i < l);
     zz_u64 *out = a.ws + ((size_t)row * a.chunks + ch) * (W + 1);
     if (l < 4 * W && rank < W) out[rank] = key;
     if (l == 0) {
@@ -146,13 +196,23 @@ __global__ __launch_bounds__(256) void zz_beam_part_kernel(ZzBeamArgs a) {
     }
 }
 
+// Dynamic LDS: each row's lists and sums, as the workspace holds them.
 __global__ __launch_bounds__(1024) void zz_beam_merge_kernel(ZzBeamArgs a) {
+    extern __shared__ __attribute__((aligned(16))) zz_u64 lists[];
     __shared__ zz_u64 tot[ZZ_BEAM_MAXW][ZZ_BEAM_MAXW];      // ordered totals, 0: no candidate
     __shared__ int tk[ZZ_BEAM_MAXW][ZZ_BEAM_MAXW];
     __shared__ uint8_t fin[ZZ_BEAM_MAXW];
     const int n = blockIdx.x, w = zz_wave_id(), l = threadIdx.x & 63, W = a.W, row = n * W + w, C = a.chunks;
-    const bool done = a.done && a.done[row];
+    // everything that is read, before anything waits: a finished beam's lists mean nothing, and
+    // are not looked at
+    const int words = C * (W + 1);
+    zz_u64 *mine = lists + (size_t)w * words;
+    const zz_u64 *from = a.ws + (size_t)row * words;
+    const uint8_t flag = a.done ? a.done[row] : 0;
     float c = a.score[row];
+#pragma unroll 8
+    for (int i = l; i < words; i += 64) mine[i] = from[i];
+    const bool done = flag;
     if (c != c) c = -INFINITY;
     if (done) {
         if (l < W) {
@@ -160,12 +220,12 @@ __global__ __launch_bounds__(1024) void zz_beam_merge_kernel(ZzBeamArgs a) {
             tk[w][l] = a.pad;
         }
     } else {
-        const zz_u64 *p = a.ws + ((size_t)row * C + l) * (W + 1);
+        const zz_u64 *p = mine + l * (W + 1);
         const zz_u64 ms = l < C ? p[W] : 0;
         const float m = l < C ? __uint_as_float((unsigned)ms) : -INFINITY, M = zz_wave_max(m);
-        double s = l < C ? (double)__uint_as_float((unsigned)(ms >> 32)) : 0.0;
-        s *= m == M ? 1.0 : exp((double)m - (double)M);
-        s = zz_wave_sum(s);
+        float part = l < C ? __uint_as_float((unsigned)(ms >> 32)) : 0.0f;
+        if (m != M) part *= __builtin_amdgcn_exp2f((m - M) * ZZ_LOG2E);
+        const double s = zz_wave_sum((double)part);
         const double ls = log(s);
         // the chunks' sorted lists, one a lane: W times the largest head
         int at = 0;
@@ -211,6 +271,7 @@ __global__ __launch_bounds__(1024) void zz_beam_merge_kernel(ZzBeamArgs a) {
 // A thread owns one piece G of a row's bytes in all W rows of a sequence: it reads what
 // the W beams continue, then writes, so that moving in place needs no second buffer. Rows
 // that stay where they are move nothing in place.
+typedef unsigned zz_u4 __attribute__((ext_vector_type(4)));
 template <typename G, int WM>
 __global__ __launch_bounds__(256) void zz_beam_reorder_kernel(uint8_t *dst, const uint8_t *src, const int *parent, int W,
                                                               int64_t ostride, int64_t rstride, int64_t first,
@@ -240,16 +301,12 @@ __global__ __launch_bounds__(256) void zz_beam_reorder_kernel(uint8_t *dst, cons
 int zz_lib_here(const char *who);                                             // zz_fp8.hip
 int zz_ranges_meet(const void *a, int64_t n, const void *b, int64_t m);
 
-// 16-byte pieces a thread holds: 8 (f32 8192 elements a workgroup, bf16 16384), or 2 where
-// that leaves too few workgroups
-static int beam_pieces(int N, int W, int V, int dtype) {
-    const int per = dtype == ZZ_F32 ? 4 : 8;
-    const int64_t small = (V + 2 * 256 * per - 1) / (2 * 256 * per);
-    const int64_t wgs = (int64_t)N * W * ((V + 8 * 256 * per - 1) / (8 * 256 * per));
-    return small <= 64 && wgs < 512 ? 2 : 8;
+// elements a thread holds: 32 (8192 a workgroup), or 8 where that leaves too few workgroups
+static int beam_elems(int N, int W, int V) {
+    return V <= 64 * 2048 && (int64_t)N * W * ((V + 8191) / 8192) < 512 ? 8 : 32;
 }
-static int beam_chunks(int pieces, int V, int dtype) {
-    const int per = dtype == ZZ_F32 ? 4 : 8, c = pieces * 256 * per;
+static int beam_chunks(int N, int W, int V) {
+    const int c = 256 * beam_elems(N, W, V);
     return (V + c - 1) / c;
 }
 static int beam_sizes_ok(int N, int W, int V) {
@@ -258,12 +315,7 @@ static int beam_sizes_ok(int N, int W, int V) {
 
 extern "C" int64_t zz_beam_ws_bytes(int N, int W, int V) {
     if (!beam_sizes_ok(N, W, V)) return -1;
-    int c = 0;
-    for (int t : {ZZ_F32, ZZ_BF16}) {
-        const int k = beam_chunks(beam_pieces(N, W, V, t), V, t);
-        c = k > c ? k : c;
-    }
-    return (int64_t)N * W * c * (W + 1) * 8;
+    return (int64_t)N * W * beam_chunks(N, W, V) * (W + 1) * 8;
 }
 
 extern "C" int zz_beam_step_dev(int dtype, const void *d_logits, int64_t ldl, int N, int W, int V,
@@ -297,18 +349,18 @@ extern "C" int zz_beam_step_dev(int dtype, const void *d_logits, int64_t ldl, in
     }
     if (!zz_lib_here(who)) return 0;
     hipStream_t st = stream ? (hipStream_t)stream : zz_lib_stream();
-    const int np = beam_pieces(N, W, V, dtype);
-    ZzBeamArgs a{d_logits, ldl, N, W, V, beam_chunks(np, V, dtype), eos, pad, d_score, d_done, d_score_out, d_parent,
+    ZzBeamArgs a{d_logits, ldl, N, W, V, beam_chunks(N, W, V), eos, pad, d_score, d_done, d_score_out, d_parent,
                  d_token, d_done_out, (zz_u64 *)d_ws};
     const dim3 g(a.chunks, (unsigned)R), b(256);
+    const bool few = beam_elems(N, W, V) == 8;
     if (dtype == ZZ_F32) {
-        if (np == 2) hipLaunchKernelGGL((zz_beam_part_kernel<float, 2>), g, b, 0, st, a);
+        if (few) hipLaunchKernelGGL((zz_beam_part_kernel<float, 2>), g, b, 0, st, a);
         else hipLaunchKernelGGL((zz_beam_part_kernel<float, 8>), g, b, 0, st, a);
     } else {
-        if (np == 2) hipLaunchKernelGGL((zz_beam_part_kernel<zz_bf16, 2>), g, b, 0, st, a);
-        else hipLaunchKernelGGL((zz_beam_part_kernel<zz_bf16, 8>), g, b, 0, st, a);
+        if (few) hipLaunchKernelGGL((zz_beam_part_kernel<zz_bf16, 1>), g, b, 0, st, a);
+        else hipLaunchKernelGGL((zz_beam_part_kernel<zz_bf16, 4>), g, b, 0, st, a);
     }
-    hipLaunchKernelGGL(zz_beam_merge_kernel, dim3(N), dim3(64 * W), 0, st, a);
+    hipLaunchKernelGGL(zz_beam_merge_kernel, dim3(N), dim3(64 * W), (size_t)W * a.chunks * (W + 1) * 8, st, a);
     if (hipGetLastError() != hipSuccess) ZZ_FAIL("%s: launch failed", who);
     return 1;
 }
@@ -350,7 +402,7 @@ extern "C" int zz_beam_reorder_dev(void *d_dst, const void *d_src, const int *d_
     const uintptr_t al = (uintptr_t)d | (uintptr_t)s | (uintptr_t)row_stride | (outer > 1 ? (uintptr_t)outer_stride : 0);
     const int64_t gsz = al % 16 == 0 ? 16 : al % 4 == 0 ? 4 : 1, body = row_bytes / gsz, tail = row_bytes - body * gsz;
     if (body) {
-        if (gsz == 16) launch_reorder<uint4>(d, s, d_parent, N, W, outer, outer_stride, row_stride, 0, body, st);
+        if (gsz == 16) launch_reorder<zz_u4>(d, s, d_parent, N, W, outer, outer_stride, row_stride, 0, body, st);
         else if (gsz == 4) launch_reorder<unsigned>(d, s, d_parent, N, W, outer, outer_stride, row_stride, 0, body, st);
         else launch_reorder<uint8_t>(d, s, d_parent, N, W, outer, outer_stride, row_stride, 0, body, st);
     }
