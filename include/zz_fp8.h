@@ -63,7 +63,7 @@ int zz_fp8_upload_dev(int mat, const uint8_t *d_codes, const float *d_scales);
 /* y [S, O] = rows [S, I] times the matrix's transpose: for each block of 128 columns the
  * codes' product in f32, times the row's and the matrix block's scale, added up in f32 in
  * the order of the columns or of groups of them; rounded once to `dtype`. Rows of y are
- * ldy elements apart (0: O); what lies between them is left as it was. S <= 2^20. d_q is
+ * ldy elements apart (0: O); what lies between them is left as it was. S <= 2^20, S * O < 2^37. d_q is
  * aligned to 16 bytes. Results do not depend on other rows' values and are the same on
  * every call. */
 int zz_fp8_matmul_dev(int mat, const uint8_t *d_q, const float *d_s, int S, int dtype, void *d_y,

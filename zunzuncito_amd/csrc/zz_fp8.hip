@@ -111,7 +111,7 @@ struct Fp8Mat {
 };
 static std::vector<Fp8Mat *> g_mats;
 
-static size_t packed_bytes(const Fp8Mat *m) { return (size_t)((m->O + 15) / 16) * zz_f8_nb(m->I) * 2048; }
+static size_t packed_bytes(const Fp8Mat *m) { return (size_t)((m->O + 31) / 32) * zz_f8_nb(m->I) * 4096; }
 static size_t scale_count(const Fp8Mat *m) { return (size_t)zz_f8_nb(m->O) * zz_f8_nb(m->I); }
 
 static void free_mat(Fp8Mat *m) {
@@ -205,6 +205,7 @@ extern "C" int zz_fp8_matmul_dev(int id, const uint8_t *d_q, const float *d_s, i
     if (!m || !m->loaded) ZZ_FAIL("zz_fp8_matmul_dev: no such matrix, or it has no weights yet");
     if (!ldy) ldy = m->O;
     if (ldy < m->O) ZZ_FAIL("zz_fp8_matmul_dev: rows of y closer than their width");
+    if ((int64_t)S * m->O >= (int64_t)1 << 37) ZZ_FAIL("zz_fp8_matmul_dev: S * O < 2^37");
     const int64_t nq = S * zz_fp8_row_bytes(m->I), ns = (int64_t)zz_f8_nb(m->I) * S * 4, ny = span(ldy, S, m->O, esz);
     if (zz_ranges_meet(d_y, ny, d_q, nq) || zz_ranges_meet(d_y, ny, d_s, ns))
         ZZ_FAIL("zz_fp8_matmul_dev: y overlaps the rows");

@@ -76,9 +76,9 @@ struct ZzF8RowsArgs {
 int zz_launch_add_norm_fp8(int dtype, const ZzF8RowsArgs &a, hipStream_t st);
 int zz_launch_rows_fp8(int dtype, const ZzF8RowsArgs &a, hipStream_t st);
 
-// A resident matrix: codes in 16-row groups, [O/16][nb][2][64 lanes][16 B], lane 16q + r of
-// half h holding row r's columns 64h + 16q .. + 15 of the block: what the lane's operands of
-// the block's four matrix-core steps are made of (step j: bytes 8 (j & 1) .. + 7 of half
+// A resident matrix: codes in 32-row groups, [O/32][nb][4][64 lanes][16 B], lane 32h + r of
+// piece p holding row r's columns 32p + 16h .. + 15 of the block: what the lane's operands of
+// the block's eight matrix-core steps are made of (step j: bytes 8 (j & 1) .. + 7 of piece
 // j / 2). The steps' columns are in an order of their own, which the activation rows follow
 // and a dot product does not see. Rows from O and columns from I on are zero.
 struct ZzF8Mat {

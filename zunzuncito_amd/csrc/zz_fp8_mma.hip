@@ -9,15 +9,22 @@
 // 1e-4 of the terms' magnitude at worst, where the f16 form is 1e-8 and 2e-7 off. They would
 // run at twice the rate.
 //
-// A block of 128 columns is four v_mfma_f32_16x16x32_f16 of 16 matrix rows times 16
-// activation rows; each of the four results a lane then enters the f32 accumulator by one
-// fma with the two scales' product. Lane 16q + r of a result holds matrix rows 4q..4q+3 of
-// the group and activation row r, so a lane needs one row scale and a group one matrix scale.
+// A block of 128 columns is eight v_mfma_f32_32x32x16_f16 of 32 matrix rows times 32
+// activation rows; each of the 16 results a lane then enters the f32 accumulator by one fma
+// with the two scales' product. Lane 32h + r holds activation row r and the matrix rows
+// 8k + 4h .. + 3 (k = 0..3) of the group, so a lane needs one row scale and a group one matrix
+// scale. (The 16x16x32 form leaves 3 of 4 issue slots to the conversions and fma's beside it,
+// this one 7 of 8: with 3 vector operations for each 16 cycles of matrix work, as here, 24 and
+// 19 cycles were measured.)
 #include "zz_fp8_dev.h"
+#include <math.h>
+#ifdef ZZ_TUNE
+#include <stdlib.h>
+#endif
 
 typedef _Float16 zz_h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 zz_h8 __attribute__((ext_vector_type(8)));
-typedef float zz_v4f __attribute__((ext_vector_type(4)));
+typedef float zz_v16f __attribute__((ext_vector_type(16)));
 
 // 8 codes (two words) as f16: v_cvt_scalef32_pk_f16_fp8 at scale 1, exact, NaN stays NaN
 __device__ __forceinline__ zz_h8 zz_f8_half(unsigned a, unsigned b) {
@@ -27,17 +34,14 @@ __device__ __forceinline__ zz_h8 zz_f8_half(unsigned a, unsigned b) {
     const zz_h2 t = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)b, 1.0f, true);
     return zz_h8{p[0], p[1], q[0], q[1], r[0], r[1], t[0], t[1]};
 }
+// step e (0, 1) of a 16-byte piece
+__device__ __forceinline__ zz_h8 zz_f8_step(uint4 v, int e) { return e ? zz_f8_half(v.z, v.w) : zz_f8_half(v.x, v.y); }
 
-// the four steps' operands of a lane's two 16-byte pieces of a block
-struct ZzF8Frag { zz_h8 h[4]; };
-__device__ __forceinline__ ZzF8Frag zz_f8_frag(uint4 a, uint4 b) {
-    return {{zz_f8_half(a.x, a.y), zz_f8_half(a.z, a.w), zz_f8_half(b.x, b.y), zz_f8_half(b.z, b.w)}};
-}
-__device__ __forceinline__ zz_v4f zz_f8_mma(const ZzF8Frag &a, const ZzF8Frag &b) {
-    zz_v4f c = {0.0f, 0.0f, 0.0f, 0.0f};
+__device__ __forceinline__ zz_v16f zz_f8_zero() {
+    zz_v16f z;
 #pragma unroll
-    for (int j = 0; j < 4; j++) c = __builtin_amdgcn_mfma_f32_16x16x32_f16(a.h[j], b.h[j], c, 0, 0, 0);
-    return c;
+    for (int i = 0; i < 16; i++) z[i] = 0.0f;
+    return z;
 }
 
 // matrix rows o..o+3 of activation row t
@@ -55,6 +59,21 @@ __device__ __forceinline__ void zz_f8_store4(T *y, int64_t ldy, int t, int o, in
         if (o + i < O) zz_put(p + i, v[i]);
 }
 
+// 16 bytes of a result row, n of its elements inside the row
+template <typename T>
+__device__ __forceinline__ void zz_f8_store(T *p, const float (&v)[16 / sizeof(T)], int n, bool vec) {
+    constexpr int E = 16 / sizeof(T);
+    if (vec && n >= E) {
+        if constexpr (E == 4) *(float4 *)p = make_float4(v[0], v[1], v[2], v[3]);
+        else *(uint4 *)p = make_uint4(zz_bf16_bits(v[0]) | zz_bf16_bits(v[1]) << 16, zz_bf16_bits(v[2]) | zz_bf16_bits(v[3]) << 16,
+                                      zz_bf16_bits(v[4]) | zz_bf16_bits(v[5]) << 16, zz_bf16_bits(v[6]) | zz_bf16_bits(v[7]) << 16);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < E; i++)
+        if (i < n) zz_put(p + i, v[i]);
+}
+
 struct ZzF8Mm {
     ZzF8Mat m;
     const uint8_t *q;
@@ -64,32 +83,227 @@ struct ZzF8Mm {
     int64_t ldy;
 };
 
-// One workgroup per 16 matrix rows and 16 activation rows; its waves take every fourth
-// block and meet in LDS, where the partial sums are added in the waves' order. Rows behind
-// the last one are read as the last one, and not stored.
-template <typename T>
-__global__ __launch_bounds__(256) void zz_fp8_mm_kernel(ZzF8Mm a) {
-    __shared__ float part[4][64][4];
-    const int tid = threadIdx.x, w = zz_wave_id(), l = tid & 63, r = l & 15, qq = l >> 4;
-    const int g = blockIdx.x, t = blockIdx.y * 16 + r, tc = min(t, a.S - 1), nb = a.nb;
-    const uint8_t *wp = a.m.w + (size_t)g * nb * 2048 + l * 16;
-    const uint8_t *xp = a.q + (size_t)tc * nb * ZZ_F8B + 16 * qq;
-    const float *ws = a.m.ws + (size_t)(g / 8) * nb;
-    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int b = w; b < nb; b += 4) {
-        const uint4 w0 = *(const uint4 *)(wp + (size_t)b * 2048), w1 = *(const uint4 *)(wp + (size_t)b * 2048 + 1024);
-        const uint4 x0 = *(const uint4 *)(xp + b * ZZ_F8B), x1 = *(const uint4 *)(xp + b * ZZ_F8B + 64);
-        const float sc = a.s[(size_t)b * a.S + tc] * ws[b];
-        const zz_v4f p = zz_f8_mma(zz_f8_frag(w0, w1), zz_f8_frag(x0, x1));
+// Few rows: a workgroup per 32 matrix rows and 32 activation rows; its NW waves take every
+// NW-th block, the next one's codes requested before the current one is multiplied, and meet
+// in LDS, where the partial sums are added in the waves' order. Rows behind the last one are
+// read as the last one, and not stored.
+template <typename T, int NW>
+__global__ __launch_bounds__(64 * NW) void zz_fp8_few_kernel(ZzF8Mm a) {
+    __shared__ float part[NW][16][64];
+    const int tid = threadIdx.x, w = zz_wave_id(), l = tid & 63, r = l & 31, h = l >> 5, nb = a.nb;
+    const int g = blockIdx.x, t = blockIdx.y * 32 + r, tc = min(t, a.S - 1);
+    const uint8_t *wp = a.m.w + (size_t)g * nb * 4096 + l * 16;
+    const uint8_t *xp = a.q + (size_t)tc * nb * ZZ_F8B + 16 * h;
+    const float *ws = a.m.ws + (size_t)(g / 4) * nb, *sp = a.s + tc;
+    zz_v16f acc = zz_f8_zero();
+    uint4 wc[4], xc[4];
+    float sc = 0.0f;
+    auto load = [&](int b, uint4 (&W)[4], uint4 (&X)[4], float &s) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) acc[i] = fmaf(p[i], sc, acc[i]);
+        for (int p = 0; p < 4; p++) W[p] = *(const uint4 *)(wp + (size_t)b * 4096 + p * 1024);
+#pragma unroll
+        for (int p = 0; p < 4; p++) X[p] = *(const uint4 *)(xp + b * ZZ_F8B + p * 32);
+        s = sp[(size_t)b * a.S] * ws[b];
+    };
+    if (w < nb) load(w, wc, xc, sc);
+    for (int b = w; b < nb; b += NW) {
+        uint4 wn[4], xn[4];
+        float sn = 0.0f;
+        if (b + NW < nb) load(b + NW, wn, xn, sn);
+        zz_v16f p = zz_f8_zero();
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+            p = __builtin_amdgcn_mfma_f32_32x32x16_f16(zz_f8_step(wc[k >> 1], k & 1), zz_f8_step(xc[k >> 1], k & 1), p, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 16; i++) acc[i] = fmaf(p[i], sc, acc[i]);
+#pragma unroll
+        for (int i = 0; i < 4; i++) { wc[i] = wn[i]; xc[i] = xn[i]; }
+        sc = sn;
     }
-    *(float4 *)part[w][l] = make_float4(acc[0], acc[1], acc[2], acc[3]);
-    __syncthreads();
-    if (w == 0 && t < a.S) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) acc[i] = (part[0][l][i] + part[1][l][i]) + (part[2][l][i] + part[3][l][i]);
-        zz_f8_store4((T *)a.y, a.ldy, t, 16 * g + 4 * qq, a.m.O, a.vec, acc);
+    for (int i = 0; i < 16; i++) part[w][i][l] = acc[i];
+    __syncthreads();
+    if (w < 4 && t < a.S) {
+        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int q = 0; q < NW; q++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) v[i] += part[q][4 * w + i][l];
+        zz_f8_store4((T *)a.y, a.ldy, t, 32 * g + 8 * w + 4 * h, a.m.O, a.vec, v);
+    }
+}
+
+// 16 bytes (4 bytes) a lane from base + off straight into LDS at lds + 16 (4) * lane, counted
+// by vmcnt; no register receives anything. (m0 is named so that nothing of the compiler's is
+// kept in it; it warns that it never does.)
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+__device__ __forceinline__ void zz_dma16(const void *base, unsigned off, unsigned lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory", "m0");
+}
+__device__ __forceinline__ void zz_dma4(const void *base, unsigned off, unsigned lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory", "m0");
+}
+#pragma clang diagnostic pop
+template <int N>
+__device__ __forceinline__ void zz_wait_vm() {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+// Many rows: a workgroup owns a tile of 32*RO*WO matrix rows times 32*RS*WS activation rows.
+// KS groups of WO*WS waves take every KS-th block of 128 columns; a wave owns RO x RS tiles of
+// 32 x 32. Blocks arrive in LDS NS - 1 rounds ahead without passing registers: matrix codes in
+// operand order (a wave's read is one contiguous kilobyte), activation rows as they are, their
+// eight 16-byte pieces permuted by (row / 2) % 8 on the way in, so that 16 rows' reads meet 64
+// different banks. One barrier a round. Both operands are made f16 as they leave LDS.
+//
+// At 8192 x 4224 x 2816 (bf16 out) the 128 x 128 tile takes 195 us, 1.00 PFLOP/s; a library
+// f16 product of that shape takes 239 (225 in bf16). Of a round's 1.5 us (two workgroups a
+// CU), 0.85 are matrix work at 2.4 GHz; the clock is 2.0 to 2.2 GHz under it, and for each
+// matrix step a wave issues 3.25 vector operations in 16 cycles (two conversions, one fma).
+// Measured beside it and not better: codes through registers (209), 256 x 128 tiles (206),
+// f16 activations in LDS (217), a fma phase interleaved with the next tile's products (208),
+// touching later lines for the L2 (237). 33 x 64 tiles on 512 places leave the last of five
+// rounds an eighth full.
+template <int RO, int RS, int WO, int WS, int KS, int NS>
+struct ZzF8Async {
+    static constexpr int GW = WO * WS, NT = 64 * GW * KS, O = 32 * RO * WO, S = 32 * RS * WS;
+    static constexpr int WB = O * 128, XB = S * 128, SB = S * 4 < 256 ? 256 : S * 4, BLOCK = WB + XB + SB;
+    static constexpr int STAGE = KS * BLOCK, LDS = NS * STAGE;
+    static constexpr int WI = O / 8 / GW, XI = S / 8 / GW, DMA = WI + XI + 1;   // a wave's requests a block
+    static_assert(O / 8 % GW == 0 && S / 8 % GW == 0 && SB / 256 <= GW, "whole requests a wave");
+    static_assert(LDS >= O * S * 4, "the result's tile");
+};
+
+template <typename T, int RO, int RS, int WO, int WS, int KS, int NS>
+__global__ __launch_bounds__(64 * WO * WS * KS, 2) void zz_fp8_async_kernel(ZzF8Mm a) {
+    typedef ZzF8Async<RO, RS, WO, WS, KS, NS> C;
+    extern __shared__ __attribute__((aligned(1024))) char lds[];
+    const int tid = threadIdx.x, l = tid & 63, r = l & 31, h = l >> 5, nb = a.nb;
+    const int kg = zz_wave_id() / C::GW, w = zz_wave_id() % C::GW, wo = w % WO, ws = w / WO;
+    const int OT = (a.m.O + C::O - 1) / C::O, ST = (a.S + C::S - 1) / C::S;
+    constexpr int PW = 8;
+    const int id = (blockIdx.x % 8) * (gridDim.x / 8) + blockIdx.x / 8;
+    if (id >= OT * ST) return;
+    const int pan = id / (OT * PW), in = id - pan * OT * PW, pw = min(PW, ST - pan * PW);
+    const int ot = in / pw, st = pan * PW + in % pw;
+    const int gt = ot * WO * RO, g0 = gt + wo * RO, gl = (a.m.O + 31) / 32 - 1, t0 = st * C::S, last = a.S - 1 - t0;
+    const float *wsp = a.m.ws + (size_t)(min(g0, gl) / 4) * nb;
+    const unsigned lb = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char *)lds + kg * C::BLOCK;
+    // this wave's requests: matrix pieces w*WI .. (4 a group), row octets w*XI .., 64 scales
+    const uint8_t *wsrc[C::WI];
+#pragma unroll
+    for (int i = 0; i < C::WI; i++) {
+        const int pc = w * C::WI + i;
+        wsrc[i] = a.m.w + (size_t)min(gt + pc / 4, gl) * nb * 4096 + pc % 4 * 1024;
+    }
+    const uint8_t *xsrc = a.q + (size_t)t0 * nb * ZZ_F8B;
+    const float *ssrc = a.s + t0;
+    unsigned xo[C::XI];
+#pragma unroll
+    for (int i = 0; i < C::XI; i++)
+        xo[i] = (unsigned)min((w * C::XI + i) * 8 + (l >> 3), last) * nb * ZZ_F8B +
+                16 * ((l & 7) ^ ((((w * C::XI + i) & 1) << 2) | (l >> 4)));
+    constexpr int SI = C::SB / 256;
+    const unsigned so = 4 * (unsigned)min(w % SI * 64 + l, last);
+    auto fetch = [&](int it, int slot) {
+        const int b = min(it * KS + kg, nb - 1);          // behind the last block: its data, not used
+        const unsigned d = lb + slot * C::STAGE;
+#pragma unroll
+        for (int i = 0; i < C::WI; i++) zz_dma16(wsrc[i] + (size_t)b * 4096, l * 16, d + (w * C::WI + i) * 1024);
+#pragma unroll
+        for (int i = 0; i < C::XI; i++) zz_dma16(xsrc + (size_t)b * ZZ_F8B, xo[i], d + C::WB + (w * C::XI + i) * 1024);
+        zz_dma4(ssrc + (size_t)b * a.S, so, d + C::WB + C::XB + w % SI * 256);
+    };
+    zz_v16f acc[RO][RS];
+#pragma unroll
+    for (int i = 0; i < RO; i++)
+#pragma unroll
+        for (int j = 0; j < RS; j++) acc[i][j] = zz_f8_zero();
+    const int rounds = (nb + KS - 1) / KS;
+#pragma unroll
+    for (int i = 0; i < NS - 1; i++)
+        if (i < rounds) fetch(i, i);
+    int slot = 0, into = NS - 1;
+    for (int it = 0; it < rounds; it++) {
+        const int b = it * KS + kg;
+        const float wsc = b < nb ? wsp[b] : 0.0f;
+        // round it has arrived for this wave; behind the barrier, for all, and the one before it
+        // is read
+        if (it + NS - 2 < rounds) zz_wait_vm<C::DMA *(NS - 2)>();
+        else zz_wait_vm<0>();
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (it + NS - 1 < rounds) fetch(it + NS - 1, into);
+        const char *d = lds + slot * C::STAGE + kg * C::BLOCK;
+        slot = slot + 1 == NS ? 0 : slot + 1;
+        into = into + 1 == NS ? 0 : into + 1;
+        if (KS > 1 && b >= nb) continue;
+        float sc[RS];
+#pragma unroll
+        for (int j = 0; j < RS; j++) sc[j] = *(const float *)(d + C::WB + C::XB + 4 * ((ws * RS + j) * 32 + r)) * wsc;
+        zz_v16f p[RO][RS];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            uint4 wv[RO], xv[RS];
+#pragma unroll
+            for (int i = 0; i < RO; i++) wv[i] = *(const uint4 *)(d + ((wo * RO + i) * 4 + k) * 1024 + l * 16);
+#pragma unroll
+            for (int j = 0; j < RS; j++)
+                xv[j] = *(const uint4 *)(d + C::WB + ((ws * RS + j) * 32 + r) * 128 + 16 * ((2 * k + h) ^ ((r >> 1) & 7)));
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                zz_h8 wf[RO], xf[RS];
+#pragma unroll
+                for (int i = 0; i < RO; i++) wf[i] = zz_f8_step(wv[i], e);
+#pragma unroll
+                for (int j = 0; j < RS; j++) xf[j] = zz_f8_step(xv[j], e);
+#pragma unroll
+                for (int i = 0; i < RO; i++)
+#pragma unroll
+                    for (int j = 0; j < RS; j++)
+                        p[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(wf[i], xf[j], k || e ? p[i][j] : zz_f8_zero(), 0, 0, 0);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < RO; i++)
+#pragma unroll
+            for (int j = 0; j < RS; j++)
+#pragma unroll
+                for (int k = 0; k < 16; k++) acc[i][j][k] = fmaf(p[i][j][k], sc[j], acc[i][j][k]);
+    }
+    // The tile goes through LDS, [row][column] in 16-byte pieces (a row's pieces permuted by the
+    // row, for the banks), where the K groups are added in their order; then whole lines leave.
+    float *tile = (float *)lds;
+    auto place = [&](int t, int o) { return tile + t * C::O + 4 * ((((o >> 2) ^ t) & 7) | ((o >> 2) & ~7)); };
+#pragma unroll
+    for (int g = 0; g < KS; g++) {
+        __syncthreads();                                  // the last block, or the group before, is read
+        if (kg == g)
+#pragma unroll
+            for (int i = 0; i < RO; i++)
+#pragma unroll
+                for (int j = 0; j < RS; j++)
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        float4 *q = (float4 *)place((ws * RS + j) * 32 + r, (wo * RO + i) * 32 + 8 * k + 4 * h);
+                        float4 v = make_float4(acc[i][j][4 * k], acc[i][j][4 * k + 1], acc[i][j][4 * k + 2], acc[i][j][4 * k + 3]);
+                        if (g) {
+                            const float4 u = *q;
+                            v = make_float4(u.x + v.x, u.y + v.y, u.z + v.z, u.w + v.w);
+                        }
+                        *q = v;
+                    }
+    }
+    __syncthreads();
+    constexpr int E = 16 / sizeof(T), RL = C::O / E;      // elements a lane stores, lanes a row
+    for (int i = tid; i < C::S * RL; i += C::NT) {
+        const int t = i / RL, o = (i % RL) * E;
+        if (t > last) break;
+        float v[E];
+#pragma unroll
+        for (int e = 0; e < E; e += 4) *(float4 *)(v + e) = *(const float4 *)place(t, o + e);
+        zz_f8_store((T *)a.y + (int64_t)(t0 + t) * a.ldy + gt * 32 + o, v, a.m.O - gt * 32 - o, a.vec);
     }
 }
 
@@ -98,37 +312,103 @@ __global__ __launch_bounds__(256) void zz_fp8_pack_kernel(const uint8_t *src, in
                                                           int64_t n) {
     const int64_t p = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (p >= n) return;
-    const int l = (int)(p & 63), h = (int)(p >> 6) & 1;
-    const int64_t gb = p >> 7, g = gb / nb;
-    const int b = (int)(gb - g * nb), k = b * ZZ_F8B + 64 * h + 16 * (l >> 4);
-    const int64_t row = g * 16 + (l & 15);
+    const int l = (int)(p & 63), pc = (int)(p >> 6) & 3;
+    const int64_t gb = p >> 8, g = gb / nb;
+    const int b = (int)(gb - g * nb), k = b * ZZ_F8B + 32 * pc + 16 * (l >> 5);
+    const int64_t row = g * 32 + (l & 31);
     unsigned w[4] = {0, 0, 0, 0};
     if (row < O) {
         const uint8_t *s = src + row * I + k;
+        if (k + 16 <= I) {
+            __builtin_memcpy(w, s, 16);
+        } else {
 #pragma unroll
-        for (int j = 0; j < 16; j++)
-            if (k + j < I) w[j >> 2] |= (unsigned)s[j] << (8 * (j & 3));
+            for (int j = 0; j < 16; j++)
+                if (k + j < I) w[j >> 2] |= (unsigned)s[j] << (8 * (j & 3));
+        }
     }
     *(uint4 *)(dst + 16 * p) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 int zz_launch_fp8_pack(const uint8_t *codes, int O, int I, uint8_t *dst, hipStream_t st) {
     const int nb = zz_f8_nb(I);
-    const int64_t n = (int64_t)((O + 15) / 16) * nb * 128;
+    const int64_t n = (int64_t)((O + 31) / 32) * nb * 256;
     hipLaunchKernelGGL(zz_fp8_pack_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, codes, O, I, nb, dst, n);
     return hipGetLastError() == hipSuccess;
 }
 
+template <typename T, int RO, int RS, int WO, int WS, int KS, int NS>
+static bool launch_async(const ZzF8Mm &a, hipStream_t st) {
+    typedef ZzF8Async<RO, RS, WO, WS, KS, NS> C;
+    const int64_t n = ((int64_t)((a.m.O + C::O - 1) / C::O) * ((a.S + C::S - 1) / C::S) + 7) / 8 * 8;
+    if (n * C::NT > 0xffffffffll) return false;           // a launch's threads in one dimension
+    hipLaunchKernelGGL((zz_fp8_async_kernel<T, RO, RS, WO, WS, KS, NS>), dim3((unsigned)n), dim3(C::NT), C::LDS, st, a);
+    return true;
+}
+
+template <typename T, int NW>
+static bool launch_few(const ZzF8Mm &a, hipStream_t st) {
+    hipLaunchKernelGGL((zz_fp8_few_kernel<T, NW>), dim3((a.m.O + 31) / 32, (a.S + 31) / 32), dim3(64 * NW), 0, st, a);
+    return true;
+}
+
+// Which form: the one that is expected to take the shortest. A form's workgroups go round by
+// round through the 256 CUs, `per` of them on a CU at once; a round with k workgroups on the
+// busiest CU takes fix[k-1] + slope[k-1] * (blocks that a K group runs) microseconds, fitted to
+// 95 shapes (O 704 to 65536, I 256 to 8192, S 1 to 8192) with an rms error of 6 to 17 %. Over
+// them the choice lies 2 % behind the best form of each, 15 % at most; any one form for all
+// would be up to 5 times slower (1 x 4224 x 2816: 4.8 and 25 us for the first and last;
+// 4096 x 4224 x 2816: 295 and 109).
+struct ZzF8Form { int o, s, ks, per; float fix[4], slope[4]; };
+static const ZzF8Form mm_forms[] = {
+    {32, 32, 16, 1, {0.5f}, {2.1f}},
+    {32, 32, 4, 4, {2.5f, 2.3f, 2.6f, 0.7f}, {0.52f, 1.14f, 1.64f, 2.11f}},
+    {64, 32, 4, 1, {2.5f}, {0.97f}},
+    {64, 64, 4, 1, {3.5f}, {1.19f}},
+    {64, 64, 2, 2, {3.1f, 2.9f}, {0.79f, 1.19f}},
+    {64, 64, 1, 3, {2.8f, 3.9f, 2.1f}, {0.49f, 0.66f, 0.95f}},
+    {64, 128, 1, 3, {3.4f, 6.0f, 4.0f}, {0.74f, 0.96f, 1.49f}},
+    {128, 128, 1, 2, {4.5f, 7.8f}, {1.04f, 1.59f}},
+};
+static int mm_plan(int O, int S, int nb) {
+    int best = 0;
+    float least = INFINITY;
+    for (int v = 0; v < (int)(sizeof mm_forms / sizeof *mm_forms); v++) {
+        const ZzF8Form &f = mm_forms[v];
+        const int64_t n = (int64_t)((O + f.o - 1) / f.o) * ((S + f.s - 1) / f.s);
+        const int r = (nb + f.ks - 1) / f.ks, cap = 256 * f.per, rem = (int)(n % cap);
+        float t = (float)(n / cap) * (f.fix[f.per - 1] + f.slope[f.per - 1] * r);
+        if (rem) t += f.fix[(rem - 1) / 256] + f.slope[(rem - 1) / 256] * r;
+        if (t < least) {
+            least = t;
+            best = v;
+        }
+    }
+    return best;
+}
+
 template <typename T>
-static void launch_mm(const ZzF8Mm &a, hipStream_t st) {
-    hipLaunchKernelGGL(zz_fp8_mm_kernel<T>, dim3((a.m.O + 15) / 16, (a.S + 15) / 16), dim3(256), 0, st, a);
+static bool launch_mm(const ZzF8Mm &a, hipStream_t st) {
+#ifdef ZZ_TUNE
+    const char *e = getenv("ZZ_TILE");
+    const int v = e && atoi(e) >= 0 ? atoi(e) : mm_plan(a.m.O, a.S, a.nb);
+#else
+    const int v = mm_plan(a.m.O, a.S, a.nb);
+#endif
+    if (v == 0) return launch_few<T, 16>(a, st);
+    if (v == 1) return launch_few<T, 4>(a, st);
+    if (v == 2) return launch_async<T, 1, 1, 2, 1, 4, 2>(a, st);
+    if (v == 3) return launch_async<T, 1, 1, 2, 2, 4, 2>(a, st);
+    if (v == 4) return launch_async<T, 1, 1, 2, 2, 2, 2>(a, st);
+    if (v == 5) return launch_async<T, 1, 1, 2, 2, 1, 3>(a, st);
+    if (v == 6) return launch_async<T, 1, 2, 2, 2, 1, 2>(a, st);
+    return launch_async<T, 2, 2, 2, 2, 1, 2>(a, st);
 }
 
 int zz_launch_fp8_matmul(const ZzF8Mat &m, const uint8_t *q, const float *s, int S, int dtype, void *y,
                          int64_t ldy, hipStream_t st) {
     const int esz = dtype == 0 ? 4 : 2;
     ZzF8Mm a{m, q, s, S, zz_f8_nb(m.I), 0, y, ldy};
-    a.vec = (uintptr_t)y % (4 * esz) == 0 && ldy % 4 == 0;
-    dtype == 0 ? launch_mm<float>(a, st) : launch_mm<zz_bf16>(a, st);
-    return hipGetLastError() == hipSuccess;
+    a.vec = (uintptr_t)y % 16 == 0 && ldy * esz % 16 == 0;
+    return (dtype == 0 ? launch_mm<float>(a, st) : launch_mm<zz_bf16>(a, st)) && hipGetLastError() == hipSuccess;
 }
