@@ -44,17 +44,23 @@ __device__ __forceinline__ void zz_get8(float (&v)[8], const T *p, int n) {
 #pragma unroll
     for (int j = 0; j < 8; j++) v[j] = j < n ? zz_f32_of(p[j]) : 0.0f;
 }
+typedef unsigned zz_u4 __attribute__((ext_vector_type(4)));
+// nt: stores that are not kept in the caches
 template <bool VEC, typename T>
-__device__ __forceinline__ void zz_put8(T *p, const float (&v)[8], int n) {
+__device__ __forceinline__ void zz_put8(T *p, const float (&v)[8], int n, bool nt) {
     if (VEC && n >= 8) {
+        zz_u4 w[sizeof(T) / 2];
         if constexpr (sizeof(T) == 4) {
-            *(float4 *)p = make_float4(v[0], v[1], v[2], v[3]);
-            *(float4 *)(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
-        } else {
-            unsigned w[4];
 #pragma unroll
-            for (int j = 0; j < 4; j++) w[j] = zz_bf16_bits(v[2 * j]) | zz_bf16_bits(v[2 * j + 1]) << 16;
-            *(uint4 *)p = make_uint4(w[0], w[1], w[2], w[3]);
+            for (int j = 0; j < 8; j++) w[j >> 2][j & 3] = __float_as_uint(v[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++) w[0][j] = zz_bf16_bits(v[2 * j]) | zz_bf16_bits(v[2 * j + 1]) << 16;
+        }
+#pragma unroll
+        for (int j = 0; j < (int)(sizeof(T) / 2); j++) {
+            if (nt) __builtin_nontemporal_store(w[j], (zz_u4 *)p + j);
+            else ((zz_u4 *)p)[j] = w[j];
         }
         return;
     }
@@ -63,6 +69,11 @@ __device__ __forceinline__ void zz_put8(T *p, const float (&v)[8], int n) {
         if (j < n) zz_put(p + j, v[j]);
 }
 
+// An output of at least this many bytes, a quarter of the 256 MB cache in front of memory, is
+// stored past it: who reads it next finds little of it there, and its dirty lines would be
+// written back under the next kernels' reads.
+#define ZZ_NT_BYTES ((int64_t)64 << 20)
+
 struct ZzF8RowsArgs {
     const void *x, *res;        // res, sum, w may be null
     void *sum;
@@ -70,6 +81,7 @@ struct ZzF8RowsArgs {
     int64_t ldx, ldr, lds;      // elements
     float eps;
     int S, D, vec;              // vec: every full group of 8 lies at 16 bytes
+    int nt;                     // the sum is stored past the caches
     uint8_t *q;                 // [S][nb * 128]
     float *s;                   // [nb][S]
 };

@@ -27,6 +27,8 @@ __device__ __forceinline__ uint2 zz_f8_block(const float (&y)[8], float *scale) 
     return make_uint2((unsigned)c[0], (unsigned)c[1]);
 }
 
+// 8192 x 2816 in f32 take 58 us, 5.2 TB/s, which is what a large copy reaches (63 with the sum
+// kept in the caches); one row 3.3 us, a launch's 2.2 and one trip to memory.
 // One workgroup per row, NU groups of 8 per thread held in registers between the sum of
 // squares and the codes: x and res are read once, sum and codes written once.
 template <typename T, int NU, bool VEC>
@@ -50,7 +52,7 @@ __global__ __launch_bounds__(256) void zz_add_norm_fp8_kernel(ZzF8RowsArgs a) {
         }
 #pragma unroll
         for (int j = 0; j < 8; j++) ss = fmaf(h[i][j], h[i][j], ss);
-        if (sum && e < D) zz_put8<VEC>(sum + e, h[i], D - e);
+        if (sum && e < D) zz_put8<VEC>(sum + e, h[i], D - e, a.nt);
     }
     // a thread's at most 32 squares in f32, the threads' sums in double
     double t = zz_wave_sum((double)ss);
