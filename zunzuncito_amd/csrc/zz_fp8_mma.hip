@@ -83,52 +83,92 @@ struct ZzF8Mm {
     int64_t ldy;
 };
 
-// Few rows: a workgroup per 32 matrix rows and 32 activation rows; its NW waves take every
-// NW-th block, the next one's codes requested before the current one is multiplied, and meet
-// in LDS, where the partial sums are added in the waves' order. Rows behind the last one are
-// read as the last one, and not stored.
-template <typename T, int NW>
+// Few rows: a workgroup per RG groups of 32 matrix rows and RS tiles of 32 activation rows;
+// its NW waves take every NW-th block, straight from memory into registers (PF: the next one's
+// codes requested before the current one is multiplied), and meet in LDS, where the partial
+// sums are added in the waves' order. Rows behind the last one are read as the last one, and
+// not stored.
+template <typename T, int RG, int RS, int NW, bool PF>
 __global__ __launch_bounds__(64 * NW) void zz_fp8_few_kernel(ZzF8Mm a) {
-    __shared__ float part[NW][16][64];
+    extern __shared__ __attribute__((aligned(16))) float part[];     // [NW][RG][RS][16][64]
     const int tid = threadIdx.x, w = zz_wave_id(), l = tid & 63, r = l & 31, h = l >> 5, nb = a.nb;
-    const int g = blockIdx.x, t = blockIdx.y * 32 + r, tc = min(t, a.S - 1);
-    const uint8_t *wp = a.m.w + (size_t)g * nb * 4096 + l * 16;
-    const uint8_t *xp = a.q + (size_t)tc * nb * ZZ_F8B + 16 * h;
-    const float *ws = a.m.ws + (size_t)(g / 4) * nb, *sp = a.s + tc;
-    zz_v16f acc = zz_f8_zero();
-    uint4 wc[4], xc[4];
-    float sc = 0.0f;
-    auto load = [&](int b, uint4 (&W)[4], uint4 (&X)[4], float &s) {
+    const int g0 = blockIdx.x * RG, gl = (a.m.O + 31) / 32 - 1, t0 = blockIdx.y * 32 * RS;
+    const uint8_t *wp[RG], *xp[RS];
+    const float *ws = a.m.ws + (size_t)(g0 / 4) * nb, *sp[RS];
 #pragma unroll
-        for (int p = 0; p < 4; p++) W[p] = *(const uint4 *)(wp + (size_t)b * 4096 + p * 1024);
+    for (int i = 0; i < RG; i++) wp[i] = a.m.w + (size_t)min(g0 + i, gl) * nb * 4096 + l * 16;
 #pragma unroll
-        for (int p = 0; p < 4; p++) X[p] = *(const uint4 *)(xp + b * ZZ_F8B + p * 32);
-        s = sp[(size_t)b * a.S] * ws[b];
-    };
-    if (w < nb) load(w, wc, xc, sc);
-    for (int b = w; b < nb; b += NW) {
-        uint4 wn[4], xn[4];
-        float sn = 0.0f;
-        if (b + NW < nb) load(b + NW, wn, xn, sn);
-        zz_v16f p = zz_f8_zero();
-#pragma unroll
-        for (int k = 0; k < 8; k++)
-            p = __builtin_amdgcn_mfma_f32_32x32x16_f16(zz_f8_step(wc[k >> 1], k & 1), zz_f8_step(xc[k >> 1], k & 1), p, 0, 0, 0);
-#pragma unroll
-        for (int i = 0; i < 16; i++) acc[i] = fmaf(p[i], sc, acc[i]);
-#pragma unroll
-        for (int i = 0; i < 4; i++) { wc[i] = wn[i]; xc[i] = xn[i]; }
-        sc = sn;
+    for (int j = 0; j < RS; j++) {
+        const int t = min(t0 + 32 * j + r, a.S - 1);
+        xp[j] = a.q + (size_t)t * nb * ZZ_F8B + 16 * h;
+        sp[j] = a.s + t;
     }
+    zz_v16f acc[RG][RS];
 #pragma unroll
-    for (int i = 0; i < 16; i++) part[w][i][l] = acc[i];
+    for (int i = 0; i < RG; i++)
+#pragma unroll
+        for (int j = 0; j < RS; j++) acc[i][j] = zz_f8_zero();
+    struct Block { uint4 w[RG][4], x[RS][4]; float s[RS]; };
+    auto load = [&](int b, Block &B) {
+#pragma unroll
+        for (int i = 0; i < RG; i++)
+#pragma unroll
+            for (int p = 0; p < 4; p++) B.w[i][p] = *(const uint4 *)(wp[i] + (size_t)b * 4096 + p * 1024);
+#pragma unroll
+        for (int j = 0; j < RS; j++) {
+#pragma unroll
+            for (int p = 0; p < 4; p++) B.x[j][p] = *(const uint4 *)(xp[j] + b * ZZ_F8B + p * 32);
+            B.s[j] = sp[j][(size_t)b * a.S];
+        }
+    };
+    Block c;
+    if (w < nb) load(w, c);
+    for (int b = w; b < nb; b += NW) {
+        Block n;
+        if (PF && b + NW < nb) load(b + NW, n);
+        const float wsc = ws[b];
+        zz_v16f p[RG][RS];
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            zz_h8 wf[RG], xf[RS];
+#pragma unroll
+            for (int i = 0; i < RG; i++) wf[i] = zz_f8_step(c.w[i][k >> 1], k & 1);
+#pragma unroll
+            for (int j = 0; j < RS; j++) xf[j] = zz_f8_step(c.x[j][k >> 1], k & 1);
+#pragma unroll
+            for (int i = 0; i < RG; i++)
+#pragma unroll
+                for (int j = 0; j < RS; j++)
+                    p[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(wf[i], xf[j], k ? p[i][j] : zz_f8_zero(), 0, 0, 0);
+        }
+        float sc[RS];
+#pragma unroll
+        for (int j = 0; j < RS; j++) sc[j] = c.s[j] * wsc;
+        if (PF) c = n;
+        else if (b + NW < nb) load(b + NW, c);
+#pragma unroll
+        for (int i = 0; i < RG; i++)
+#pragma unroll
+            for (int j = 0; j < RS; j++)
+#pragma unroll
+                for (int k = 0; k < 16; k++) acc[i][j][k] = fmaf(p[i][j][k], sc[j], acc[i][j][k]);
+    }
+    constexpr int TL = RG * RS * 16 * 64;                 // a wave's partial sums
+#pragma unroll
+    for (int i = 0; i < RG; i++)
+#pragma unroll
+        for (int j = 0; j < RS; j++)
+#pragma unroll
+            for (int k = 0; k < 16; k++) part[w * TL + ((i * RS + j) * 16 + k) * 64 + l] = acc[i][j][k];
     __syncthreads();
-    if (w < 4 && t < a.S) {
+    for (int q = w; q < RG * RS * 4; q += NW) {           // four matrix rows of a tile a wave
+        const int i = q / (RS * 4), j = q / 4 % RS, k = q % 4, t = t0 + 32 * j + r;
+        if (t >= a.S) continue;
         float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int q = 0; q < NW; q++)
+        for (int u = 0; u < NW; u++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) v[i] += part[q][4 * w + i][l];
-        zz_f8_store4((T *)a.y, a.ldy, t, 32 * g + 8 * w + 4 * h, a.m.O, a.vec, v);
+            for (int e = 0; e < 4; e++) v[e] += part[u * TL + ((i * RS + j) * 16 + 4 * k + e) * 64 + l];
+        zz_f8_store4((T *)a.y, a.ldy, t, 32 * (g0 + i) + 8 * k + 4 * h, a.m.O, a.vec, v);
     }
 }
 
@@ -346,26 +386,27 @@ static bool launch_async(const ZzF8Mm &a, hipStream_t st) {
     return true;
 }
 
-template <typename T, int NW>
+template <typename T, int RG, int RS, int NW, bool PF>
 static bool launch_few(const ZzF8Mm &a, hipStream_t st) {
-    hipLaunchKernelGGL((zz_fp8_few_kernel<T, NW>), dim3((a.m.O + 31) / 32, (a.S + 31) / 32), dim3(64 * NW), 0, st, a);
+    const dim3 g((a.m.O + 32 * RG - 1) / (32 * RG), (a.S + 32 * RS - 1) / (32 * RS));
+    hipLaunchKernelGGL((zz_fp8_few_kernel<T, RG, RS, NW, PF>), g, dim3(64 * NW), NW * RG * RS * 4096, st, a);
     return true;
 }
 
 // Which form: the one that is expected to take the shortest. A form's workgroups go round by
 // round through the 256 CUs, `per` of them on a CU at once; a round with k workgroups on the
 // busiest CU takes fix[k-1] + slope[k-1] * (blocks that a K group runs) microseconds, fitted to
-// 95 shapes (O 704 to 65536, I 256 to 8192, S 1 to 8192) with an rms error of 6 to 17 %. Over
-// them the choice lies 2 % behind the best form of each, 15 % at most; any one form for all
-// would be up to 5 times slower (1 x 4224 x 2816: 4.8 and 25 us for the first and last;
-// 4096 x 4224 x 2816: 295 and 109).
+// 89 shapes (O 704 to 65536, I 256 to 8192, S 1 to 8192) with an rms error of 6 to 17 %. Over
+// them the choice lies 2 % behind the best form of each, and up to 15 %. Any one form for all
+// loses far more: the first and the last take 4.8 and 25.6 us for 1 x 4224 x 2816, 295 and 109
+// for 4096 rows.
 struct ZzF8Form { int o, s, ks, per; float fix[4], slope[4]; };
 static const ZzF8Form mm_forms[] = {
-    {32, 32, 16, 1, {0.5f}, {2.1f}},
-    {32, 32, 4, 4, {2.5f, 2.3f, 2.6f, 0.7f}, {0.52f, 1.14f, 1.64f, 2.11f}},
-    {64, 32, 4, 1, {2.5f}, {0.97f}},
-    {64, 64, 4, 1, {3.5f}, {1.19f}},
-    {64, 64, 2, 2, {3.1f, 2.9f}, {0.79f, 1.19f}},
+    {32, 32, 16, 1, {1.9f}, {2.0f}},
+    {32, 32, 4, 4, {2.9f, 2.3f, 2.6f, 0.7f}, {0.52f, 1.14f, 1.64f, 2.11f}},
+    {64, 32, 8, 1, {2.6f}, {1.4f}},
+    {64, 64, 4, 1, {3.4f}, {1.14f}},
+    {64, 64, 2, 2, {3.0f, 2.8f}, {0.82f, 1.14f}},
     {64, 64, 1, 3, {2.8f, 3.9f, 2.1f}, {0.49f, 0.66f, 0.95f}},
     {64, 128, 1, 3, {3.4f, 6.0f, 4.0f}, {0.74f, 0.96f, 1.49f}},
     {128, 128, 1, 2, {4.5f, 7.8f}, {1.04f, 1.59f}},
@@ -395,11 +436,11 @@ static bool launch_mm(const ZzF8Mm &a, hipStream_t st) {
 #else
     const int v = mm_plan(a.m.O, a.S, a.nb);
 #endif
-    if (v == 0) return launch_few<T, 16>(a, st);
-    if (v == 1) return launch_few<T, 4>(a, st);
-    if (v == 2) return launch_async<T, 1, 1, 2, 1, 4, 2>(a, st);
-    if (v == 3) return launch_async<T, 1, 1, 2, 2, 4, 2>(a, st);
-    if (v == 4) return launch_async<T, 1, 1, 2, 2, 2, 2>(a, st);
+    if (v == 0) return launch_few<T, 1, 1, 16, false>(a, st);
+    if (v == 1) return launch_few<T, 1, 1, 4, true>(a, st);
+    if (v == 2) return launch_few<T, 2, 1, 8, false>(a, st);
+    if (v == 3) return launch_async<T, 1, 2, 2, 1, 4, 2>(a, st);
+    if (v == 4) return launch_async<T, 1, 2, 2, 1, 2, 2>(a, st);
     if (v == 5) return launch_async<T, 1, 1, 2, 2, 1, 3>(a, st);
     if (v == 6) return launch_async<T, 1, 2, 2, 2, 1, 2>(a, st);
     return launch_async<T, 2, 2, 2, 2, 1, 2>(a, st);
