@@ -146,10 +146,11 @@ def case(S, O, I, seed):
 
 
 # one of everything, ragged tiles in each direction, block edges of the matrix's scales, and
-# sizes on both sides of each choice between kernels
+# sizes at which each of the kernel's forms is the one chosen
 SHAPES = [(1, 1, 1), (1, 16, 128), (2, 17, 129), (1, 2816, 2112), (3, 1000, 1088), (16, 129, 300), (17, 128, 2816),
           (21, 1000, 1088), (33, 257, 511), (64, 704, 2816), (65, 2112, 640), (100, 130, 1000), (128, 256, 256),
-          (200, 1500, 700), (256, 512, 128), (300, 257, 1025), (513, 640, 2816), (700, 2816, 704), (1025, 300, 130)]
+          (200, 1500, 700), (256, 512, 128), (300, 257, 1025), (513, 640, 2816), (700, 2816, 704), (1025, 300, 130),
+          (300, 2000, 1100), (2100, 2050, 200), (2500, 2500, 300)]
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
@@ -178,9 +179,12 @@ def test_product(dtype, S, O, I):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
-@pytest.mark.parametrize("S, ldy, off", [(5, 133, 0), (40, 200, 1), (300, 136, 0), (300, 131, 3)])
-def test_product_strides(dtype, S, ldy, off):
-    O, I = 130, 200
+@pytest.mark.parametrize("S, O, I, ldy, off", [(5, 130, 200, 133, 0), (40, 130, 200, 200, 1), (300, 130, 200, 136, 0),
+                                               (300, 130, 200, 131, 3), (300, 2000, 1100, 2008, 0), (700, 2816, 704, 2817, 5),
+                                               (1500, 1500, 600, 1504, 8), (2100, 2050, 200, 2051, 1),
+                                               (2500, 2500, 300, 2501, 0)])
+def test_product_strides(dtype, S, O, I, ldy, off):
+    print("case", S, O, I, ldy, off, dtype, flush=True)
     xq, xs, wq, ws = case(S, O, I, 5)
     m = zz.Fp8Matrix(O, I)
     try:
@@ -194,6 +198,31 @@ def test_product_strides(dtype, S, ldy, off):
         want, mag = R.product(xq, xs, wq, ws, O, I)
         assert np.all(np.abs(v[:, :O] - want) <= R.product_bound(mag, want, I, dtype))
         assert np.all(v[:, O:] == -3.0) and bool((y[:off] == -3.0).all())
+    finally:
+        m.close()
+
+
+@pytest.mark.parametrize("S, O, I", [(70, 300, 300), (300, 2000, 1100), (700, 2816, 704), (1500, 1500, 600),
+                                     (2100, 2050, 200), (2500, 2500, 300)])
+def test_product_rows_apart(S, O, I):
+    """A row of NaN codes and one of infinite scales touch no other row, in every form."""
+    print("case", S, O, I, flush=True)
+    xq, xs, wq, ws = case(S, O, I, 8)
+    m = zz.Fp8Matrix(O, I)
+    try:
+        m.upload(wq, ws)
+        Q, Sc = torch.from_numpy(xq).cuda(), torch.from_numpy(xs).cuda()
+        ys = [torch.empty(S, O, device="cuda") for _ in range(2)]
+        for y, bad in zip(ys, (False, True)):
+            if bad:
+                Q[S // 2, I - 1] = 0xFF
+                Sc[0, S - 1] = float("inf")
+            m.matmul_dev(Q.data_ptr(), Sc.data_ptr(), S, y.data_ptr(), stream=stream())
+        torch.cuda.synchronize()
+        keep = torch.ones(S, dtype=torch.bool)
+        keep[[S // 2, S - 1]] = False
+        assert torch.equal(ys[0][keep.cuda()], ys[1][keep.cuda()])
+        assert bool(ys[1][S // 2].isnan().all()) and not bool(ys[1][S - 1].isfinite().any())
     finally:
         m.close()
 
