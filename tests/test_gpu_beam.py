@@ -77,6 +77,13 @@ def test_step(dtype, N, W, V):
             assert bool((got[1] == 0).all())
 
 
+def test_step_widest():
+    """The most beams over the largest vocabulary: the longest lists that a merge holds."""
+    N, W, V = 1, 16, zz.ZZ_BEAM_MAXV
+    logits, score, _ = draw(N, W, V, F32, 4)
+    check(logits, score, None, N, W, V)
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("V, ldl, off", [(1001, 1001, 1), (1001, 1010, 3), (9000, 9001, 0), (4096, 8192, 4)])
 def test_step_strides(dtype, V, ldl, off):
@@ -316,16 +323,20 @@ def tied_head(V, D, seed):
     return np.concatenate([d.view(np.uint8).reshape(-1, 2), q], 1).reshape(-1)
 
 
-@pytest.mark.parametrize("W, eos", [(1, -1), (3, 9), (5, -1), (16, 3)])
-def test_stack_search(W, eos):
+@pytest.mark.parametrize("W, eos, flash", [(1, -1, False), (3, 9, False), (5, -1, False), (16, 3, False), (4, 2, True)])
+def test_stack_search(W, eos, flash):
     """zz_stack_beam_dev step by step: the same embedding, blocks, head and step called one by
-    one; one beam is the greedy decode."""
+    one; one beam is the greedy decode. With a FlashHead only the probed tokens have logits."""
     L = Z.make_layer("gemma", seed=39, E=16, K=4, D=512, MI=256)
     b, m, d = gpu_block(L, Z.make_dense(L.D, 512, 40))
     V, D, n = 1024, L.D, 6
     head = zz.Head(tied_head(V, D, 4), V, D, np.ones(D, np.float32), 1e-6, float(np.sqrt(D)), 30.0)
     stack = zz.Stack([b], head)
     try:
+        if flash:
+            ids = np.random.default_rng(8).permutation(V).astype(np.int32).reshape(32, 32)
+            head.flash(tied_head(32, D, 5), 32, ids, 32, 5, np.ones(32, np.float32), 1, np.array([2, 7], np.int32))
+            head.use_flash(True)
         start = torch.tensor([17], dtype=torch.int32, device="cuda")
         seq = torch.full((W + 1, n + 1), -5, dtype=torch.int32, device="cuda")
         score = torch.full((W + 1,), -5.0, device="cuda")
@@ -345,6 +356,7 @@ def test_stack_search(W, eos):
                 k = min(4, W - w)
                 head.logits_dev(H[w:].data_ptr(), k, lg[w:].data_ptr(), stream=stream())
             torch.cuda.synchronize()
+            assert flash == bool(torch.isinf(lg).any())
             so, pa, tk, do = check(lg.cpu(), sc, dn, 1, W, V, eos=eos, pad=max(eos, 0))
             hist = [hist[int(p)] + [int(t)] for p, t in zip(pa[0], tk[0])]
             sc, dn = so, do.bool()

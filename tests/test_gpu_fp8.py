@@ -334,3 +334,32 @@ def test_two_matrices_streams_and_graphs():
     finally:
         a.close()
         b.close()
+
+
+@pytest.mark.parametrize("S", [3, 20])
+def test_product_large_matrix(S):
+    """A matrix past the caches (64 MiB and more), against its own rows in a small one and
+    against 64 bits for some of them."""
+    O, I = 65600, 1088
+    g = torch.Generator(device="cuda").manual_seed(S)
+    wq = torch.randint(0, 127, (O, I), generator=g, dtype=torch.uint8, device="cuda")
+    wq += (torch.rand(O, I, generator=g, device="cuda") < 0.5).to(torch.uint8) * 128
+    ws = torch.rand(R.blocks(O), R.blocks(I), generator=g, device="cuda")
+    xq, xs, _, _ = case(S, 1, I, S)
+    Q, Sc = torch.from_numpy(xq).cuda(), torch.from_numpy(xs).cuda()
+    m = zz.Fp8Matrix(O, I)
+    try:
+        torch.cuda.synchronize()
+        m.upload_dev(wq.data_ptr(), ws.data_ptr())
+        y = torch.full((S + 1, O), -3.0, device="cuda")
+        m.matmul_dev(Q.data_ptr(), Sc.data_ptr(), S, y.data_ptr(), stream=stream())
+        torch.cuda.synchronize()
+        assert bool((y[S] == -3.0).all())
+        for at, n in ((0, 128), (33 * 128, 256), (O - 64, 64)):
+            part = wq[at:at + n].cpu().numpy()
+            sc = ws[at // 128:at // 128 + R.blocks(n)].cpu().numpy()
+            want, mag = R.product(xq, xs, part, sc, n, I)
+            off = np.abs(y[:S, at:at + n].double().cpu().numpy() - want)
+            assert np.all(off <= R.product_bound(mag, want, I, F32))
+    finally:
+        m.close()
