@@ -77,6 +77,30 @@ def test_step(dtype, N, W, V):
             assert bool((got[1] == 0).all())
 
 
+# both sides of the vocabulary that one launch takes; a last chunk of a few tokens; lists for
+# one wave's lanes and for more; one beam, one chunk or one token of each beam ahead of the rest
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("N, W, V", [(9, 16, 2048), (9, 16, 2049), (2, 5, 2060), (3, 16, 6147), (1, 9, 8200), (2, 16, 20000),
+                                     (70, 8, 16400), (1, 4, 65540)])
+@pytest.mark.parametrize("ahead", ["beam", "chunk", "tokens", "few"])
+def test_step_places(dtype, N, W, V, ahead):
+    logits, score, g = draw(N, W, V, dtype, N + V)
+    if ahead == "beam":
+        score[:, W // 2] = 100.0
+    elif ahead == "chunk":
+        logits[:, -(V % 2048 or 2048):] += 20.0
+    elif ahead == "tokens":
+        score[:] = -1.0
+        logits[:] = logits[:1]                           # equal beams: every total W times
+    else:
+        keep = torch.rand(N * W, V, generator=g) < 3 * W / V
+        keep[:, V // 2] = True
+        logits[~keep] = -float("inf")
+    check(logits, score, None, N, W, V)
+    done = torch.rand(N, W, generator=g) < 0.5
+    check(logits, score, done, N, W, V)
+
+
 def test_step_widest():
     """The most beams over the largest vocabulary: the longest lists that a merge holds."""
     N, W, V = 1, 16, zz.ZZ_BEAM_MAXV

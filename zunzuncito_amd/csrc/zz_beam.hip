@@ -8,6 +8,8 @@
 //                         largest keys in order, its maximum and sum of exponentials
 //   zz_beam_merge_kernel  a workgroup per sequence: a wave per beam joins the chunks' lists
 //                         and sums (in double), then one wave picks the W best totals
+// or, for a small vocabulary, one: zz_beam_small_kernel, whose waves make their beams' lists
+// themselves.
 #include "zz_common.h"
 #include "zz_kernels.h"
 #include "zz_fp8_dev.h"
@@ -44,6 +46,14 @@ __device__ __forceinline__ zz_u64 zz_beam_key(float v, int t) {
     return ((zz_u64)zz_ord32(v + 0.0f) << 32) | (0xffffffffu - (unsigned)t);
 }
 
+// lane q's (q wave-uniform)
+__device__ __forceinline__ unsigned zz_lane_u32(unsigned v, int q) {
+    return (unsigned)__builtin_amdgcn_readlane((int)v, q);
+}
+__device__ __forceinline__ zz_u64 zz_lane_u64(zz_u64 v, int q) {
+    return ((zz_u64)zz_lane_u32((unsigned)(v >> 32), q) << 32) | zz_lane_u32((unsigned)v, q);
+}
+
 // the wave's largest key: the upper words first, the lower ones only where several lanes share
 // the upper word (equal logits)
 __device__ __forceinline__ zz_u64 zz_wave_max64(zz_u64 v) {
@@ -52,7 +62,7 @@ __device__ __forceinline__ zz_u64 zz_wave_max64(zz_u64 v) {
     const unsigned H = zz_group_reduce<64>(hi, mx);
     const zz_u64 at = __ballot(hi == H);
     unsigned L;
-    if (__popcll(at) == 1) L = (unsigned)__builtin_amdgcn_readlane((int)lo, __ffsll((long long)at) - 1);
+    if (__popcll(at) == 1) L = zz_lane_u32(lo, __ffsll((long long)at) - 1);
     else L = zz_group_reduce<64>(hi == H ? lo : 0u, mx);
     return ((zz_u64)H << 32) | L;
 }
@@ -69,23 +79,27 @@ struct ZzBeamArgs {
     zz_u64 *ws;                     // [N*W][chunks][W + 1]: keys, then (maximum, sum)
 };
 
-// NV pieces of 16 bytes a thread, piece i * 256 + tid of the chunk counted from the row's first
-// token: the sum's order does not depend on where the row lies, so equal rows have equal
-// totals. A row of an odd vocabulary begins at any multiple of its element; the loads need no
-// more. The pieces across the row's end go element by element.
+// what a wave's lanes stored in LDS, read by the others
+__device__ __forceinline__ void zz_wave_lds() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// One wave's share of a row: NV pieces of 16 bytes a lane, pieces first, first + step, ... of the
+// row, counted from its first token: the sum's order does not depend on where the row lies, so
+// equal rows have equal totals. A row of an odd vocabulary begins at any multiple of its
+// element; the loads need no more. A piece across the row's end goes element by element.
+// best[0 .. W) receives the W largest keys in order (0 where there are fewer), *m_out the
+// maximum, *s_out the sum of exponentials against it. cand: 64 keys of LDS of the wave's own.
 template <typename T, int NV>
-__global__ __launch_bounds__(256) void zz_beam_part_kernel(ZzBeamArgs a) {
+__device__ __forceinline__ void zz_beam_wave(const T *L, int V, int first, int step, int W, zz_u64 *cand, zz_u64 *best,
+                                             float *m_out, float *s_out) {
     constexpr int VE = 16 / sizeof(T), NE = NV * VE;
-    __shared__ zz_u64 cand[4][64];
-    __shared__ zz_u64 best[4][ZZ_BEAM_MAXW];
-    __shared__ float wm[4], wsum[4];
-    const int row = blockIdx.y, ch = blockIdx.x, tid = threadIdx.x, l = tid & 63, w = tid >> 6, W = a.W, V = a.V;
-    if (a.done && a.done[row]) return;
-    const T *L = (const T *)a.logits + row * a.ldl;
+    const int l = threadIdx.x & 63;
     float v[NE];
 #pragma unroll
     for (int i = 0; i < NV; i++) {
-        const int e = (ch * NV * 256 + i * 256 + tid) * VE;
+        const int e = (first + i * step) * VE;
         if (e + VE <= V) {
             unsigned u[4];
             __builtin_memcpy(u, L + e, 16);
@@ -105,7 +119,7 @@ __global__ __launch_bounds__(256) void zz_beam_part_kernel(ZzBeamArgs a) {
     }
     // the token of element k, or -1 where it lies outside the row
     auto tok = [&](int k) {
-        const int t = (ch * NV * 256 + (k / VE) * 256 + tid) * VE + k % VE;
+        const int t = (first + k / VE * step) * VE + k % VE;
         return t < V ? t : -1;
     };
     float lm = -INFINITY;
@@ -132,35 +146,54 @@ __global__ __launch_bounds__(256) void zz_beam_part_kernel(ZzBeamArgs a) {
     }
     s = zz_wave_sum(s);
     // The W-th largest of the lanes' maxima: at least W logits reach it, and the W best do. What
-    // reaches it is a few more than W, unless many are equal.
-    float left = lm, line = m;
-    for (int k = 1; k < W; k++) {
-        const zz_u64 at = __ballot(left == line);
-        if (l == __ffsll((long long)at) - 1) left = -INFINITY;
-        line = zz_wave_max(left);
+    // reaches it is a few more than W, unless many are equal. Rounds of a wave's maximum find it
+    // for a few beams (4: 4.1 us a launch over 2048 logits, against 4.5); beyond, it is the least
+    // of the maxima with fewer than W above them, counted (16: 6.7 against 7.5).
+    float line = m;
+    if (W <= 4) {
+        float left = lm;
+        for (int k = 1; k < W; k++) {
+            const zz_u64 at = __ballot(left == line);
+            if (l == __ffsll((long long)at) - 1) left = -INFINITY;
+            line = zz_wave_max(left);
+        }
+    } else {
+        float *lms = (float *)cand;
+        lms[l] = lm;
+        zz_wave_lds();
+        int above = 0;
+#pragma unroll
+        for (int j = 0; j < 64; j++) above += lms[j] > lm;
+        line = -zz_wave_max(above < W ? -lm : -INFINITY);
+        zz_wave_lds();
     }
-    if (l < W) best[w][l] = 0;
-    cand[w][l] = 0;
-    int total = line == -INFINITY ? 65 : 0;              // padding would be among them
-    if (total == 0) {
+    if (l < W) best[l] = 0;
+    cand[l] = 0;
+    zz_wave_lds();
+    int total = 0;
+    auto gather = [&](auto in) {
 #pragma unroll
         for (int k = 0; k < NE; k++) {
-            const zz_u64 at = __ballot(v[k] >= line);
+            const bool is = in(k);
+            const zz_u64 at = __ballot(is);
             if (at) {
                 const int o = total + __builtin_amdgcn_mbcnt_hi((unsigned)(at >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)at, 0));
-                if (v[k] >= line && o < 64) cand[w][o] = zz_beam_key(v[k], tok(k));
+                if (is && o < 64) cand[o] = zz_beam_key(v[k], tok(k));
                 total += __popcll(at);
             }
         }
-    }
+    };
+    if (line != -INFINITY) gather([&](int k) { return v[k] >= line; });
+    else gather([&](int k) { return tok(k) >= 0; });     // what lies outside the row is there too
     if (total <= 64) {
+        zz_wave_lds();
         // a candidate a lane: its place is the number of better ones
-        const zz_u64 key = cand[w][l];
+        const zz_u64 key = cand[l];
         int rank = 0;
         for (int j = 0; j < total; j += 8)
 #pragma unroll
-            for (int i = 0; i < 8; i++) rank += cand[w][j + i] > key;
-        if (l < total && rank < W) best[w][rank] = key;
+            for (int i = 0; i < 8; i++) rank += cand[j + i] > key;
+        if (l < total && rank < W) best[rank] = key;
     } else {
         // W rounds of the wave's largest remaining key
         zz_u64 prev = ~0ull;
@@ -173,99 +206,210 @@ __global__ __launch_bounds__(256) void zz_beam_part_kernel(ZzBeamArgs a) {
                 if (key < prev && key > b) b = key;
             }
             prev = zz_wave_max64(b);
-            if (l == 0) best[w][k] = prev;
+            if (l == 0) best[k] = prev;
         }
     }
+    *m_out = m;
+    *s_out = s;
+}
+
+__device__ __forceinline__ zz_u64 zz_beam_sum(float m, float s) { return ((zz_u64)__float_as_uint(s) << 32) | __float_as_uint(m); }
+
+// A workgroup per (chunk, row); its four waves' shares are interleaved piece by piece.
+template <typename T, int NV>
+__global__ __launch_bounds__(256) void zz_beam_part_kernel(ZzBeamArgs a) {
+    __shared__ zz_u64 cand[4][64];
+    __shared__ zz_u64 best[4][ZZ_BEAM_MAXW];
+    __shared__ float wm[4], wsum[4];
+    const int row = blockIdx.y, ch = blockIdx.x, tid = threadIdx.x, l = tid & 63, w = tid >> 6, W = a.W;
+    if (a.done && a.done[row]) return;
+    float m, s;
+    zz_beam_wave<T, NV>((const T *)a.logits + row * a.ldl, a.V, ch * NV * 256 + tid, 256, W, cand[w], best[w], &m, &s);
     if (l == 0) { wm[w] = m; wsum[w] = s; }
     __syncthreads();
     if (w != 0) return;
     // the four waves' lists, a key a lane: its place among all is the number of better ones
     const zz_u64 key = l < 4 * W ? best[l / W][l % W] : 0;
     cand[0][l] = key;
+    zz_wave_lds();
     int rank = 0;
     for (int j = 0; j < 4 * W; j += 4)
 #pragma unroll
-        for (int i = 0; i < 4; i++) rank += cand[0][j + i] > key || (cand[0][j + i] == key && j + i < l);
+        for (int i = 0; i < 4; i++) rank += (cand[0][j + i] > key) | ((cand[0][j + i] == key) & (j + i < l));
     zz_u64 *out = a.ws + ((size_t)row * a.chunks + ch) * (W + 1);
     if (l < 4 * W && rank < W) out[rank] = key;
     if (l == 0) {
         const float M = fmaxf(fmaxf(wm[0], wm[1]), fmaxf(wm[2], wm[3]));
         float t = 0.0f;
         for (int q = 0; q < 4; q++) t += wm[q] == M ? wsum[q] : wsum[q] * __builtin_amdgcn_exp2f((wm[q] - M) * ZZ_LOG2E);
-        out[W] = ((zz_u64)__float_as_uint(t) << 32) | __float_as_uint(M);
+        out[W] = zz_beam_sum(M, t);
+    }
+}
+
+// The W best of n <= 64 lists of distinct keys (list i at p + i * stride: W keys in order, 0
+// behind the last), by one wave: lane k < W receives the k-th, 0 if there are fewer. Serial rounds
+// of a wave's maximum cost their latency W times over; so a key's place is counted, as the number
+// of better ones, among as many of the lists' first keys as the wave has lanes. Where these are
+// not all keys, the W-th of them (by its logit) is a bound that the W best reach, and few others
+// do; only if more than 64 reach it, rounds decide. cand: 64 keys of LDS of the wave's own.
+__device__ __forceinline__ zz_u64 zz_beam_best(const zz_u64 *p, int stride, int n, int W, zz_u64 *cand) {
+    const int l = threadIdx.x & 63;
+    if (n == 1) return l < W ? p[l] : 0;
+    // 64 / n keys of each, down to a power of two, or one that holds W
+    const int sh = min(__builtin_clz(n - 1) - 26, W > 1 ? 32 - __builtin_clz(W - 1) : 0);
+    const int i = l >> sh, k = l & ((1 << sh) - 1);
+    zz_u64 key = i < n && k < W ? p[i * stride + k] : 0;
+    int m = n << sh;
+    if (1 << sh < W) {
+        const unsigned hi = (unsigned)(key >> 32);
+        unsigned *his = (unsigned *)cand;
+        his[l] = hi;
+        zz_wave_lds();
+        int above = 0;
+#pragma unroll
+        for (int j = 0; j < 64; j++) above += his[j] > hi;
+        const unsigned line = zz_group_reduce<64>(above < W ? ~hi : 0u, [](unsigned x, unsigned y) { return x > y ? x : y; });
+        const zz_u64 bar = (zz_u64)~line << 32;
+        zz_wave_lds();
+        cand[l] = 0;
+        m = bar ? 0 : 65;
+        for (int q = 0; q < W && m <= 64; q++) {
+            const zz_u64 mine = l < n ? p[l * stride + q] : 0;
+            const zz_u64 in = __ballot(mine >= bar);
+            if (!in) break;
+            const int o = m + __builtin_amdgcn_mbcnt_hi((unsigned)(in >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)in, 0));
+            if (mine >= bar && o < 64) cand[o] = mine;
+            m += __popcll(in);
+        }
+        if (m > 64) {
+            int first = 0;
+            zz_u64 head = l < n ? p[l * stride] : 0, got = 0;
+            for (int q = 0; q < W; q++) {
+                const zz_u64 b = zz_wave_max64(head);
+                if (l == q) got = b;
+                if (head == b && b) {
+                    first++;
+                    head = first < W ? p[l * stride + first] : 0;
+                }
+            }
+            return got;
+        }
+        zz_wave_lds();
+        key = cand[l];
+    } else {
+        cand[l] = key;
+        zz_wave_lds();
+    }
+    int rank = 0;
+    for (int j = 0; j < m; j += 8)
+#pragma unroll
+        for (int u = 0; u < 8; u++) rank += cand[j + u] > key;
+    zz_wave_lds();
+    cand[l] = 0;
+    zz_wave_lds();
+    if (key) cand[rank] = key;
+    zz_wave_lds();
+    return cand[l];
+}
+
+// What a sequence's workgroup picks from, in LDS.
+struct ZzBeamPick {
+    zz_u64 tot[ZZ_BEAM_MAXW][ZZ_BEAM_MAXW];              // a beam's best totals in order, 0: none
+    zz_u64 cand[ZZ_BEAM_MAXW][64];                       // a wave's own
+};
+
+// A wave per beam: `mine`, its row's C lists with their sums, to the row's W best totals, and
+// these to their places among the sequence's.
+__device__ __forceinline__ void zz_beam_finish(const ZzBeamArgs &a, ZzBeamPick &P, const zz_u64 *mine, int C, bool done,
+                                               float c) {
+    const int w = zz_wave_id(), l = threadIdx.x & 63, W = a.W;
+    if (c != c) c = -INFINITY;
+    zz_u64 tot = 0;
+    int tok = a.pad;
+    if (done) {
+        if (l == 0) tot = zz_ord64((double)c);
+    } else {
+        const zz_u64 ms = l < C ? mine[l * (W + 1) + W] : 0;
+        const float m = l < C ? __uint_as_float((unsigned)ms) : -INFINITY, M = zz_wave_max(m);
+        float part = l < C ? __uint_as_float((unsigned)(ms >> 32)) : 0.0f;
+        if (m != M) part *= __builtin_amdgcn_exp2f((m - M) * ZZ_LOG2E);
+        const double ls = log(zz_wave_sum((double)part));
+        const zz_u64 b = zz_beam_best(mine, W + 1, C, W, P.cand[w]);
+        const float L = zz_unord32((unsigned)(b >> 32));
+        // the logit relative to its row's largest first: a row at the type's lowest value
+        // keeps its bits; a row of minus infinities offers nothing better
+        double t = (double)c + ((L == M ? 0.0 : (double)L - (double)M) - ls);
+        if (t != t || M == -INFINITY) t = -(double)INFINITY;
+        if (b && l < W) tot = zz_ord64(t);
+        tok = (int)(0xffffffffu - (unsigned)b);
+    }
+    if (l < W) P.tot[w][l] = tot;
+    __syncthreads();
+    // A total's place is the number of better ones: its own list's before it, and in each other
+    // list those not below it (equal totals go to the lower beam), found by halving. Lane l's
+    // row of 16 lanes goes through every fourth list for the l % 16-th total.
+    const int k = l & 15, part = l >> 4;
+    const zz_u64 own = k < W ? P.tot[w][k] : 0;
+    int at[ZZ_BEAM_MAXW / 4] = {};
+#pragma unroll
+    for (int s = 0; s < 5; s++) {
+        const int step = s < 4 ? 8 >> s : 1;
+#pragma unroll
+        for (int j = 0; j < ZZ_BEAM_MAXW / 4; j++) {
+            const int list = part + 4 * j;
+            if (list < W && at[j] + step <= W && P.tot[list][at[j] + step - 1] >= own + (list > w)) at[j] += step;
+        }
+    }
+    int rank = 0;
+#pragma unroll
+    for (int j = 0; j < ZZ_BEAM_MAXW / 4; j++) rank += part + 4 * j == w ? k : at[j];
+    rank = zz_rows_sum(rank);
+    if (l < W && own && rank < W) {
+        const int o = blockIdx.x * W + rank;
+        a.score_out[o] = (float)zz_unord64(own);
+        a.parent[o] = w;
+        a.token[o] = tok;
+        if (a.done_out) a.done_out[o] = done || (a.eos >= 0 && tok == a.eos);
     }
 }
 
 // Dynamic LDS: each row's lists and sums, as the workspace holds them.
 __global__ __launch_bounds__(1024) void zz_beam_merge_kernel(ZzBeamArgs a) {
     extern __shared__ __attribute__((aligned(16))) zz_u64 lists[];
-    __shared__ zz_u64 tot[ZZ_BEAM_MAXW][ZZ_BEAM_MAXW];      // ordered totals, 0: no candidate
-    __shared__ int tk[ZZ_BEAM_MAXW][ZZ_BEAM_MAXW];
-    __shared__ uint8_t fin[ZZ_BEAM_MAXW];
-    const int n = blockIdx.x, w = zz_wave_id(), l = threadIdx.x & 63, W = a.W, row = n * W + w, C = a.chunks;
+    __shared__ ZzBeamPick P;
+    const int w = zz_wave_id(), l = threadIdx.x & 63, row = blockIdx.x * a.W + w;
     // everything that is read, before anything waits: a finished beam's lists mean nothing, and
     // are not looked at
-    const int words = C * (W + 1);
+    const int words = a.chunks * (a.W + 1);
     zz_u64 *mine = lists + (size_t)w * words;
     const zz_u64 *from = a.ws + (size_t)row * words;
-    const uint8_t flag = a.done ? a.done[row] : 0;
-    float c = a.score[row];
+    const uint8_t done = a.done ? a.done[row] : 0;
+    const float c = a.score[row];
 #pragma unroll 8
     for (int i = l; i < words; i += 64) mine[i] = from[i];
-    const bool done = flag;
-    if (c != c) c = -INFINITY;
-    if (done) {
-        if (l < W) {
-            tot[w][l] = l == 0 ? zz_ord64((double)c) : 0;
-            tk[w][l] = a.pad;
-        }
-    } else {
-        const zz_u64 *p = mine + l * (W + 1);
-        const zz_u64 ms = l < C ? p[W] : 0;
-        const float m = l < C ? __uint_as_float((unsigned)ms) : -INFINITY, M = zz_wave_max(m);
-        float part = l < C ? __uint_as_float((unsigned)(ms >> 32)) : 0.0f;
-        if (m != M) part *= __builtin_amdgcn_exp2f((m - M) * ZZ_LOG2E);
-        const double s = zz_wave_sum((double)part);
-        const double ls = log(s);
-        // the chunks' sorted lists, one a lane: W times the largest head
-        int at = 0;
-        zz_u64 head = l < C ? p[0] : 0;
-        for (int k = 0; k < W; k++) {
-            const zz_u64 b = zz_wave_max64(head);
-            if (l == k) {
-                const float L = zz_unord32((unsigned)(b >> 32));
-                // the logit relative to its row's largest first: a row at the type's lowest value
-                // keeps its bits; a row of minus infinities offers nothing better
-                double t = (double)c + ((L == M ? 0.0 : (double)L - (double)M) - ls);
-                if (t != t || M == -INFINITY) t = -(double)INFINITY;
-                tot[w][k] = b ? zz_ord64(t) : 0;
-                tk[w][k] = (int)(0xffffffffu - (unsigned)b);
-            }
-            if (head == b && b) {
-                at++;
-                head = at < W ? p[at] : 0;
-            }
-        }
+    zz_wave_lds();
+    zz_beam_finish(a, P, mine, a.chunks, done, c);
+}
+
+// A workgroup per sequence and a wave per beam, for rows that a wave's registers hold. At 2048
+// logits of f32 one launch against two: 5.2 us against 6.8 (1 sequence of 4 beams), 7.3 against
+// 9.1 (32 of 8), 11.3 against 16.2 (64 of 16); in two shares of 2048 each (4096 logits) it lost
+// (9.1 against 8.2), since a wave then waits for its row twice.
+#define ZZ_BEAM_SMALL 2048
+template <typename T>
+__global__ __launch_bounds__(1024) void zz_beam_small_kernel(ZzBeamArgs a) {
+    __shared__ ZzBeamPick P;
+    __shared__ zz_u64 lists[ZZ_BEAM_MAXW][ZZ_BEAM_MAXW + 1];
+    const int w = zz_wave_id(), l = threadIdx.x & 63, W = a.W, row = blockIdx.x * W + w;
+    const bool done = a.done && a.done[row];
+    const float c = a.score[row];
+    if (!done) {
+        float m, s;
+        zz_beam_wave<T, ZZ_BEAM_SMALL * sizeof(T) / 1024>((const T *)a.logits + row * a.ldl, a.V, l, 64, W, P.cand[w], lists[w], &m, &s);
+        if (l == 0) lists[w][W] = zz_beam_sum(m, s);
     }
-    if (l == 0) fin[w] = done;
-    __syncthreads();
-    if (w != 0) return;
-    // the beams' lists, one a lane; equal totals go to the lower beam
-    int at = 0;
-    zz_u64 head = l < W ? tot[l][0] : 0;
-    for (int k = 0; k < W; k++) {
-        const zz_u64 b = zz_wave_max64(head);
-        const int who = __ffsll((long long)__ballot(head == b && l < W)) - 1;
-        if (l == who) {
-            const int o = n * W + k, t = tk[l][at];
-            a.score_out[o] = (float)zz_unord64(b);
-            a.parent[o] = l;
-            a.token[o] = t;
-            if (a.done_out) a.done_out[o] = fin[l] || (a.eos >= 0 && t == a.eos);
-            at++;
-            head = at < W ? tot[l][at] : 0;
-        }
-    }
+    zz_wave_lds();
+    zz_beam_finish(a, P, lists[w], 1, done, c);
 }
 
 // A thread owns one piece G of a row's bytes in all W rows of a sequence: it reads what
@@ -354,7 +498,14 @@ extern "C" int zz_beam_step_dev(int dtype, const void *d_logits, int64_t ldl, in
     }
     if (!zz_lib_here(who)) return 0;
     hipStream_t st = stream ? (hipStream_t)stream : zz_lib_stream();
-    ZzBeamArgs a{d_logits, ldl, N, W, V, beam_chunks(N, W, V), eos, pad, d_score, d_done, d_score_out, d_parent,
+    if (V <= ZZ_BEAM_SMALL) {
+        const ZzBeamArgs a{d_logits, ldl, N, W, V, 0, eos, pad, d_score, d_done, d_score_out, d_parent, d_token, d_done_out, nullptr};
+        if (dtype == ZZ_F32) hipLaunchKernelGGL((zz_beam_small_kernel<float>), dim3(N), dim3(64 * W), 0, st, a);
+        else hipLaunchKernelGGL((zz_beam_small_kernel<zz_bf16>), dim3(N), dim3(64 * W), 0, st, a);
+        if (hipGetLastError() != hipSuccess) ZZ_FAIL("%s: launch failed", who);
+        return 1;
+    }
+    const ZzBeamArgs a{d_logits, ldl, N, W, V, beam_chunks(N, W, V), eos, pad, d_score, d_done, d_score_out, d_parent,
                  d_token, d_done_out, (zz_u64 *)d_ws};
     const dim3 g(a.chunks, (unsigned)R), b(256);
     const bool few = beam_elems(N, W, V) == 8;

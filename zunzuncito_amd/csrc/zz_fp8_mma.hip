@@ -18,9 +18,6 @@
 // 19 cycles were measured.)
 #include "zz_fp8_dev.h"
 #include <math.h>
-#ifdef ZZ_TUNE
-#include <stdlib.h>
-#endif
 
 typedef _Float16 zz_h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 zz_h8 __attribute__((ext_vector_type(8)));
@@ -435,12 +432,7 @@ static int mm_plan(int O, int S, int nb) {
 
 template <typename T>
 static bool launch_mm(const ZzF8Mm &a, hipStream_t st) {
-#ifdef ZZ_TUNE
-    const char *e = getenv("ZZ_TILE");
-    const int v = e && atoi(e) >= 0 ? atoi(e) : mm_plan(a.m.O, a.S, a.nb);
-#else
     const int v = mm_plan(a.m.O, a.S, a.nb);
-#endif
     if (v == 0) return launch_few<T, 1, 1, 16, false, false>(a, st);
     // a large matrix, read once, past the caches; the activation rows come from the L2 for each
     // workgroup again, which 64 matrix rows a workgroup halve (200000 x 2816: 4 rows 85 us and 89
