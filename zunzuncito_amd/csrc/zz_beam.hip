@@ -9,7 +9,9 @@
 //   zz_beam_merge_kernel  a workgroup per sequence: a wave per beam joins the chunks' lists
 //                         and sums (in double), then one wave picks the W best totals
 // or, for a small vocabulary, one: zz_beam_small_kernel, whose waves make their beams' lists
-// themselves.
+// themselves. A step of 16 sequences of 8 beams over 262144 f32 logits takes 32 us, 134 MB at
+// 4.2 TB/s, 25 us of it in the first launch at 5.4 TB/s; in bf16 28.7 us, bound by the work on an
+// element (maximum, exponential, comparison) and by what a chunk does after them.
 #include "zz_common.h"
 #include "zz_kernels.h"
 #include "zz_fp8_dev.h"
@@ -85,117 +87,92 @@ __device__ __forceinline__ void zz_wave_lds() {
     __builtin_amdgcn_wave_barrier();
 }
 
-// One wave's share of a row: NV pieces of 16 bytes a lane, pieces first, first + step, ... of the
-// row, counted from its first token: the sum's order does not depend on where the row lies, so
-// equal rows have equal totals. A row of an odd vocabulary begins at any multiple of its
-// element; the loads need no more. A piece across the row's end goes element by element.
-// best[0 .. W) receives the W largest keys in order (0 where there are fewer), *m_out the
-// maximum, *s_out the sum of exponentials against it. cand: 64 keys of LDS of the wave's own.
+// A thread's share of a row: NV pieces of 16 bytes, pieces first, first + step, ... counted from
+// the row's first token: the sum's order does not depend on where the row lies, so equal rows
+// have equal totals. A row of an odd vocabulary begins at any multiple of its element; the loads
+// need no more. A piece across the row's end goes element by element.
 template <typename T, int NV>
-__device__ __forceinline__ void zz_beam_wave(const T *L, int V, int first, int step, int W, zz_u64 *cand, zz_u64 *best,
-                                             float *m_out, float *s_out) {
-    constexpr int VE = 16 / sizeof(T), NE = NV * VE;
-    const int l = threadIdx.x & 63;
+struct ZzBeamShare {
+    static constexpr int VE = 16 / sizeof(T), NE = NV * VE;
     float v[NE];
+    int V, first, step;
+
+    __device__ __forceinline__ ZzBeamShare(const T *L, int V_, int first_, int step_) : V(V_), first(first_), step(step_) {
 #pragma unroll
-    for (int i = 0; i < NV; i++) {
-        const int e = (first + i * step) * VE;
-        if (e + VE <= V) {
-            unsigned u[4];
-            __builtin_memcpy(u, L + e, 16);
+        for (int i = 0; i < NV; i++) {
+            const int e = (first + i * step) * VE;
+            if (e + VE <= V) {
+                unsigned u[4];
+                __builtin_memcpy(u, L + e, 16);
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                if constexpr (VE == 4) {
-                    v[4 * i + j] = __uint_as_float(u[j]);
-                } else {
-                    v[8 * i + 2 * j] = __uint_as_float(u[j] << 16);
-                    v[8 * i + 2 * j + 1] = __uint_as_float(u[j] & 0xffff0000u);
+                for (int j = 0; j < 4; j++) {
+                    if constexpr (VE == 4) {
+                        v[4 * i + j] = __uint_as_float(u[j]);
+                    } else {
+                        v[8 * i + 2 * j] = __uint_as_float(u[j] << 16);
+                        v[8 * i + 2 * j + 1] = __uint_as_float(u[j] & 0xffff0000u);
+                    }
                 }
-            }
-        } else {
+            } else {
 #pragma unroll
-            for (int j = 0; j < VE; j++) v[VE * i + j] = e + j < V ? zz_f32_of(L[e + j]) : NAN;
+                for (int j = 0; j < VE; j++) v[VE * i + j] = e + j < V ? zz_f32_of(L[e + j]) : NAN;
+            }
         }
     }
     // the token of element k, or -1 where it lies outside the row
-    auto tok = [&](int k) {
+    __device__ __forceinline__ int tok(int k) const {
         const int t = (first + k / VE * step) * VE + k % VE;
         return t < V ? t : -1;
-    };
-    float lm = -INFINITY;
-#pragma unroll
-    for (int k = 0; k < NE; k++) {
-        v[k] = fmaxf(v[k], -INFINITY);                   // a NaN counts as minus infinity
-        lm = fmaxf(lm, v[k]);
     }
-    const float m = zz_wave_max(lm);
-    float s = 0.0f;
-    if (fabsf(m) < 16384.0f) {
-        // 2^(v log2(e) - c), c = m log2(e) rounded; what c's rounding left is a common factor
-        const float c = m * ZZ_LOG2E, off = fmaf(m, ZZ_LOG2E, -c);
-#pragma unroll
-        for (int k = 0; k < NE; k++) s += __builtin_amdgcn_exp2f(fmaf(v[k], ZZ_LOG2E, -c));
-        s *= __builtin_amdgcn_exp2f(-off);
-    } else if (fabsf(m) != INFINITY) {
-#pragma unroll
-        for (int k = 0; k < NE; k++) s += __builtin_amdgcn_exp2f((v[k] - m) * ZZ_LOG2E);
-    } else {
-        // the infinite logits share the probability; at minus infinity the sum is not used
-#pragma unroll
-        for (int k = 0; k < NE; k++) s += v[k] == m ? 1.0f : 0.0f;
-    }
-    s = zz_wave_sum(s);
-    // The W-th largest of the lanes' maxima: at least W logits reach it, and the W best do. What
-    // reaches it is a few more than W, unless many are equal. Rounds of a wave's maximum find it
-    // for a few beams (4: 4.1 us a launch over 2048 logits, against 4.5); beyond, it is the least
-    // of the maxima with fewer than W above them, counted (16: 6.7 against 7.5).
-    float line = m;
-    if (W <= 4) {
-        float left = lm;
-        for (int k = 1; k < W; k++) {
-            const zz_u64 at = __ballot(left == line);
-            if (l == __ffsll((long long)at) - 1) left = -INFINITY;
-            line = zz_wave_max(left);
-        }
-    } else {
-        float *lms = (float *)cand;
-        lms[l] = lm;
-        zz_wave_lds();
-        int above = 0;
-#pragma unroll
-        for (int j = 0; j < 64; j++) above += lms[j] > lm;
-        line = -zz_wave_max(above < W ? -lm : -INFINITY);
-        zz_wave_lds();
-    }
-    if (l < W) best[l] = 0;
-    cand[l] = 0;
-    zz_wave_lds();
-    int total = 0;
-    auto gather = [&](auto in) {
+    __device__ __forceinline__ float max() {
+        float m = -INFINITY;
 #pragma unroll
         for (int k = 0; k < NE; k++) {
-            const bool is = in(k);
-            const zz_u64 at = __ballot(is);
-            if (at) {
-                const int o = total + __builtin_amdgcn_mbcnt_hi((unsigned)(at >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)at, 0));
-                if (is && o < 64) cand[o] = zz_beam_key(v[k], tok(k));
-                total += __popcll(at);
-            }
+            v[k] = fmaxf(v[k], -INFINITY);               // a NaN counts as minus infinity
+            m = fmaxf(m, v[k]);
         }
-    };
-    if (line != -INFINITY) gather([&](int k) { return v[k] >= line; });
-    else gather([&](int k) { return tok(k) >= 0; });     // what lies outside the row is there too
-    if (total <= 64) {
-        zz_wave_lds();
-        // a candidate a lane: its place is the number of better ones
-        const zz_u64 key = cand[l];
-        int rank = 0;
-        for (int j = 0; j < total; j += 8)
+        return m;
+    }
+    // the sum of exp(v - m)
+    __device__ __forceinline__ float sum(float m) const {
+        float s = 0.0f;
+        if (fabsf(m) < 16384.0f) {
+            // 2^(v log2(e) - c), c = m log2(e) rounded; what c's rounding left is a common factor
+            const float c = m * ZZ_LOG2E, off = fmaf(m, ZZ_LOG2E, -c);
 #pragma unroll
-            for (int i = 0; i < 8; i++) rank += cand[j + i] > key;
-        if (l < total && rank < W) best[rank] = key;
-    } else {
-        // W rounds of the wave's largest remaining key
+            for (int k = 0; k < NE; k++) s += __builtin_amdgcn_exp2f(fmaf(v[k], ZZ_LOG2E, -c));
+            s *= __builtin_amdgcn_exp2f(-off);
+        } else if (fabsf(m) != INFINITY) {
+#pragma unroll
+            for (int k = 0; k < NE; k++) s += __builtin_amdgcn_exp2f((v[k] - m) * ZZ_LOG2E);
+        } else {
+            // the infinite logits share the probability; at minus infinity the sum is not used
+#pragma unroll
+            for (int k = 0; k < NE; k++) s += v[k] == m ? 1.0f : 0.0f;
+        }
+        return s;
+    }
+    // the wave's keys of logits that reach the line, to cand while they are up to 64; their number
+    __device__ __forceinline__ int gather(float line, zz_u64 *cand) const {
+        int total = 0;
+        auto walk = [&](auto in) {
+#pragma unroll
+            for (int k = 0; k < NE; k++) {
+                const bool is = in(k);
+                const zz_u64 at = __ballot(is);
+                if (at) {
+                    const int o = total + __builtin_amdgcn_mbcnt_hi((unsigned)(at >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)at, 0));
+                    if (is && o < 64) cand[o] = zz_beam_key(v[k], tok(k));
+                    total += __popcll(at);
+                }
+            }
+        };
+        if (line != -INFINITY) walk([&](int k) { return v[k] >= line; });
+        else walk([&](int k) { return tok(k) >= 0; });   // what lies outside the row is there too
+        return total;
+    }
+    // the wave's W largest keys, a round each: for more than 64 at the line
+    __device__ __forceinline__ void rounds(int W, zz_u64 *best) const {
         zz_u64 prev = ~0ull;
         for (int k = 0; k < W; k++) {
             zz_u64 b = 0;
@@ -206,44 +183,93 @@ __device__ __forceinline__ void zz_beam_wave(const T *L, int V, int first, int s
                 if (key < prev && key > b) b = key;
             }
             prev = zz_wave_max64(b);
-            if (l == 0) best[k] = prev;
+            if ((threadIdx.x & 63) == 0) best[k] = prev;
         }
     }
-    *m_out = m;
-    *s_out = s;
+};
+
+// The W-th largest of the lanes' lm, m the largest. Rounds of a wave's maximum find it for up to
+// 8 beams (a step of 1 sequence over 4096 logits, 4 beams: 6.3 us against 6.6); beyond, it is the
+// least of those with fewer than W above them, counted (16 beams: 9.7 us against 10.7).
+// lms: 64 floats of LDS.
+__device__ __forceinline__ float zz_beam_line(float lm, float m, int W, float *lms) {
+    const int l = threadIdx.x & 63;
+    float line = m;
+    if (W <= 8) {
+        for (int k = 1; k < W; k++) {
+            const zz_u64 at = __ballot(lm == line);
+            if (l == __ffsll((long long)at) - 1) lm = -INFINITY;
+            line = zz_wave_max(lm);
+        }
+        return line;
+    }
+    lms[l] = lm;
+    zz_wave_lds();
+    int above = 0;
+#pragma unroll
+    for (int j = 0; j < 64; j++) above += lms[j] > lm;
+    line = -zz_wave_max(above < W ? -lm : -INFINITY);
+    zz_wave_lds();
+    return line;
+}
+
+// The place of a lane's key among n <= 64 distinct ones, one a lane and 0 beyond: the number of
+// better ones. keys: 64 of LDS, which then hold them.
+__device__ __forceinline__ int zz_beam_place(zz_u64 key, int n, zz_u64 *keys) {
+    keys[threadIdx.x & 63] = key;
+    zz_wave_lds();
+    int rank = 0;
+    for (int j = 0; j < n; j += 8)
+#pragma unroll
+        for (int u = 0; u < 8; u++) rank += keys[j + u] > key;
+    zz_wave_lds();
+    return rank;
 }
 
 __device__ __forceinline__ zz_u64 zz_beam_sum(float m, float s) { return ((zz_u64)__float_as_uint(s) << 32) | __float_as_uint(m); }
 
-// A workgroup per (chunk, row); its four waves' shares are interleaved piece by piece.
+// A workgroup per (chunk, row); its waves' pieces are interleaved. At least W logits reach the
+// W-th largest of 64 groups' maxima (a lane of each wave is a group), and the W best do: a few
+// more than W, unless many are equal. One wave finds that line while the others sum, and ranks
+// what all gathered.
 template <typename T, int NV>
 __global__ __launch_bounds__(256) void zz_beam_part_kernel(ZzBeamArgs a) {
     __shared__ zz_u64 cand[4][64];
-    __shared__ zz_u64 best[4][ZZ_BEAM_MAXW];
-    __shared__ float wm[4], wsum[4];
-    const int row = blockIdx.y, ch = blockIdx.x, tid = threadIdx.x, l = tid & 63, w = tid >> 6, W = a.W;
+    __shared__ float lms[256], wsum[4], lines;
+    __shared__ int count[4];
+    const int row = blockIdx.y, ch = blockIdx.x, tid = threadIdx.x, l = tid & 63, w = zz_wave_id(), W = a.W;
     if (a.done && a.done[row]) return;
-    float m, s;
-    zz_beam_wave<T, NV>((const T *)a.logits + row * a.ldl, a.V, ch * NV * 256 + tid, 256, W, cand[w], best[w], &m, &s);
-    if (l == 0) { wm[w] = m; wsum[w] = s; }
+    ZzBeamShare<T, NV> x((const T *)a.logits + row * a.ldl, a.V, ch * NV * 256 + tid, 256);
+    lms[tid] = x.max();
     __syncthreads();
-    if (w != 0) return;
-    // the four waves' lists, a key a lane: its place among all is the number of better ones
-    const zz_u64 key = l < 4 * W ? best[l / W][l % W] : 0;
-    cand[0][l] = key;
-    zz_wave_lds();
-    int rank = 0;
-    for (int j = 0; j < 4 * W; j += 4)
-#pragma unroll
-        for (int i = 0; i < 4; i++) rank += (cand[0][j + i] > key) | ((cand[0][j + i] == key) & (j + i < l));
-    zz_u64 *out = a.ws + ((size_t)row * a.chunks + ch) * (W + 1);
-    if (l < 4 * W && rank < W) out[rank] = key;
-    if (l == 0) {
-        const float M = fmaxf(fmaxf(wm[0], wm[1]), fmaxf(wm[2], wm[3]));
-        float t = 0.0f;
-        for (int q = 0; q < 4; q++) t += wm[q] == M ? wsum[q] : wsum[q] * __builtin_amdgcn_exp2f((wm[q] - M) * ZZ_LOG2E);
-        out[W] = zz_beam_sum(M, t);
+    const float lm = fmaxf(fmaxf(lms[l], lms[64 + l]), fmaxf(lms[128 + l], lms[192 + l])), m = zz_wave_max(lm);
+    if (w == 0) {
+        const float line = zz_beam_line(lm, m, W, (float *)cand[0]);
+        if (l == 0) lines = line;
     }
+    const float s = zz_wave_sum(x.sum(m));
+    if (l == 0) wsum[w] = s;
+    __syncthreads();
+    int n = x.gather(lines, cand[w]);
+    if (l == 0) count[w] = n;
+    __syncthreads();
+    int c0 = count[0], c1 = count[1], c2 = count[2], c3 = count[3];
+    if (c0 + c1 + c2 + c3 > 64) {
+        x.rounds(W, cand[w]);
+        __syncthreads();
+        c0 = c1 = c2 = c3 = W;
+    }
+    if (w != 0) return;
+    n = c0 + c1 + c2 + c3;
+    const int q = (l >= c0) + (l >= c0 + c1) + (l >= c0 + c1 + c2);
+    const int before = (q > 0 ? c0 : 0) + (q > 1 ? c1 : 0) + (q > 2 ? c2 : 0);
+    const zz_u64 key = l < n ? cand[q][l - before] : 0;
+    zz_wave_lds();
+    const int rank = zz_beam_place(key, n, cand[0]);
+    zz_u64 *out = a.ws + ((size_t)row * a.chunks + ch) * (W + 1);
+    if (key && rank < W) out[rank] = key;
+    if (l < W && l >= __popcll(__ballot(key != 0))) out[l] = 0;
+    if (l == 0) out[W] = zz_beam_sum(m, (wsum[0] + wsum[1]) + (wsum[2] + wsum[3]));
 }
 
 // The W best of n <= 64 lists of distinct keys (list i at p + i * stride: W keys in order, 0
@@ -296,15 +322,8 @@ __device__ __forceinline__ zz_u64 zz_beam_best(const zz_u64 *p, int stride, int 
         }
         zz_wave_lds();
         key = cand[l];
-    } else {
-        cand[l] = key;
-        zz_wave_lds();
     }
-    int rank = 0;
-    for (int j = 0; j < m; j += 8)
-#pragma unroll
-        for (int u = 0; u < 8; u++) rank += cand[j + u] > key;
-    zz_wave_lds();
+    const int rank = zz_beam_place(key, m, cand);
     cand[l] = 0;
     zz_wave_lds();
     if (key) cand[rank] = key;
@@ -391,22 +410,33 @@ __global__ __launch_bounds__(1024) void zz_beam_merge_kernel(ZzBeamArgs a) {
     zz_beam_finish(a, P, mine, a.chunks, done, c);
 }
 
-// A workgroup per sequence and a wave per beam, for rows that a wave's registers hold. At 2048
-// logits of f32 one launch against two: 5.2 us against 6.8 (1 sequence of 4 beams), 7.3 against
-// 9.1 (32 of 8), 11.3 against 16.2 (64 of 16); in two shares of 2048 each (4096 logits) it lost
-// (9.1 against 8.2), since a wave then waits for its row twice.
+// A workgroup per sequence and a wave per beam, for rows that a wave's registers hold. One launch
+// against two at 2048 f32 logits: 5.1 us against 6.0 (1 sequence of 4 beams), 6.9 against 7.1
+// (1 of 8), 7.5 against 7.9 (32 of 8). Beyond 8 beams a workgroup's waves share their SIMDs and
+// it loses: 8.5 against 7.9 (1 of 12), 10.8 against 8.9 (1 of 16).
 #define ZZ_BEAM_SMALL 2048
 template <typename T>
-__global__ __launch_bounds__(1024) void zz_beam_small_kernel(ZzBeamArgs a) {
+__global__ __launch_bounds__(512) void zz_beam_small_kernel(ZzBeamArgs a) {
     __shared__ ZzBeamPick P;
-    __shared__ zz_u64 lists[ZZ_BEAM_MAXW][ZZ_BEAM_MAXW + 1];
+    __shared__ zz_u64 lists[8][ZZ_BEAM_MAXW + 1];
     const int w = zz_wave_id(), l = threadIdx.x & 63, W = a.W, row = blockIdx.x * W + w;
     const bool done = a.done && a.done[row];
     const float c = a.score[row];
     if (!done) {
-        float m, s;
-        zz_beam_wave<T, ZZ_BEAM_SMALL * sizeof(T) / 1024>((const T *)a.logits + row * a.ldl, a.V, l, 64, W, P.cand[w], lists[w], &m, &s);
-        if (l == 0) lists[w][W] = zz_beam_sum(m, s);
+        ZzBeamShare<T, ZZ_BEAM_SMALL * sizeof(T) / 1024> x((const T *)a.logits + row * a.ldl, a.V, l, 64);
+        zz_u64 *best = lists[w], *cand = P.cand[w];
+        const float lm = x.max(), m = zz_wave_max(lm), s = zz_wave_sum(x.sum(m));
+        const int n = x.gather(zz_beam_line(lm, m, W, (float *)cand), cand);
+        if (l < W) best[l] = 0;
+        if (l == 0) best[W] = zz_beam_sum(m, s);
+        zz_wave_lds();
+        if (n <= 64) {
+            const zz_u64 key = l < n ? cand[l] : 0;
+            const int rank = zz_beam_place(key, n, cand);
+            if (key && rank < W) best[rank] = key;
+        } else {
+            x.rounds(W, best);
+        }
     }
     zz_wave_lds();
     zz_beam_finish(a, P, lists[w], 1, done, c);
@@ -498,7 +528,7 @@ extern "C" int zz_beam_step_dev(int dtype, const void *d_logits, int64_t ldl, in
     }
     if (!zz_lib_here(who)) return 0;
     hipStream_t st = stream ? (hipStream_t)stream : zz_lib_stream();
-    if (V <= ZZ_BEAM_SMALL) {
+    if (V <= ZZ_BEAM_SMALL && W <= 8) {
         const ZzBeamArgs a{d_logits, ldl, N, W, V, 0, eos, pad, d_score, d_done, d_score_out, d_parent, d_token, d_done_out, nullptr};
         if (dtype == ZZ_F32) hipLaunchKernelGGL((zz_beam_small_kernel<float>), dim3(N), dim3(64 * W), 0, st, a);
         else hipLaunchKernelGGL((zz_beam_small_kernel<zz_bf16>), dim3(N), dim3(64 * W), 0, st, a);
