@@ -150,7 +150,8 @@ def case(S, O, I, seed):
 SHAPES = [(1, 1, 1), (1, 16, 128), (2, 17, 129), (1, 2816, 2112), (3, 1000, 1088), (16, 129, 300), (17, 128, 2816),
           (21, 1000, 1088), (33, 257, 511), (64, 704, 2816), (65, 2112, 640), (100, 130, 1000), (128, 256, 256),
           (200, 1500, 700), (256, 512, 128), (300, 257, 1025), (513, 640, 2816), (700, 2816, 704), (1025, 300, 130),
-          (300, 2000, 1100), (2100, 2050, 200), (2500, 2500, 300)]
+          (300, 2000, 1100), (2100, 2050, 200), (2500, 2500, 300), (385, 4697, 603), (1441, 4314, 131),
+          (1025, 4161, 1025), (3651, 3351, 386), (900, 9043, 1323)]
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
@@ -182,7 +183,8 @@ def test_product(dtype, S, O, I):
 @pytest.mark.parametrize("S, O, I, ldy, off", [(5, 130, 200, 133, 0), (40, 130, 200, 200, 1), (300, 130, 200, 136, 0),
                                                (300, 130, 200, 131, 3), (300, 2000, 1100, 2008, 0), (700, 2816, 704, 2817, 5),
                                                (1500, 1500, 600, 1504, 8), (2100, 2050, 200, 2051, 1),
-                                               (2500, 2500, 300, 2501, 0)])
+                                               (2500, 2500, 300, 2501, 0), (385, 4697, 603, 4703, 3),
+                                               (1025, 4161, 700, 4164, 4), (3651, 3351, 386, 3353, 1)])
 def test_product_strides(dtype, S, O, I, ldy, off):
     print("case", S, O, I, ldy, off, dtype, flush=True)
     xq, xs, wq, ws = case(S, O, I, 5)
@@ -203,7 +205,8 @@ def test_product_strides(dtype, S, O, I, ldy, off):
 
 
 @pytest.mark.parametrize("S, O, I", [(70, 300, 300), (300, 2000, 1100), (700, 2816, 704), (1500, 1500, 600),
-                                     (2100, 2050, 200), (2500, 2500, 300)])
+                                     (2100, 2050, 200), (2500, 2500, 300), (385, 4697, 603), (1025, 4161, 700),
+                                     (3651, 3351, 386)])
 def test_product_rows_apart(S, O, I):
     """A row of NaN codes and one of infinite scales touch no other row, in every form."""
     print("case", S, O, I, flush=True)

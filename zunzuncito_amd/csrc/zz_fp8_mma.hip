@@ -198,14 +198,14 @@ __device__ __forceinline__ void zz_wait_vm() {
 // eight 16-byte pieces permuted by (row / 2) % 8 on the way in, so that 16 rows' reads meet 64
 // different banks. One barrier a round. Both operands are made f16 as they leave LDS.
 //
-// At 8192 x 4224 x 2816 (bf16 out) the 128 x 128 tile takes 195 us, 1.00 PFLOP/s; a library
-// f16 product of that shape takes 239 (225 in bf16). Of a round's 1.5 us (two workgroups a
-// CU), 0.85 are matrix work at 2.4 GHz; the clock is 2.0 to 2.2 GHz under it, and for each
-// matrix step a wave issues 3.25 vector operations in 16 cycles (two conversions, one fma).
-// Measured beside it and not better: codes through registers (209), 256 x 128 tiles (206),
-// f16 activations in LDS (217), a fma phase interleaved with the next tile's products (208),
-// touching later lines for the L2 (237). 33 x 64 tiles on 512 places leave the last of five
-// rounds an eighth full.
+// At 8192 x 4224 x 2816 (bf16 out) 128 x 128 tiles take 182 us, 1.07 PFLOP/s (the last 64 of 2112
+// in quarters; whole they leave a fifth round an eighth full, 191 us); a library f16 product of
+// that shape takes 239 (225 in bf16). Of a round's 1.5 us (two workgroups a CU), 0.85 are matrix
+// work at 2.4 GHz; the clock is 2.0 to 2.2 GHz under it, and for each matrix step a wave issues
+// 3.25 vector operations in 16 cycles (two conversions, one fma). Measured beside it and not
+// better (191 then): codes through registers (209), 256 x 128 tiles (206), f16 activations in LDS
+// (217), a fma phase interleaved with the next tile's products (208), touching later lines for
+// the L2 (237).
 template <int RO, int RS, int WO, int WS, int KS, int NS>
 struct ZzF8Async {
     static constexpr int GW = WO * WS, NT = 64 * GW * KS, O = 32 * RO * WO, S = 32 * RS * WS;
@@ -216,19 +216,13 @@ struct ZzF8Async {
     static_assert(LDS >= O * S * 4, "the result's tile");
 };
 
+// one tile: the result's rows from t0 and columns from 32 * gt
 template <typename T, int RO, int RS, int WO, int WS, int KS, int NS>
-__global__ __launch_bounds__(64 * WO * WS * KS, 2) void zz_fp8_async_kernel(ZzF8Mm a) {
+__device__ __forceinline__ void zz_fp8_tile(const ZzF8Mm &a, char *lds, int gt, int t0) {
     typedef ZzF8Async<RO, RS, WO, WS, KS, NS> C;
-    extern __shared__ __attribute__((aligned(1024))) char lds[];
     const int tid = threadIdx.x, l = tid & 63, r = l & 31, h = l >> 5, nb = a.nb;
     const int kg = zz_wave_id() / C::GW, w = zz_wave_id() % C::GW, wo = w % WO, ws = w / WO;
-    const int OT = (a.m.O + C::O - 1) / C::O, ST = (a.S + C::S - 1) / C::S;
-    constexpr int PW = 8;
-    const int id = (blockIdx.x % 8) * (gridDim.x / 8) + blockIdx.x / 8;
-    if (id >= OT * ST) return;
-    const int pan = id / (OT * PW), in = id - pan * OT * PW, pw = min(PW, ST - pan * PW);
-    const int ot = in / pw, st = pan * PW + in % pw;
-    const int gt = ot * WO * RO, g0 = gt + wo * RO, gl = (a.m.O + 31) / 32 - 1, t0 = st * C::S, last = a.S - 1 - t0;
+    const int g0 = gt + wo * RO, gl = (a.m.O + 31) / 32 - 1, last = a.S - 1 - t0;
     const float *wsp = a.m.ws + (size_t)(min(g0, gl) / 4) * nb;
     const unsigned lb = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char *)lds + kg * C::BLOCK;
     // this wave's requests: matrix pieces w*WI .. (4 a group), row octets w*XI .., 64 scales
@@ -349,6 +343,47 @@ __global__ __launch_bounds__(64 * WO * WS * KS, 2) void zz_fp8_async_kernel(ZzF8
     }
 }
 
+// Tile id's place: panels of PW row tiles, whose columns the XCDs go through side by side.
+__device__ __forceinline__ void zz_fp8_at(int id, int OT, int ST, int *ot, int *st) {
+    constexpr int PW = 8;
+    const int pan = id / (OT * PW), in = id - pan * OT * PW, pw = min(PW, ST - pan * PW);
+    *ot = in / pw;
+    *st = pan * PW + in % pw;
+}
+
+template <typename T, int RO, int RS, int WO, int WS, int KS, int NS>
+__global__ __launch_bounds__(64 * WO * WS * KS, 2) void zz_fp8_async_kernel(ZzF8Mm a) {
+    typedef ZzF8Async<RO, RS, WO, WS, KS, NS> C;
+    extern __shared__ __attribute__((aligned(1024))) char lds[];
+    const int OT = (a.m.O + C::O - 1) / C::O, ST = (a.S + C::S - 1) / C::S;
+    const int id = (blockIdx.x % 8) * (gridDim.x / 8) + blockIdx.x / 8;
+    if (id >= OT * ST) return;
+    int ot, st;
+    zz_fp8_at(id, OT, ST, &ot, &st);
+    zz_fp8_tile<T, RO, RS, WO, WS, KS, NS>(a, lds, ot * C::O / 32, st * C::S);
+}
+
+// Tiles of 64 RO x 64 RS; those from `whole` on in parts of 64 x 64, which run as a last round
+// of their own or beside a last round of whole tiles.
+template <typename T, int RO, int RS>
+__global__ __launch_bounds__(256, 2) void zz_fp8_tiles_kernel(ZzF8Mm a, int whole) {
+    extern __shared__ __attribute__((aligned(1024))) char lds[];
+    const int OT = (a.m.O + 64 * RO - 1) / (64 * RO), ST = (a.S + 64 * RS - 1) / (64 * RS);
+    const int g = (whole + 7) / 8, x = blockIdx.x;
+    int ot, st;
+    if (x < 8 * g) {
+        const int id = x % 8 * g + x / 8;
+        if (id >= whole) return;
+        zz_fp8_at(id, OT, ST, &ot, &st);
+        zz_fp8_tile<T, RO, RS, 2, 2, 1, 2>(a, lds, ot * 2 * RO, st * 64 * RS);
+    } else {
+        const int part = (x - 8 * g) % (RO * RS);
+        zz_fp8_at(whole + (x - 8 * g) / (RO * RS), OT, ST, &ot, &st);
+        const int gt = (ot * RO + part % RO) * 2, t0 = (st * RS + part / RO) * 64;
+        if (gt * 32 < a.m.O && t0 < a.S) zz_fp8_tile<T, 1, 1, 2, 2, 1, 3>(a, lds, gt, t0);
+    }
+}
+
 // one 16-byte piece of the packed layout per thread
 __global__ __launch_bounds__(256) void zz_fp8_pack_kernel(const uint8_t *src, int O, int I, int nb, uint8_t *dst,
                                                           int64_t n) {
@@ -388,6 +423,18 @@ static bool launch_async(const ZzF8Mm &a, hipStream_t st) {
     return true;
 }
 
+template <typename T, int RO, int RS>
+static bool launch_tiles(const ZzF8Mm &a, bool split, hipStream_t st) {
+    typedef ZzF8Async<RO, RS, 2, 2, 1, 2> C;
+    typedef ZzF8Async<1, 1, 2, 2, 1, 3> P;
+    const int64_t n = (int64_t)((a.m.O + C::O - 1) / C::O) * ((a.S + C::S - 1) / C::S);
+    const int64_t whole = split ? n - n % 256 : n, g = (whole + 7) / 8 * 8 + (n - whole) * RO * RS;
+    if (g * C::NT > 0xffffffffll) return false;           // a launch's threads in one dimension
+    hipLaunchKernelGGL((zz_fp8_tiles_kernel<T, RO, RS>), dim3((unsigned)g), dim3(C::NT), (C::LDS > P::LDS ? C::LDS : P::LDS),
+                       st, a, (int)whole);
+    return true;
+}
+
 template <typename T, int RG, int RS, int NW, bool PF, bool NT>
 static bool launch_few(const ZzF8Mm &a, hipStream_t st) {
     const dim3 g((a.m.O + 32 * RG - 1) / (32 * RG), (a.S + 32 * RS - 1) / (32 * RS));
@@ -397,30 +444,45 @@ static bool launch_few(const ZzF8Mm &a, hipStream_t st) {
 
 // Which form: the one that is expected to take the shortest. A form's workgroups go round by
 // round through the 256 CUs, `per` of them on a CU at once; a round with k workgroups on the
-// busiest CU takes fix[k-1] + slope[k-1] * (blocks that a K group runs) microseconds, fitted to
-// 89 shapes (O 704 to 65536, I 256 to 8192, S 1 to 8192) with an rms error of 6 to 17 %. Over
-// them the choice lies 2 % behind the best form of each, and up to 15 %. Any one form for all
-// loses far more: the first and the last take 4.8 and 25.6 us for 1 x 4224 x 2816, 295 and 109
-// for 4096 rows.
-struct ZzF8Form { int o, s, ks, per; float fix[4], slope[4]; };
+// busiest CU takes fix[k-1] + slope[k-1] * (blocks that a K group runs) microseconds. A form with
+// `parts` runs what is over a multiple of 256 tiles in that many parts each, if these are at most
+// one a CU: 2.9 + 0.49 * blocks after a full round, or less beside workgroups that are there
+// (`busy`: fixed, a block, a block with a part on each CU). Fitted to 114 shapes (O 704 to 65536,
+// I 256 to 8192, S 1 to 8192) with an rms error of 6 to 17 %. Over them the choice lies 2 % behind
+// the best form of each, and up to 17 %. Any one form for all loses far more: the first and the
+// last but one take 4.8 and 25.6 us for 1 x 4224 x 2816, 295 and 109 for 4096 rows; without the
+// parts 4096 x 4224 x 2816 takes 107 us where it takes 95, 1000 x 4224 x 2816 36 for 30.
+struct ZzF8Form { int o, s, ks, per; float fix[4], slope[4]; int parts; float busy[3]; };
 static const ZzF8Form mm_forms[] = {
     {32, 32, 16, 1, {1.9f}, {2.0f}},
     {32, 32, 4, 4, {2.9f, 2.3f, 2.6f, 0.7f}, {0.52f, 1.14f, 1.64f, 2.11f}},
     {64, 32, 8, 1, {2.6f}, {1.4f}},
+    {64, 32, 2, 4, {2.8f, 3.2f, 2.9f, 2.5f}, {0.64f, 0.80f, 1.16f, 1.43f}},
     {64, 64, 4, 1, {3.4f}, {1.14f}},
     {64, 64, 2, 2, {3.0f, 2.8f}, {0.82f, 1.14f}},
     {64, 64, 1, 3, {2.8f, 3.9f, 2.1f}, {0.49f, 0.66f, 0.95f}},
     {64, 128, 1, 3, {3.4f, 6.0f, 4.0f}, {0.74f, 0.96f, 1.49f}},
+    {64, 128, 1, 3, {3.4f, 6.0f, 4.0f}, {0.74f, 0.96f, 1.49f}, 2, {0.2f, 0.05f, 0.10f}},
     {128, 128, 1, 2, {4.5f, 7.8f}, {1.04f, 1.59f}},
+    {128, 128, 1, 2, {4.5f, 7.8f}, {1.04f, 1.59f}, 4, {1.6f, 0.03f, 0.13f}},
 };
 static int mm_plan(int O, int S, int nb) {
     int best = 0;
     float least = INFINITY;
-    for (int v = 0; v < (int)(sizeof mm_forms / sizeof *mm_forms); v++) {
+    // up to 32 rows the first three: the others' tiles are half empty
+    for (int v = 0; v < (S <= 32 ? 3 : (int)(sizeof mm_forms / sizeof *mm_forms)); v++) {
         const ZzF8Form &f = mm_forms[v];
-        const int64_t n = (int64_t)((O + f.o - 1) / f.o) * ((S + f.s - 1) / f.s);
-        const int r = (nb + f.ks - 1) / f.ks, cap = 256 * f.per, rem = (int)(n % cap);
-        float t = (float)(n / cap) * (f.fix[f.per - 1] + f.slope[f.per - 1] * r);
+        int64_t n = (int64_t)((O + f.o - 1) / f.o) * ((S + f.s - 1) / f.s);
+        const int r = (nb + f.ks - 1) / f.ks, cap = 256 * f.per;
+        float t = 0.0f;
+        if (f.parts) {
+            const int parts = (int)(n % 256) * f.parts;
+            if (!parts || parts > 256) continue;
+            n -= n % 256;
+            t = n % cap ? f.busy[0] + (f.busy[1] + f.busy[2] * parts / 256.0f) * r : 2.9f + 0.49f * r;
+        }
+        const int rem = (int)(n % cap);
+        t += (float)(n / cap) * (f.fix[f.per - 1] + f.slope[f.per - 1] * r);
         if (rem) t += f.fix[(rem - 1) / 256] + f.slope[(rem - 1) / 256] * r;
         if (t < least) {
             least = t;
@@ -441,11 +503,12 @@ static bool launch_mm(const ZzF8Mm &a, hipStream_t st) {
         return a.S <= 8 ? launch_few<T, 1, 1, 8, true, true>(a, st) : launch_few<T, 2, 1, 4, true, true>(a, st);
     if (v == 1) return launch_few<T, 1, 1, 4, true, false>(a, st);
     if (v == 2) return launch_few<T, 2, 1, 8, false, false>(a, st);
-    if (v == 3) return launch_async<T, 1, 2, 2, 1, 4, 2>(a, st);
-    if (v == 4) return launch_async<T, 1, 2, 2, 1, 2, 2>(a, st);
-    if (v == 5) return launch_async<T, 1, 1, 2, 2, 1, 3>(a, st);
-    if (v == 6) return launch_async<T, 1, 2, 2, 2, 1, 2>(a, st);
-    return launch_async<T, 2, 2, 2, 2, 1, 2>(a, st);
+    if (v == 3) return launch_async<T, 1, 1, 2, 1, 2, 2>(a, st);
+    if (v == 4) return launch_async<T, 1, 2, 2, 1, 4, 2>(a, st);
+    if (v == 5) return launch_async<T, 1, 2, 2, 1, 2, 2>(a, st);
+    if (v == 6) return launch_async<T, 1, 1, 2, 2, 1, 3>(a, st);
+    if (v <= 8) return launch_tiles<T, 1, 2>(a, v == 8, st);
+    return launch_tiles<T, 2, 2>(a, v == 10, st);
 }
 
 int zz_launch_fp8_matmul(const ZzF8Mat &m, const uint8_t *q, const float *s, int S, int dtype, void *y,
