@@ -39,9 +39,11 @@ int64_t zz_fp8_row_bytes(int64_t D);
  *   scale = max(max|y|, 2^-100) / 448,  code = e4m3(y / scale), round to nearest even.
  * x, res and sum are of `dtype` with rows ldx, ldr, lds elements apart (0: D); w [D] is
  * f32 (NULL: ones). 1 <= D <= 8192, S <= 2^20. d_sum may be d_x or d_res itself, rows as
- * far apart; the outputs overlap nothing else. d_q is aligned to 16 bytes. A NaN or
- * infinity in a row makes codes of that row NaN or its scales infinite and touches no
- * other row. */
+ * far apart; the outputs overlap nothing else (ranges are judged from their first byte to
+ * their last, what lies between strided rows included). d_q is aligned to 16 bytes. The
+ * squares and their mean are in double, so that no row of finite h leaves their range; a
+ * row of zeros with eps 0 is 0 / 0. A NaN or infinity in a row makes codes of that row NaN
+ * or its scales infinite and touches no other row. */
 int zz_add_norm_fp8_dev(int dtype, const void *d_x, int64_t ldx, const void *d_res, int64_t ldr,
                         void *d_sum, int64_t lds, const float *d_w, float eps, int S, int D,
                         uint8_t *d_q, float *d_s, void *stream);
@@ -53,19 +55,21 @@ int zz_rows_fp8_dev(int dtype, const void *d_x, int64_t ldx, int S, int D, uint8
 
 /* A resident matrix [O, I], O <= 2^24, I <= 65536, O * I < 2^35; returns its id, or -1.
  * Its weights are laid out once, in the matrix cores' order, by an upload (host or device
- * pointers; synchronous; a later upload replaces them, and calls already enqueued on other
- * streams have to be waited for first). */
+ * pointers; synchronous, on the library's stream: what fills d_codes and d_scales on another
+ * stream, and calls with the matrix there, have to be waited for first). A later upload
+ * replaces them. A matrix without an upload has no product; one that a captured graph uses
+ * is destroyed after the graph. */
 int zz_fp8_create(int O, int I);
 void zz_fp8_destroy(int mat);
 int zz_fp8_upload(int mat, const uint8_t *codes, const float *scales);
 int zz_fp8_upload_dev(int mat, const uint8_t *d_codes, const float *d_scales);
 
 /* y [S, O] = rows [S, I] times the matrix's transpose: for each block of 128 columns the
- * codes' product in f32, times the row's and the matrix block's scale, added up in f32 in
- * the order of the columns or of groups of them; rounded once to `dtype`. Rows of y are
- * ldy elements apart (0: O); what lies between them is left as it was. S <= 2^20, S * O < 2^37. d_q is
- * aligned to 16 bytes. Results do not depend on other rows' values and are the same on
- * every call. */
+ * codes' product in f32, times the f32 product of the row's and the block's scale, added up
+ * in f32 in the order of the columns or of groups of them; rounded once to `dtype`. Rows of
+ * y are ldy elements apart (0: O); what lies between them is left as it was. S <= 2^20,
+ * S * O < 2^37. d_q is aligned to 16 bytes. Results do not depend on other rows' values and
+ * are the same on every call of the same sizes. */
 int zz_fp8_matmul_dev(int mat, const uint8_t *d_q, const float *d_s, int S, int dtype, void *d_y,
                       int64_t ldy, void *stream);
 

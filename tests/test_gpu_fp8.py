@@ -67,6 +67,23 @@ def test_add_norm(dtype, S, D):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("D", [5, 300, 2816])
+def test_add_norm_range(dtype, D):
+    """Rows whose squares 32 bits do not hold, with and without eps."""
+    x, _, w = inputs(6, D, dtype, D)
+    x = (x.float() * torch.tensor([1e-38, 1e-30, 1e-18, 1.0, 1e19, 1e36])[:, None]).to(dtype)
+    X, Wt = x.cuda(), w.cuda()
+    for eps in (0.0, 1e-6):
+        q, s = buffers(6, D)
+        zz.add_norm_fp8_dev(X.data_ptr(), 0, 0, Wt.data_ptr(), 6, D, eps, q.data_ptr(), s.data_ptr(), KIND[dtype],
+                            stream=stream())
+        qh, sh = taken(q, s, 6, D)
+        h, y = R.norm_rows(x, None, w, float(np.float32(eps)))
+        assert np.isfinite(y).all()
+        R.check_rows(y, qh, sh, R.norm_delta(D))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("D, ldx, off", [(2816, 5632, 0), (200, 203, 0), (256, 512, 1), (129, 160, 3)])
 def test_add_norm_strides_and_in_place(dtype, D, ldx, off):
     """Rows apart, a start that no vector load fits, sum stored over res and over x."""

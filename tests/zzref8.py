@@ -59,10 +59,9 @@ def check_rows(y, q, s, delta):
 
 
 def norm_delta(D):
-    """How far a row's y may be off: a thread's chain of at most 32 squares and fma's (its sum
-    is off by 32 U, the root by half of that), the sum's rounding to f32 and the addition of
-    eps (half of each), the root, the reciprocal, and the two products."""
-    return (16 + 1 + 4) * U
+    """How far a row's y may be off: the squares, their sum and the root are in 64 bits; the
+    reciprocal's rounding to f32 and the two products are half a step each."""
+    return 3 * U + D * 2.0 ** -52
 
 
 def product(xq, xs, wq, ws, O, I):
