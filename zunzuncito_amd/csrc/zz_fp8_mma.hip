@@ -85,7 +85,7 @@ struct ZzF8Mm {
 // codes requested before the current one is multiplied), and meet in LDS, where the partial
 // sums are added in the waves' order. Rows behind the last one are read as the last one, and
 // not stored. NT: the matrix is read once and does not stay in the caches: 3 rows against
-// 262144 x 2816 in 107 us, 6.9 TB/s, instead of 120.
+// 262144 x 2816 in 104 us, 7.1 TB/s, instead of 120.
 template <typename T, int RG, int RS, int NW, bool PF, bool NT>
 __global__ __launch_bounds__(64 * NW) void zz_fp8_few_kernel(ZzF8Mm a) {
     extern __shared__ __attribute__((aligned(16))) float part[];     // [NW][RG][RS][16][64]
@@ -201,11 +201,11 @@ __device__ __forceinline__ void zz_wait_vm() {
 // At 8192 x 4224 x 2816 (bf16 out) 128 x 128 tiles take 182 us, 1.07 PFLOP/s (the last 64 of 2112
 // in quarters; whole they leave a fifth round an eighth full, 191 us); a library f16 product of
 // that shape takes 239 (225 in bf16). Of a round's 1.5 us (two workgroups a CU), 0.85 are matrix
-// work at 2.4 GHz; the clock is 2.0 to 2.2 GHz under it, and for each matrix step a wave issues
-// 3.25 vector operations in 16 cycles (two conversions, one fma). Measured beside it and not
-// better (191 then): codes through registers (209), 256 x 128 tiles (206), f16 activations in LDS
-// (217), a fma phase interleaved with the next tile's products (208), touching later lines for
-// the L2 (237).
+// work at 2.4 GHz; the clock is 2.0 to 2.2 GHz under it, and for 16 cycles of matrix work a wave
+// issues 3.25 vector operations (two conversions, one fma). Measured beside it and not better
+// (191 then): codes through registers (209), 256 x 128 tiles (206), f16 activations in LDS (217),
+// a fma phase interleaved with the next tile's products (208), touching later lines for the L2
+// (237).
 template <int RO, int RS, int WO, int WS, int KS, int NS>
 struct ZzF8Async {
     static constexpr int GW = WO * WS, NT = 64 * GW * KS, O = 32 * RO * WO, S = 32 * RS * WS;
