@@ -6,6 +6,7 @@
 #include "../../include/zz_fp8.h"
 
 #include <math.h>
+#include <new>
 #include <vector>
 
 #define ZZ_FAIL(...)               \
@@ -133,7 +134,16 @@ extern "C" int zz_fp8_create(int O, int I) {
         return -1;
     }
     if (!zz_lib_here("zz_fp8_create")) return -1;
-    Fp8Mat *m = new Fp8Mat();
+    size_t id = 0;
+    while (id < g_mats.size() && g_mats[id]) id++;
+    Fp8Mat *m = nullptr;
+    try {
+        if (id == g_mats.size()) g_mats.push_back(nullptr);
+        m = new Fp8Mat();
+    } catch (const std::bad_alloc &) {
+        zz_set_error("zz_fp8_create: out of memory");
+        return -1;
+    }
     m->O = O;
     m->I = I;
     if (hipMalloc(&m->w, packed_bytes(m)) != hipSuccess || hipMalloc(&m->ws, 4 * scale_count(m)) != hipSuccess) {
@@ -142,10 +152,8 @@ extern "C" int zz_fp8_create(int O, int I) {
         free_mat(m);
         return -1;
     }
-    for (size_t i = 0; i < g_mats.size(); i++)
-        if (!g_mats[i]) { g_mats[i] = m; return (int)i; }
-    g_mats.push_back(m);
-    return (int)g_mats.size() - 1;
+    g_mats[id] = m;
+    return (int)id;
 }
 
 extern "C" void zz_fp8_destroy(int id) {
