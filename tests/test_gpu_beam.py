@@ -108,6 +108,30 @@ def test_step_widest():
     check(logits, score, None, N, W, V)
 
 
+def test_step_and_reorder_past_32_bits():
+    """Logits and states at offsets that 32 bits do not hold: some sequences of many, against
+    64 bits and against the rows moved one by one."""
+    N, W, V = 1200, 16, 131072
+    g = torch.Generator(device="cuda").manual_seed(2)
+    logits = torch.empty(N * W, V, dtype=BF16, device="cuda").normal_(generator=g)
+    score = -torch.rand(N, W, device="cuda", generator=g)
+    so, pa, tk = torch.empty_like(score), *(torch.empty(N, W, dtype=torch.int32, device="cuda") for _ in range(2))
+    do = torch.empty(N, W, dtype=torch.uint8, device="cuda")
+    ws = torch.empty(zz.beam_ws_bytes(N, W, V), dtype=torch.uint8, device="cuda")
+    zz.beam_step_dev(logits.data_ptr(), N, W, V, score.data_ptr(), so.data_ptr(), pa.data_ptr(), tk.data_ptr(), ws.data_ptr(),
+                     ws.numel(), d_done_out=do.data_ptr(), eos=1, dtype=zz.ZZ_BF16, stream=stream())
+    torch.cuda.synchronize()
+    for n in (0, N // 2, N - 1):
+        got = [t[n:n + 1].cpu() for t in (so, pa, tk, do)]
+        R.check_beam(logits[n * W:(n + 1) * W].cpu(), score[n:n + 1].cpu(), None, 0, 1, 1, W, got)
+    states = logits.view(N, W, V)                        # as states of 256 KB a beam, in place
+    keep = states[:, :, ::4099].clone()
+    zz.beam_reorder_dev(logits.data_ptr(), logits.data_ptr(), pa.data_ptr(), N, W, row_stride=2 * V, row_bytes=2 * V - 6,
+                        stream=stream())
+    torch.cuda.synchronize()
+    assert torch.equal(states[:, :, ::4099], torch.gather(keep, 1, pa.long()[:, :, None].expand_as(keep)))
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("V, ldl, off", [(1001, 1001, 1), (1001, 1010, 3), (9000, 9001, 0), (4096, 8192, 4)])
 def test_step_strides(dtype, V, ldl, off):
@@ -395,6 +419,8 @@ def test_stack_search(W, eos, flash):
         assert seq.view(-1)[:W].cpu().tolist() == [17] * W
         with pytest.raises(RuntimeError, match="W <= 16"):
             stack.beam_dev(start.data_ptr(), 17, n, seq.data_ptr(), score.data_ptr(), stream=stream())
+        with pytest.raises(RuntimeError, match="overlaps"):
+            stack.beam_dev(seq.data_ptr() + 4 * n, W, n, seq.data_ptr(), score.data_ptr(), stream=stream())
     finally:
         stack.close()
         head.close()

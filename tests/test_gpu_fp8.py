@@ -383,3 +383,37 @@ def test_product_large_matrix(S):
             assert np.all(off <= R.product_bound(mag, want, I, F32))
     finally:
         m.close()
+
+
+def test_rows_and_product_past_32_bits():
+    """The most rows, at offsets that 32 bits do not hold: norm, rounding and product of the
+    first, the last and some between against 64 bits."""
+    S, D, O = 1 << 20, 2200, 40
+    at = [0, 1, S // 2 - 1, S - 33, S - 1]
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.empty(S, D, dtype=BF16, device="cuda").normal_(generator=g)
+    sm = torch.empty_like(x)
+    nb = R.blocks(D)
+    q = torch.empty(S, nb * 128, dtype=torch.uint8, device="cuda")
+    s = torch.empty(nb, S, device="cuda")
+    zz.add_norm_fp8_dev(x.data_ptr(), x.data_ptr(), sm.data_ptr(), 0, S, D, 1e-6, q.data_ptr(), s.data_ptr(), zz.ZZ_BF16,
+                        stream=stream())
+    torch.cuda.synchronize()
+    xh = x[at].cpu()
+    h, y = R.norm_rows(xh, xh, None, float(np.float32(1e-6)))
+    R.check_rows(y, q[at].cpu(), s[:, at].cpu(), R.norm_delta(D))
+    assert torch.equal(sm[at].cpu(), torch.from_numpy(h).float().to(BF16))
+    zz.rows_fp8_dev(x.data_ptr(), S, D, q.data_ptr(), s.data_ptr(), zz.ZZ_BF16, stream=stream())
+    torch.cuda.synchronize()
+    R.check_rows(xh.double().numpy(), q[at].cpu(), s[:, at].cpu(), 0.0)
+    _, _, wq, ws = case(1, O, D, 6)
+    m = zz.Fp8Matrix(O, D)
+    try:
+        m.upload(wq, ws)
+        out = torch.empty(S, O, device="cuda")
+        m.matmul_dev(q.data_ptr(), s.data_ptr(), S, out.data_ptr(), stream=stream())
+        torch.cuda.synchronize()
+        want, mag = R.product(q[at].cpu().numpy(), s[:, at].cpu().numpy(), wq, ws, O, D)
+        assert np.all(np.abs(out[at].double().cpu().numpy() - want) <= R.product_bound(mag, want, D, F32))
+    finally:
+        m.close()
