@@ -10,8 +10,9 @@
 //                         and sums (in double), then one wave picks the W best totals
 // or, for a small vocabulary, one: zz_beam_small_kernel, whose waves make their beams' lists
 // themselves. A step of 16 sequences of 8 beams over 262144 f32 logits takes 32 us, 134 MB at
-// 4.2 TB/s, 25 us of it in the first launch at 5.4 TB/s; in bf16 28.7 us, bound by the work on an
-// element (maximum, exponential, comparison) and by what a chunk does after them.
+// 4.2 TB/s, 26 us of it in the first launch at 5.2 TB/s; in bf16 29 us. There it is the chain of
+// a chunk's steps, at five workgroups a CU, and neither bytes nor instructions: without the
+// instructions that make NaN harmless it took as long.
 #include "zz_common.h"
 #include "zz_kernels.h"
 #include "zz_fp8_dev.h"
