@@ -417,3 +417,27 @@ def test_rows_and_product_past_32_bits():
         assert np.all(np.abs(out[at].double().cpu().numpy() - want) <= R.product_bound(mag, want, D, F32))
     finally:
         m.close()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("D", [1, 7, 9, 500, 511, 513, 1023, 1025, 2047, 4097])
+def test_rows_of_other_widths(dtype, D):
+    """Few threads a row and many, rows that share a workgroup, a last group that reads on into
+    the next row: what follows a row's end, and the buffer's, is NaN."""
+    for S in (1, 2, 3, 5):
+        x, res, w = inputs(S, D, dtype, 7 * S + D, 2)
+        nan = torch.full((1,), float("nan"), dtype=dtype)
+        x[:, D:], res[:, D:] = nan, nan
+        X, Rs, Wt = (torch.cat([t.view(-1).to(t.dtype), torch.full((64,), float("nan"), dtype=t.dtype)]).cuda() for t in (x, res, w))
+        q, s = buffers(S, D)
+        sm = torch.full((S, 2 * D), -5.0, dtype=dtype, device="cuda")
+        zz.add_norm_fp8_dev(X.data_ptr(), Rs.data_ptr(), sm.data_ptr(), Wt.data_ptr(), S, D, 1e-6, q.data_ptr(), s.data_ptr(),
+                            KIND[dtype], ldx=2 * D, ldr=2 * D, lds=2 * D, stream=stream())
+        qh, sh = taken(q, s, S, D)
+        h, y = R.norm_rows(x[:, :D], res[:, :D], w, float(np.float32(1e-6)))
+        R.check_rows(y, qh, sh, R.norm_delta(D))
+        assert torch.equal(sm[:, :D].cpu(), torch.from_numpy(h).float().to(dtype)) and bool((sm[:, D:] == -5.0).all())
+        q, s = buffers(S, D)
+        zz.rows_fp8_dev(X.data_ptr(), S, D, q.data_ptr(), s.data_ptr(), KIND[dtype], ldx=2 * D, stream=stream())
+        qh, sh = taken(q, s, S, D)
+        R.check_rows(x[:, :D].double().numpy(), qh, sh, 0.0)

@@ -443,38 +443,40 @@ __global__ __launch_bounds__(512) void zz_beam_small_kernel(ZzBeamArgs a) {
     zz_beam_finish(a, P, lists[w], 1, done, c);
 }
 
-// A thread owns one piece G of a row's bytes in all W rows of a sequence: it reads what
-// the W beams continue, then writes, so that moving in place needs no second buffer. Rows
-// that stay where they are move nothing in place.
+// A thread owns 16 bytes of a row, at any alignment, in all W rows of a sequence: it reads what
+// the W beams continue, then writes, so that moving in place needs no second buffer. Rows that
+// stay where they are move nothing in place. The first workgroup moves the bytes behind the last
+// whole piece as well.
 // NT: the rows are stored past the caches, which their own dirty lines would fill (16 x 8 beams
 // with 0.26 GB of states: the next step's pass over 134 MB of logits took 43 us instead of 32).
-template <typename G, int WM, bool NT>
+template <int WM, bool NT>
 __global__ __launch_bounds__(256) void zz_beam_reorder_kernel(uint8_t *dst, const uint8_t *src, const int *parent, int W,
-                                                              int64_t ostride, int64_t rstride, int64_t first,
-                                                              int64_t pieces) {
+                                                              int64_t ostride, int64_t rstride, int64_t bytes) {
     const int n = blockIdx.y, tid = threadIdx.x;
-    const int64_t o = blockIdx.z;
-    const int64_t base = o * ostride + (int64_t)n * W * rstride + first;
+    const int64_t base = blockIdx.z * ostride + (int64_t)n * W * rstride, pieces = bytes / 16;
     int par[WM];
 #pragma unroll
     for (int w = 0; w < WM; w++) {
         const int p = w < W ? parent[n * W + w] : w;
         par[w] = p >= 0 && p < W ? p : w;
     }
-    for (int64_t i = (int64_t)blockIdx.x * 256 + tid; i < pieces; i += (int64_t)gridDim.x * 256) {
-        const int64_t at = base + i * (int64_t)sizeof(G);
+    auto move = [&](auto piece, auto store, int64_t at) {
+        typedef decltype(piece) G;
         G v[WM];
 #pragma unroll
         for (int w = 0; w < WM; w++)
             if (w < W && (dst != src || par[w] != w)) v[w] = *(const G *)(src + at + par[w] * rstride);
 #pragma unroll
         for (int w = 0; w < WM; w++)
-            if (w < W && (dst != src || par[w] != w)) {
-                G *to = (G *)(dst + at + w * rstride);
-                if constexpr (NT) __builtin_nontemporal_store(v[w], to);
-                else *to = v[w];
-            }
-    }
+            if (w < W && (dst != src || par[w] != w)) store(v[w], (G *)(dst + at + w * rstride));
+    };
+    for (int64_t i = (int64_t)blockIdx.x * 256 + tid; i < pieces; i += (int64_t)gridDim.x * 256)
+        move(zz_u4any{}, [](zz_u4any v, zz_u4any *to) {
+            if constexpr (NT) __builtin_nontemporal_store(v, to);
+            else *to = v;
+        }, base + i * 16);
+    if (blockIdx.x == 0 && pieces * 16 + tid < bytes)
+        move(uint8_t{}, [](uint8_t v, uint8_t *to) { *to = v; }, base + pieces * 16 + tid);
 }
 
 // ------------------------------------------------------------------ host side
@@ -554,16 +556,14 @@ extern "C" int zz_beam_step_dev(int dtype, const void *d_logits, int64_t ldl, in
     return 1;
 }
 
-template <typename G, bool NT>
+template <bool NT>
 static void launch_reorder(uint8_t *dst, const uint8_t *src, const int *parent, int N, int W, int64_t outer,
-                           int64_t ostride, int64_t rstride, int64_t first, int64_t pieces, hipStream_t st) {
-    int64_t gx = (pieces + 255) / 256;
-    if (gx > 1024) gx = 1024;
-    const auto k = W <= 4 ? zz_beam_reorder_kernel<G, 4, NT>
-                          : W <= 8 ? zz_beam_reorder_kernel<G, 8, NT> : zz_beam_reorder_kernel<G, 16, NT>;
+                           int64_t ostride, int64_t rstride, int64_t bytes, hipStream_t st) {
+    const int64_t gx = bytes < 256 * 16 ? 1 : bytes / 16 > 1024 * 256 ? 1024 : (bytes / 16 + 255) / 256;
+    const auto k = W <= 4 ? zz_beam_reorder_kernel<4, NT> : W <= 8 ? zz_beam_reorder_kernel<8, NT> : zz_beam_reorder_kernel<16, NT>;
     for (int64_t o = 0; o < outer; o += 65535)                   // a grid's z dimension
         hipLaunchKernelGGL(k, dim3((unsigned)gx, N, (unsigned)(outer - o < 65535 ? outer - o : 65535)), dim3(256), 0, st,
-                           dst + o * ostride, src + o * ostride, parent, W, ostride, rstride, first, pieces);
+                           dst + o * ostride, src + o * ostride, parent, W, ostride, rstride, bytes);
 }
 
 extern "C" int zz_beam_reorder_dev(void *d_dst, const void *d_src, const int *d_parent, int N, int W, int64_t outer,
@@ -584,17 +584,8 @@ extern "C" int zz_beam_reorder_dev(void *d_dst, const void *d_src, const int *d_
     hipStream_t st = stream ? (hipStream_t)stream : zz_lib_stream();
     uint8_t *d = (uint8_t *)d_dst;
     const uint8_t *s = (const uint8_t *)d_src;
-    // pieces as wide as every row's alignment allows, then the bytes behind the last whole one
-    const uintptr_t al = (uintptr_t)d | (uintptr_t)s | (uintptr_t)row_stride | (outer > 1 ? (uintptr_t)outer_stride : 0);
-    const int64_t gsz = al % 16 == 0 ? 16 : al % 4 == 0 ? 4 : 1, body = row_bytes / gsz, tail = row_bytes - body * gsz;
-    auto move = [&](auto launch, int64_t first, int64_t n) {
-        if (n) launch(d, s, d_parent, N, W, outer, outer_stride, row_stride, first, n, st);
-    };
-    if (gsz == 16 && outer * R * row_bytes >= ZZ_NT_BYTES) move(launch_reorder<zz_u4, true>, 0, body);
-    else if (gsz == 16) move(launch_reorder<zz_u4, false>, 0, body);
-    else if (gsz == 4) move(launch_reorder<unsigned, false>, 0, body);
-    else move(launch_reorder<uint8_t, false>, 0, body);
-    move(launch_reorder<uint8_t, false>, body * gsz, tail);
+    if (outer * R * row_bytes >= ZZ_NT_BYTES) launch_reorder<true>(d, s, d_parent, N, W, outer, outer_stride, row_stride, row_bytes, st);
+    else launch_reorder<false>(d, s, d_parent, N, W, outer, outer_stride, row_stride, row_bytes, st);
     if (hipGetLastError() != hipSuccess) ZZ_FAIL("%s: launch failed", who);
     return 1;
 }

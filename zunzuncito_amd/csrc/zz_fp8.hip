@@ -78,9 +78,7 @@ extern "C" int zz_add_norm_fp8_dev(int dtype, const void *d_x, int64_t ldx, cons
         bad |= d_w && zz_ranges_meet(d_sum, nu, d_w, nw);
     }
     if (bad) ZZ_FAIL("%s: an output overlaps another argument", who);
-    ZzF8RowsArgs a{d_x, d_res, d_sum, d_w, ldx, ldr, lds, eps, S, D, 0, nu >= ZZ_NT_BYTES, d_q, d_s};
-    auto at16 = [&](const void *p, int64_t ld) { return !p || ((uintptr_t)p % 16 == 0 && ld * esz % 16 == 0); };
-    a.vec = at16(d_x, ldx) && at16(d_res, ldr) && at16(d_sum, lds) && (uintptr_t)d_w % 16 == 0;
+    const ZzF8RowsArgs a{d_x, d_res, d_sum, d_w, ldx, ldr, lds, eps, S, D, nu >= ZZ_NT_BYTES, d_q, d_s};
     if (!zz_lib_here(who)) return 0;
     if (!zz_launch_add_norm_fp8(dtype, a, stream ? (hipStream_t)stream : zz_lib_stream()))
         ZZ_FAIL("%s: launch failed", who);
@@ -96,8 +94,7 @@ extern "C" int zz_rows_fp8_dev(int dtype, const void *d_x, int64_t ldx, int S, i
     const int64_t nx = span(ldx, S, D, esz), nq = S * zz_fp8_row_bytes(D), ns = (int64_t)zz_f8_nb(D) * S * 4;
     if (zz_ranges_meet(d_q, nq, d_x, nx) || zz_ranges_meet(d_s, ns, d_x, nx) || zz_ranges_meet(d_q, nq, d_s, ns))
         ZZ_FAIL("%s: an output overlaps another argument", who);
-    ZzF8RowsArgs a{d_x, nullptr, nullptr, nullptr, ldx, 0, 0, 0.0f, S, D, 0, 0, d_q, d_s};
-    a.vec = (uintptr_t)d_x % 16 == 0 && ldx * esz % 16 == 0;
+    const ZzF8RowsArgs a{d_x, nullptr, nullptr, nullptr, ldx, 0, 0, 0.0f, S, D, 0, d_q, d_s};
     if (!zz_lib_here(who)) return 0;
     if (!zz_launch_rows_fp8(dtype, a, stream ? (hipStream_t)stream : zz_lib_stream())) ZZ_FAIL("%s: launch failed", who);
     return 1;

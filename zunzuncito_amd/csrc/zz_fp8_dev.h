@@ -22,33 +22,44 @@ __device__ __forceinline__ unsigned zz_bf16_bits(float f) {
 __device__ __forceinline__ void zz_put(float *p, float v) { *p = v; }
 __device__ __forceinline__ void zz_put(zz_bf16 *p, float v) { p->u = (uint16_t)zz_bf16_bits(v); }
 
-// n (<= 8) consecutive elements as f32, zero behind them. VEC: all 8 lie inside, at 16 bytes
-template <bool VEC, typename T>
-__device__ __forceinline__ void zz_get8(float (&v)[8], const T *p, int n) {
-    if (VEC && n >= 8) {
+// Four words at any address: rows of odd widths and strides begin at any multiple of their
+// element, and the vector memory takes 16 bytes from there as well (by elements, a norm of 543 x
+// 5035 bf16 rows took 21 us where it takes 9.5, a product of 6183 x 2889 x 176 34 where 22).
+typedef unsigned zz_u4 __attribute__((ext_vector_type(4)));
+typedef unsigned zz_u4any __attribute__((ext_vector_type(4), aligned(1), may_alias));
+typedef unsigned zz_u2any __attribute__((ext_vector_type(2), aligned(1), may_alias));
+
+// n (<= 8) consecutive elements as f32, zero behind them. over: 8 may be read all the same
+template <typename T>
+__device__ __forceinline__ void zz_get8(float (&v)[8], const T *p, int n, bool over) {
+    if (n >= 8 || (over && n > 0)) {
+        const zz_u4 a = *(const zz_u4any *)p;
         if constexpr (sizeof(T) == 4) {
-            const float4 a = *(const float4 *)p, b = *(const float4 *)(p + 4);
-            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-            v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-        } else {
-            const uint4 a = *(const uint4 *)p;
-            const unsigned w[4] = {a.x, a.y, a.z, a.w};
+            const zz_u4 b = *((const zz_u4any *)p + 1);
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                v[2 * j] = __uint_as_float(w[j] << 16);
-                v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+                v[j] = __uint_as_float(a[j]);
+                v[4 + j] = __uint_as_float(b[j]);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                v[2 * j] = __uint_as_float(a[j] << 16);
+                v[2 * j + 1] = __uint_as_float(a[j] & 0xffff0000u);
             }
         }
+        if (n < 8)
+#pragma unroll
+            for (int j = 1; j < 8; j++) v[j] = j < n ? v[j] : 0.0f;
         return;
     }
 #pragma unroll
     for (int j = 0; j < 8; j++) v[j] = j < n ? zz_f32_of(p[j]) : 0.0f;
 }
-typedef unsigned zz_u4 __attribute__((ext_vector_type(4)));
-// nt: stores that are not kept in the caches
-template <bool VEC, typename T>
-__device__ __forceinline__ void zz_put8(T *p, const float (&v)[8], int n, bool nt) {
-    if (VEC && n >= 8) {
+// NT: stores that are not kept in the caches
+template <bool NT, typename T>
+__device__ __forceinline__ void zz_put8(T *p, const float (&v)[8], int n) {
+    if (n >= 8) {
         zz_u4 w[sizeof(T) / 2];
         if constexpr (sizeof(T) == 4) {
 #pragma unroll
@@ -59,8 +70,8 @@ __device__ __forceinline__ void zz_put8(T *p, const float (&v)[8], int n, bool n
         }
 #pragma unroll
         for (int j = 0; j < (int)(sizeof(T) / 2); j++) {
-            if (nt) __builtin_nontemporal_store(w[j], (zz_u4 *)p + j);
-            else ((zz_u4 *)p)[j] = w[j];
+            if constexpr (NT) __builtin_nontemporal_store((zz_u4any)w[j], (zz_u4any *)p + j);
+            else *((zz_u4any *)p + j) = w[j];
         }
         return;
     }
@@ -80,7 +91,7 @@ struct ZzF8RowsArgs {
     const float *w;
     int64_t ldx, ldr, lds;      // elements
     float eps;
-    int S, D, vec;              // vec: every full group of 8 lies at 16 bytes
+    int S, D;
     int nt;                     // the sum is stored past the caches
     uint8_t *q;                 // [S][nb * 128]
     float *s;                   // [nb][S]

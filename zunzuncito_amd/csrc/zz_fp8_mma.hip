@@ -43,12 +43,13 @@ __device__ __forceinline__ zz_v16f zz_f8_zero() {
 
 // matrix rows o..o+3 of activation row t
 template <typename T>
-__device__ __forceinline__ void zz_f8_store4(T *y, int64_t ldy, int t, int o, int O, bool vec, const float (&v)[4]) {
+__device__ __forceinline__ void zz_f8_store4(T *y, int64_t ldy, int t, int o, int O, const float (&v)[4]) {
     T *p = y + (int64_t)t * ldy + o;
-    if (vec && o + 4 <= O) {
-        if constexpr (sizeof(T) == 4) *(float4 *)p = make_float4(v[0], v[1], v[2], v[3]);
-        else *(uint2 *)p = make_uint2(zz_bf16_bits(v[0]) | zz_bf16_bits(v[1]) << 16,
-                                      zz_bf16_bits(v[2]) | zz_bf16_bits(v[3]) << 16);
+    if (o + 4 <= O) {
+        if constexpr (sizeof(T) == 4)
+            *(zz_u4any *)p = zz_u4any{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
+        else
+            *(zz_u2any *)p = zz_u2any{zz_bf16_bits(v[0]) | zz_bf16_bits(v[1]) << 16, zz_bf16_bits(v[2]) | zz_bf16_bits(v[3]) << 16};
         return;
     }
 #pragma unroll
@@ -58,12 +59,15 @@ __device__ __forceinline__ void zz_f8_store4(T *y, int64_t ldy, int t, int o, in
 
 // 16 bytes of a result row, n of its elements inside the row
 template <typename T>
-__device__ __forceinline__ void zz_f8_store(T *p, const float (&v)[16 / sizeof(T)], int n, bool vec) {
+__device__ __forceinline__ void zz_f8_store(T *p, const float (&v)[16 / sizeof(T)], int n) {
     constexpr int E = 16 / sizeof(T);
-    if (vec && n >= E) {
-        if constexpr (E == 4) *(float4 *)p = make_float4(v[0], v[1], v[2], v[3]);
-        else *(uint4 *)p = make_uint4(zz_bf16_bits(v[0]) | zz_bf16_bits(v[1]) << 16, zz_bf16_bits(v[2]) | zz_bf16_bits(v[3]) << 16,
-                                      zz_bf16_bits(v[4]) | zz_bf16_bits(v[5]) << 16, zz_bf16_bits(v[6]) | zz_bf16_bits(v[7]) << 16);
+    if (n >= E) {
+        zz_u4any w;
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if constexpr (E == 4) w[j] = __float_as_uint(v[j]);
+            else w[j] = zz_bf16_bits(v[2 * j]) | zz_bf16_bits(v[2 * j + 1]) << 16;
+        *(zz_u4any *)p = w;
         return;
     }
 #pragma unroll
@@ -75,7 +79,7 @@ struct ZzF8Mm {
     ZzF8Mat m;
     const uint8_t *q;
     const float *s;
-    int S, nb, vec;
+    int S, nb;
     void *y;
     int64_t ldy;
 };
@@ -170,7 +174,7 @@ __global__ __launch_bounds__(64 * NW) void zz_fp8_few_kernel(ZzF8Mm a) {
         for (int u = 0; u < NW; u++)
 #pragma unroll
             for (int e = 0; e < 4; e++) v[e] += part[u * TL + ((i * RS + j) * 16 + 4 * k + e) * 64 + l];
-        zz_f8_store4((T *)a.y, a.ldy, t, 32 * (g0 + i) + 8 * k + 4 * h, a.m.O, a.vec, v);
+        zz_f8_store4((T *)a.y, a.ldy, t, 32 * (g0 + i) + 8 * k + 4 * h, a.m.O, v);
     }
 }
 
@@ -339,7 +343,7 @@ __device__ __forceinline__ void zz_fp8_tile(const ZzF8Mm &a, char *lds, int gt, 
         float v[E];
 #pragma unroll
         for (int e = 0; e < E; e += 4) *(float4 *)(v + e) = *(const float4 *)place(t, o + e);
-        zz_f8_store((T *)a.y + (int64_t)(t0 + t) * a.ldy + gt * 32 + o, v, a.m.O - gt * 32 - o, a.vec);
+        zz_f8_store((T *)a.y + (int64_t)(t0 + t) * a.ldy + gt * 32 + o, v, a.m.O - gt * 32 - o);
     }
 }
 
@@ -513,8 +517,6 @@ static bool launch_mm(const ZzF8Mm &a, hipStream_t st) {
 
 int zz_launch_fp8_matmul(const ZzF8Mat &m, const uint8_t *q, const float *s, int S, int dtype, void *y,
                          int64_t ldy, hipStream_t st) {
-    const int esz = dtype == 0 ? 4 : 2;
-    ZzF8Mm a{m, q, s, S, zz_f8_nb(m.I), 0, y, ldy};
-    a.vec = (uintptr_t)y % 16 == 0 && ldy * esz % 16 == 0;
+    const ZzF8Mm a{m, q, s, S, zz_f8_nb(m.I), y, ldy};
     return (dtype == 0 ? launch_mm<float>(a, st) : launch_mm<zz_bf16>(a, st)) && hipGetLastError() == hipSuccess;
 }

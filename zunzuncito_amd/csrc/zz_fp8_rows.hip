@@ -31,12 +31,19 @@ __device__ __forceinline__ uint2 zz_f8_block(const float (&y)[8], float *scale) 
 
 // 8192 x 2816 in f32 take 58 us, 5.2 TB/s, which is what a large copy reaches (63 with the sum
 // kept in the caches); one row 3.3 us, a launch's 2.2 and one trip to memory.
-// One workgroup per row, NU groups of 8 per thread held in registers between the sum of
-// squares and the codes: x and res are read once, sum and codes written once.
-template <typename T, int NU, bool VEC>
+// TPR threads per row, NU groups of 8 per thread held in registers between the sum of squares
+// and the codes: x and res are read once, sum and codes written once. As few threads as hold a
+// row with one group each, at least a wave: 6000 x 512 bf16 rows take 6.9 us with a wave each
+// and 11.8 with four, 6000 x 1024 10.9 with two and 13.3 with four; with fewer threads and two
+// groups each a single row takes longer (1024: 3.4 for 2.7).
+// In 16 bits a row's last group, where 8 do not divide the width, reads on into the next row,
+// which the last row has not (6000 x 742: 11.4 us for 14.5; in f32 it lost, 13.7 for 13.0).
+template <typename T, int TPR, int NU, bool NT>
 __global__ __launch_bounds__(256) void zz_add_norm_fp8_kernel(ZzF8RowsArgs a) {
     __shared__ double red[4];
-    const int row = blockIdx.x, tid = threadIdx.x, D = a.D, nb = zz_f8_nb(D);
+    const int tid = threadIdx.x % TPR, D = a.D, nb = zz_f8_nb(D);
+    const int own = TPR == 256 ? blockIdx.x : blockIdx.x * (256 / TPR) + threadIdx.x / TPR, row = min(own, a.S - 1);
+    const bool over = sizeof(T) == 2 && row < a.S - 1 && D >= 8;
     const T *x = (const T *)a.x + row * a.ldx;
     const T *res = a.res ? (const T *)a.res + row * a.ldr : nullptr;
     T *sum = a.sum ? (T *)a.sum + row * a.lds : nullptr;
@@ -44,29 +51,34 @@ __global__ __launch_bounds__(256) void zz_add_norm_fp8_kernel(ZzF8RowsArgs a) {
     double ss = 0.0;
 #pragma unroll
     for (int i = 0; i < NU; i++) {
-        const int e = 8 * (i * 256 + tid);
-        zz_get8<VEC>(h[i], x + e, D - e);
+        const int e = 8 * (i * TPR + tid);
+        zz_get8(h[i], x + e, D - e, over);
         if (res) {
             float t[8];
-            zz_get8<VEC>(t, res + e, D - e);
+            zz_get8(t, res + e, D - e, over);
 #pragma unroll
             for (int j = 0; j < 8; j++) h[i][j] += t[j];
         }
 #pragma unroll
         for (int j = 0; j < 8; j++) ss = fma((double)h[i][j], (double)h[i][j], ss);
-        if (sum && e < D) zz_put8<VEC>(sum + e, h[i], D - e, a.nt);
+        if (sum && e < D && own < a.S) zz_put8<NT>(sum + e, h[i], D - e);
     }
     double t = zz_wave_sum(ss);
-    if ((tid & 63) == 0) red[tid >> 6] = t;
-    __syncthreads();
-    t = (red[0] + red[1]) + (red[2] + red[3]);
+    if constexpr (TPR > 64) {
+        constexpr int RW = TPR / 64;                      // a row's waves
+        const int wave = threadIdx.x >> 6, first = wave / RW * RW;
+        if ((tid & 63) == 0) red[wave] = t;
+        __syncthreads();
+        t = RW == 4 ? (red[0] + red[1]) + (red[2] + red[3]) : red[first] + red[first + 1];
+    }
+    if (own >= a.S) return;
     const float r = (float)(1.0 / sqrt(t / D + (double)a.eps));
 #pragma unroll
     for (int i = 0; i < NU; i++) {
-        const int e = 8 * (i * 256 + tid);
+        const int e = 8 * (i * TPR + tid);
         float w[8];
         if (a.w) {
-            zz_get8<VEC>(w, a.w + e, D - e);
+            zz_get8(w, a.w + e, D - e, false);
         } else {
 #pragma unroll
             for (int j = 0; j < 8; j++) w[j] = 1.0f;
@@ -83,14 +95,14 @@ __global__ __launch_bounds__(256) void zz_add_norm_fp8_kernel(ZzF8RowsArgs a) {
 }
 
 // Blocks of rows without a norm: 16 lanes per block, 16 blocks per workgroup.
-template <typename T, bool VEC>
+template <typename T>
 __global__ __launch_bounds__(256) void zz_rows_fp8_kernel(ZzF8RowsArgs a) {
     const int nb = zz_f8_nb(a.D), total = a.S * nb;
     const int id = blockIdx.x * 16 + (threadIdx.x >> 4), m = threadIdx.x & 15;
     const int at = id < total ? id : total - 1, row = at / nb, b = at - row * nb;
     const int e = b * ZZ_F8B + 8 * m;
     float v[8];
-    zz_get8<VEC>(v, (const T *)a.x + row * a.ldx + e, a.D - e);
+    zz_get8(v, (const T *)a.x + row * a.ldx + e, a.D - e, sizeof(T) == 2 && row < a.S - 1 && a.D >= 8);
     float sc;
     const uint2 c = zz_f8_block(v, &sc);
     if (id >= total) return;
@@ -98,29 +110,29 @@ __global__ __launch_bounds__(256) void zz_rows_fp8_kernel(ZzF8RowsArgs a) {
     if (m == 0) a.s[(size_t)b * a.S + row] = sc;
 }
 
-template <typename T, bool VEC>
+template <typename T, int TPR, int NU, bool NT>
 static void launch_norm(const ZzF8RowsArgs &a, hipStream_t st) {
-    const int u = (zz_f8_nb(a.D) * 16 + 255) / 256;
-    const dim3 g(a.S), b(256);
-    if (u <= 1) hipLaunchKernelGGL((zz_add_norm_fp8_kernel<T, 1, VEC>), g, b, 0, st, a);
-    else if (u <= 2) hipLaunchKernelGGL((zz_add_norm_fp8_kernel<T, 2, VEC>), g, b, 0, st, a);
-    else hipLaunchKernelGGL((zz_add_norm_fp8_kernel<T, 4, VEC>), g, b, 0, st, a);
+    hipLaunchKernelGGL((zz_add_norm_fp8_kernel<T, TPR, NU, NT>), dim3((a.S + 256 / TPR - 1) / (256 / TPR)), dim3(256), 0, st, a);
+}
+template <typename T, bool NT>
+static void launch_norm(const ZzF8RowsArgs &a, hipStream_t st) {
+    const int lanes = zz_f8_nb(a.D) * 16;
+    if (lanes <= 64) launch_norm<T, 64, 1, NT>(a, st);
+    else if (lanes <= 128) launch_norm<T, 128, 1, NT>(a, st);
+    else if (lanes <= 256) launch_norm<T, 256, 1, NT>(a, st);
+    else if (lanes <= 512) launch_norm<T, 256, 2, NT>(a, st);
+    else launch_norm<T, 256, 4, NT>(a, st);
 }
 
 int zz_launch_add_norm_fp8(int dtype, const ZzF8RowsArgs &a, hipStream_t st) {
-    if (dtype == 0) a.vec ? launch_norm<float, true>(a, st) : launch_norm<float, false>(a, st);
-    else a.vec ? launch_norm<zz_bf16, true>(a, st) : launch_norm<zz_bf16, false>(a, st);
+    if (dtype == 0) a.nt ? launch_norm<float, true>(a, st) : launch_norm<float, false>(a, st);
+    else a.nt ? launch_norm<zz_bf16, true>(a, st) : launch_norm<zz_bf16, false>(a, st);
     return hipGetLastError() == hipSuccess;
 }
 
 int zz_launch_rows_fp8(int dtype, const ZzF8RowsArgs &a, hipStream_t st) {
     const dim3 g((unsigned)(((int64_t)a.S * zz_f8_nb(a.D) + 15) / 16)), b(256);
-    if (dtype == 0) {
-        if (a.vec) hipLaunchKernelGGL((zz_rows_fp8_kernel<float, true>), g, b, 0, st, a);
-        else hipLaunchKernelGGL((zz_rows_fp8_kernel<float, false>), g, b, 0, st, a);
-    } else {
-        if (a.vec) hipLaunchKernelGGL((zz_rows_fp8_kernel<zz_bf16, true>), g, b, 0, st, a);
-        else hipLaunchKernelGGL((zz_rows_fp8_kernel<zz_bf16, false>), g, b, 0, st, a);
-    }
+    if (dtype == 0) hipLaunchKernelGGL((zz_rows_fp8_kernel<float>), g, b, 0, st, a);
+    else hipLaunchKernelGGL((zz_rows_fp8_kernel<zz_bf16>), g, b, 0, st, a);
     return hipGetLastError() == hipSuccess;
 }
