@@ -441,3 +441,23 @@ def test_rows_of_other_widths(dtype, D):
         zz.rows_fp8_dev(X.data_ptr(), S, D, q.data_ptr(), s.data_ptr(), KIND[dtype], ldx=2 * D, stream=stream())
         qh, sh = taken(q, s, S, D)
         R.check_rows(x[:, :D].double().numpy(), qh, sh, 0.0)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("S, O, I, ldy", [(4200, 4100, 140, 4160), (8300, 4104, 200, 4104)])
+def test_product_large_result(dtype, S, O, I, ldy):
+    """Results of 64 MiB and more, whose lines tiles write whole and those they do not."""
+    xq, xs, wq, ws = case(S, O, I, 9)
+    m = zz.Fp8Matrix(O, I)
+    try:
+        m.upload(wq, ws)
+        Q, Sc = torch.from_numpy(xq).cuda(), torch.from_numpy(xs).cuda()
+        y = torch.full((S, ldy), -3.0, dtype=dtype, device="cuda")
+        m.matmul_dev(Q.data_ptr(), Sc.data_ptr(), S, y.data_ptr(), KIND[dtype], ldy=ldy, stream=stream())
+        torch.cuda.synchronize()
+        assert bool((y[:, O:] == -3.0).all())
+        want, mag = R.product(xq, xs, wq, ws, O, I)
+        off = np.abs(y[:, :O].double().cpu().numpy() - want)
+        assert np.all(off <= R.product_bound(mag, want, I, dtype))
+    finally:
+        m.close()

@@ -58,7 +58,7 @@ __device__ __forceinline__ void zz_f8_store4(T *y, int64_t ldy, int t, int o, in
 }
 
 // 16 bytes of a result row, n of its elements inside the row
-template <typename T>
+template <bool NT, typename T>
 __device__ __forceinline__ void zz_f8_store(T *p, const float (&v)[16 / sizeof(T)], int n) {
     constexpr int E = 16 / sizeof(T);
     if (n >= E) {
@@ -67,7 +67,8 @@ __device__ __forceinline__ void zz_f8_store(T *p, const float (&v)[16 / sizeof(T
         for (int j = 0; j < 4; j++)
             if constexpr (E == 4) w[j] = __float_as_uint(v[j]);
             else w[j] = zz_bf16_bits(v[2 * j]) | zz_bf16_bits(v[2 * j + 1]) << 16;
-        *(zz_u4any *)p = w;
+        if constexpr (NT) __builtin_nontemporal_store(w, (zz_u4any *)p);
+        else *(zz_u4any *)p = w;
         return;
     }
 #pragma unroll
@@ -221,7 +222,7 @@ struct ZzF8Async {
 };
 
 // one tile: the result's rows from t0 and columns from 32 * gt
-template <typename T, int RO, int RS, int WO, int WS, int KS, int NS>
+template <typename T, int RO, int RS, int WO, int WS, int KS, int NS, bool NT>
 __device__ __forceinline__ void zz_fp8_tile(const ZzF8Mm &a, char *lds, int gt, int t0) {
     typedef ZzF8Async<RO, RS, WO, WS, KS, NS> C;
     const int tid = threadIdx.x, l = tid & 63, r = l & 31, h = l >> 5, nb = a.nb;
@@ -343,7 +344,7 @@ __device__ __forceinline__ void zz_fp8_tile(const ZzF8Mm &a, char *lds, int gt, 
         float v[E];
 #pragma unroll
         for (int e = 0; e < E; e += 4) *(float4 *)(v + e) = *(const float4 *)place(t, o + e);
-        zz_f8_store((T *)a.y + (int64_t)(t0 + t) * a.ldy + gt * 32 + o, v, a.m.O - gt * 32 - o);
+        zz_f8_store<NT>((T *)a.y + (int64_t)(t0 + t) * a.ldy + gt * 32 + o, v, a.m.O - gt * 32 - o);
     }
 }
 
@@ -364,12 +365,12 @@ __global__ __launch_bounds__(64 * WO * WS * KS, 2) void zz_fp8_async_kernel(ZzF8
     if (id >= OT * ST) return;
     int ot, st;
     zz_fp8_at(id, OT, ST, &ot, &st);
-    zz_fp8_tile<T, RO, RS, WO, WS, KS, NS>(a, lds, ot * C::O / 32, st * C::S);
+    zz_fp8_tile<T, RO, RS, WO, WS, KS, NS, false>(a, lds, ot * C::O / 32, st * C::S);
 }
 
 // Tiles of 64 RO x 64 RS; those from `whole` on in parts of 64 x 64, which run as a last round
 // of their own or beside a last round of whole tiles.
-template <typename T, int RO, int RS>
+template <typename T, int RO, int RS, bool NT>
 __global__ __launch_bounds__(256, 2) void zz_fp8_tiles_kernel(ZzF8Mm a, int whole) {
     extern __shared__ __attribute__((aligned(1024))) char lds[];
     const int OT = (a.m.O + 64 * RO - 1) / (64 * RO), ST = (a.S + 64 * RS - 1) / (64 * RS);
@@ -379,12 +380,12 @@ __global__ __launch_bounds__(256, 2) void zz_fp8_tiles_kernel(ZzF8Mm a, int whol
         const int id = x % 8 * g + x / 8;
         if (id >= whole) return;
         zz_fp8_at(id, OT, ST, &ot, &st);
-        zz_fp8_tile<T, RO, RS, 2, 2, 1, 2>(a, lds, ot * 2 * RO, st * 64 * RS);
+        zz_fp8_tile<T, RO, RS, 2, 2, 1, 2, NT>(a, lds, ot * 2 * RO, st * 64 * RS);
     } else {
         const int part = (x - 8 * g) % (RO * RS);
         zz_fp8_at(whole + (x - 8 * g) / (RO * RS), OT, ST, &ot, &st);
         const int gt = (ot * RO + part % RO) * 2, t0 = (st * RS + part / RO) * 64;
-        if (gt * 32 < a.m.O && t0 < a.S) zz_fp8_tile<T, 1, 1, 2, 2, 1, 3>(a, lds, gt, t0);
+        if (gt * 32 < a.m.O && t0 < a.S) zz_fp8_tile<T, 1, 1, 2, 2, 1, 3, NT>(a, lds, gt, t0);
     }
 }
 
@@ -434,8 +435,12 @@ static bool launch_tiles(const ZzF8Mm &a, bool split, hipStream_t st) {
     const int64_t n = (int64_t)((a.m.O + C::O - 1) / C::O) * ((a.S + C::S - 1) / C::S);
     const int64_t whole = split ? n - n % 256 : n, g = (whole + 7) / 8 * 8 + (n - whole) * RO * RS;
     if (g * C::NT > 0xffffffffll) return false;           // a launch's threads in one dimension
-    hipLaunchKernelGGL((zz_fp8_tiles_kernel<T, RO, RS>), dim3((unsigned)g), dim3(C::NT), (C::LDS > P::LDS ? C::LDS : P::LDS),
-                       st, a, (int)whole);
+    // large results past the caches (4096 x 8192 x 256 in f32 53 us and 38), where tiles write
+    // whole lines; else every line is written twice (8192 x 2892 x 256 in f32 33 us and 43)
+    const bool nt = a.S * a.ldy * (int64_t)sizeof(T) >= ZZ_NT_BYTES &&
+                    (uintptr_t)a.y % 64 == 0 && a.ldy * sizeof(T) % 64 == 0;
+    const auto k = nt ? zz_fp8_tiles_kernel<T, RO, RS, true> : zz_fp8_tiles_kernel<T, RO, RS, false>;
+    hipLaunchKernelGGL(k, dim3((unsigned)g), dim3(C::NT), (C::LDS > P::LDS ? C::LDS : P::LDS), st, a, (int)whole);
     return true;
 }
 
