@@ -29,7 +29,7 @@ __device__ __forceinline__ uint2 zz_f8_block(const float (&y)[8], float *scale) 
     return make_uint2((unsigned)c[0], (unsigned)c[1]);
 }
 
-// 8192 x 2816 in f32 take 58 us, 5.2 TB/s, which is what a large copy reaches (63 with the sum
+// 8192 x 2816 in f32 take 58.5 us, 5.1 TB/s, which is what a large copy reaches (63 with the sum
 // kept in the caches); one row 3.3 us, a launch's 2.2 and one trip to memory.
 // TPR threads per row, NU groups of 8 per thread held in registers between the sum of squares
 // and the codes: x and res are read once, sum and codes written once. As few threads as hold a
