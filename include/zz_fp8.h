@@ -36,7 +36,8 @@ int64_t zz_fp8_row_bytes(int64_t D);
 
 /* h = x + res (x where d_res is NULL), in f32; d_sum (NULL: not stored) receives h rounded
  * to dtype. y = h / sqrt(mean(h^2) + eps) * w, and each 128 of y as
- *   scale = max(max|y|, 2^-100) / 448,  code = e4m3(y / scale), round to nearest even.
+ *   scale = max(max|y|, 2^-100) / 448,  code = e4m3(y / scale), round to nearest even,
+ * both quotients those of f32, correctly rounded.
  * x, res and sum are of `dtype` with rows ldx, ldr, lds elements apart (0: D); w [D] is
  * f32 (NULL: ones). 1 <= D <= 8192, S <= 2^20. d_sum may be d_x or d_res itself, rows as
  * far apart; the outputs overlap nothing else (ranges are judged from their first byte to
@@ -48,8 +49,8 @@ int zz_add_norm_fp8_dev(int dtype, const void *d_x, int64_t ldx, const void *d_r
                         void *d_sum, int64_t lds, const float *d_w, float eps, int S, int D,
                         uint8_t *d_q, float *d_s, void *stream);
 
-/* The same rounding of x itself, without sum and norm; any D up to 2^20, S <= 2^20 (S * ceil(D/128)
- * <= 2^27). */
+/* The same rounding of x itself, without sum and norm: scales and codes are those of f32's
+ * quotients to the last bit. Any D up to 2^20, S <= 2^20 (S * ceil(D/128) <= 2^27). */
 int zz_rows_fp8_dev(int dtype, const void *d_x, int64_t ldx, int S, int D, uint8_t *d_q, float *d_s,
                     void *stream);
 

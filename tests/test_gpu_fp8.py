@@ -461,3 +461,35 @@ def test_product_large_result(dtype, S, O, I, ldy):
         assert np.all(off <= R.product_bound(mag, want, I, dtype))
     finally:
         m.close()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("kind", ["normal", "small integers", "halves of steps", "magnitudes"])
+def test_rows_exact(dtype, kind):
+    """Scales and codes to the last bit, at ties too: values of few bits lie right between two
+    codes often, and a quotient that is off by a bit takes the odd one."""
+    S, D = 301, 2100
+    g = torch.Generator().manual_seed(len(kind))
+    x = torch.randn(S, D, generator=g)
+    if kind == "small integers":
+        x = torch.randint(-57, 58, (S, D), generator=g).float()
+    elif kind == "halves of steps":                      # 448 the largest: all other values between two codes
+        x = torch.randint(16, 31, (S, D), generator=g).float() + 0.5
+        x = x * torch.exp2(torch.randint(-12, 4, (S, D), generator=g).float()) * (1 - 2 * torch.randint(0, 2, (S, D), generator=g))
+        x[:, ::128] = 448.0
+        x[:, -1] = -448.0
+        x = x * torch.exp2(torch.randint(-30, 31, (S, 1), generator=g).float())
+    elif kind == "magnitudes":                           # from below the floor to the largest, block by block
+        e = torch.linspace(-126, 124, S)[:, None].round()
+        x = x.clamp(-7.9, 7.9) * torch.exp2(e)
+    x = x.to(dtype)
+    x[7, 130:140] = -0.0
+    X = x.cuda()
+    q, s = buffers(S, D)
+    zz.rows_fp8_dev(X.data_ptr(), S, D, q.data_ptr(), s.data_ptr(), KIND[dtype], stream=stream())
+    qh, sh = taken(q, s, S, D)
+    want, scale = R.rows_exact(x.float().numpy())
+    assert np.array_equal(sh.numpy(), scale)
+    got = R.e4m3_value(qh.numpy())
+    assert np.array_equal(got, want), (np.count_nonzero(got != want), got.size)
+    assert np.array_equal(qh.numpy()[:, :D] >> 7, np.signbit(x.float().numpy()))

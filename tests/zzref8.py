@@ -64,6 +64,20 @@ def norm_delta(D):
     return 3 * U + D * 2.0 ** -52
 
 
+def rows_exact(x):
+    """(code values [S, whole blocks], scales [blocks, S]) of f32 rows, where nothing is open: the
+    scale is f32's a / 448, a code the e4m3 value nearest to f32's x / scale, ties to even."""
+    x = np.asarray(x, np.float32)
+    S, D = x.shape
+    p = np.zeros((S, blocks(D) * BLK), np.float32)
+    p[:, :D] = x
+    p = p.reshape(S, blocks(D), BLK)
+    s = np.maximum(np.abs(p).max(2), np.float32(FLOOR)) / np.float32(FMAX)
+    v = (p / s[:, :, None]).astype(np.float64)
+    step = 2 * e4m3_half_step(v)
+    return (np.round(v / step) * step).reshape(S, -1), s.T
+
+
 def product(xq, xs, wq, ws, O, I):
     """(y, sum of |terms|) in 64 bits: rows' codes [S, whole blocks] (uint8), scales
     [blocks, S], codes [O, I], scales [blocks of O, blocks of I]."""
