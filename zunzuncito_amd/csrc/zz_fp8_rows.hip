@@ -8,7 +8,7 @@
 // Both quotients are f32's, correctly rounded: values of few bits, as bf16 rows are, often lie
 // right between two codes, where the last bit of y / scale decides for a whole step (with
 // y * (448 / a) 3e-4 of such rows' codes are a neighbour of the right one; 1500 x 2112 bf16 took
-// 4.1 us with that and take 4.5). |y| <= a keeps y / scale under 448 * (1 + 2^-22), which rounds
+// 4.1 us with that and take 4.3). |y| <= a keeps y / scale under 448 * (1 + 2^-22), which rounds
 // to 448.
 //
 // A thread holds 8 consecutive elements: 16 lanes are one block, so its maximum is four DPP
@@ -21,7 +21,9 @@ __device__ __forceinline__ uint2 zz_f8_block(const float (&y)[8], float *scale) 
 #pragma unroll
     for (int j = 0; j < 8; j++) a = fmaxf(a, fabsf(y[j]));
     a = fmaxf(zz_group_max<16>(a), ZZ_F8FLOOR);
-    const float s = a / ZZ_F8MAX;
+    // a / 448, rounded right by one step: no quotient by 7 comes near the middle between two floats
+    constexpr float c448 = 1.0f / ZZ_F8MAX;
+    const float s0 = a * c448, s = a < INFINITY ? fmaf(-fmaf(s0, ZZ_F8MAX, -a), c448, s0) : a;
     *scale = s;
     // y / s by the block's one reciprocal: t is at most 1.5 ulp off, and what one step with its
     // remainder leaves, 2^-22 ulp, could only change a code where y / s lies that near to the
