@@ -42,8 +42,8 @@ int64_t zz_fp8_row_bytes(int64_t D);
  * f32 (NULL: ones). 1 <= D <= 8192, S <= 2^20. d_sum may be d_x or d_res itself, rows as
  * far apart; the outputs overlap nothing else (ranges are judged from their first byte to
  * their last, what lies between strided rows included). d_q is aligned to 16 bytes. The
- * squares and their mean are in double, so that no row of finite h leaves their range; a
- * row of zeros with eps 0 is 0 / 0. A NaN or infinity in a row makes codes of that row NaN
+ * squares, their mean and its root are in double, so that no row of finite h leaves their
+ * range; a row of zeros with eps 0 is 0 / 0. A NaN or infinity in a row makes codes of that row NaN
  * or its scales infinite and touches no other row. */
 int zz_add_norm_fp8_dev(int dtype, const void *d_x, int64_t ldx, const void *d_res, int64_t ldr,
                         void *d_sum, int64_t lds, const float *d_w, float eps, int S, int D,

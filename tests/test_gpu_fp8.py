@@ -493,3 +493,25 @@ def test_rows_exact(dtype, kind):
     got = R.e4m3_value(qh.numpy())
     assert np.array_equal(got, want), (np.count_nonzero(got != want), got.size)
     assert np.array_equal(qh.numpy()[:, :D] >> 7, np.signbit(x.float().numpy()))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("D", [3, 128, 1000, 2816, 8192])
+def test_add_norm_ends_of_range(dtype, D):
+    """Rows at both ends of the type, subnormal ones too, whose reciprocal root 32 bits do not
+    hold; without eps they are as good as any."""
+    S = 6
+    g = torch.Generator().manual_seed(D)
+    x = (0.5 + 0.5 * torch.rand(S, D, generator=g)) * (1 - 2 * torch.randint(0, 2, (S, D), generator=g))
+    x = (x.double() * torch.tensor([2.0 ** -129, 2.0 ** -132, 2.0 ** -140, 1.0, 2.0 ** 127, 1.99 * 2.0 ** 127])[:, None].double()).float()
+    x[2, 0] = 2.0 ** -133                                # bf16 holds no smaller one
+    x = x.to(dtype)
+    w = 1 + 0.3 * torch.randn(D, generator=g)
+    X, Wt = x.cuda(), w.cuda()
+    for wt, use in ((w, Wt.data_ptr()), (None, 0)):
+        q, s = buffers(S, D)
+        zz.add_norm_fp8_dev(X.data_ptr(), 0, 0, use, S, D, 0.0, q.data_ptr(), s.data_ptr(), KIND[dtype], stream=stream())
+        qh, sh = taken(q, s, S, D)
+        _, y = R.norm_rows(x, None, wt, 0.0)
+        assert np.isfinite(y).all() and np.abs(y).max() > 0.1
+        R.check_rows(y, qh, sh, R.norm_delta(D))

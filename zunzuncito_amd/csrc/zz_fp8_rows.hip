@@ -2,8 +2,10 @@
 // (include/zz_fp8.h), with the residual's addition and the RMS norm before it or without.
 //
 //   h = x + res;  r = 1 / sqrt(sum(h^2) / D + eps);  y = (h * r) * w
-// The squares, their sum and r before its rounding to f32 are in double: no row's leave its
-// range, and beside the row's bytes they cost nothing (58.4 us and 58.0 at 8192 x 2816).
+// The squares, their sum and r are in double: no row's leave its range, and beside the row's bytes
+// they cost nothing (58.4 us and 58.0 at 8192 x 2816). r is rounded to f32 for the product with h,
+// which is formed in double for the rows whose r has no place there (in double for all, with w
+// too, 8192 x 2816 in bf16 took 43 us for 41).
 //   per 128: a = max(max|y|, 2^-100), scale = a / 448, code = e4m3(y / scale)
 // Both quotients are f32's, correctly rounded: values of few bits, as bf16 rows are, often lie
 // right between two codes, where the last bit of y / scale decides for a whole step (with
@@ -99,7 +101,18 @@ __global__ __launch_bounds__(256) void zz_add_norm_fp8_kernel(ZzF8RowsArgs a) {
         t = RW == 4 ? (red[0] + red[1]) + (red[2] + red[3]) : red[first] + red[first + 1];
     }
     if (own >= a.S) return;
-    const float r = (float)(1.0 / sqrt(t / D + (double)a.eps));
+    const double rd = 1.0 / sqrt(t / D + (double)a.eps);
+    float r = (float)rd;
+    if (!(rd >= 0x1p-126 && rd <= 0x1p126)) {              // f32 does not hold it with all its bits
+#pragma unroll
+        for (int i = 0; i < NU; i++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                asm volatile("" : "+v"(h[i][j]));         // the squares' doubles are not kept for here
+                h[i][j] = (float)((double)h[i][j] * rd);
+            }
+        r = 1.0f;
+    }
 #pragma unroll
     for (int i = 0; i < NU; i++) {
         const int e = 8 * (i * TPR + tid);
