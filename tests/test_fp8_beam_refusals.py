@@ -129,3 +129,17 @@ def test_stack_beam_declines():
     L = zz.lib()
     assert L.zz_stack_beam_dev(-1, X, 4, 2, -1, R, Q, None) == 0
     assert "zz_stack_beam_dev" in zz.last_error()
+
+
+@pytest.mark.parametrize("bad, why", [
+    (dict(tok=None), "bad arguments"), (dict(seq=None), "bad arguments"), (dict(score=None), "bad arguments"),
+    (dict(W=0), "bad arguments"), (dict(W=17), "bad arguments"), (dict(n=-1), "bad arguments"),
+    (dict(n=(1 << 24) + 1), "bad arguments"), (dict(tok=X + 2), "misaligned"), (dict(seq=R + 1), "misaligned"),
+    (dict(score=Q + 2), "misaligned"), (dict(tok=R + 40), "overlaps"), (dict(score=R + 44), "overlaps"),
+    (dict(tok=Q + 12), "overlaps"),
+])
+def test_stack_beam_arguments(bad, why):
+    """The arguments are looked at before the stack, and before anything is written."""
+    a = {**dict(tok=X, W=4, n=2, eos=-1, seq=R, score=Q), **bad}
+    assert zz.lib().zz_stack_beam_dev(-1, a["tok"], a["W"], a["n"], a["eos"], a["seq"], a["score"], None) == 0
+    assert why in zz.last_error()

@@ -812,16 +812,19 @@ int zz_ranges_meet(const void *a, int64_t n, const void *b, int64_t m);
 
 extern "C" int zz_stack_beam_dev(int id, const int *d_tok, int W, int n, int eos, int *d_seq, float *d_score,
                                  void *stream) {
-    Stack *k = get_stack(id);
-    if (!k || !d_tok || !d_seq || !d_score || W < 1 || W > ZZ_BEAM_MAXW || n < 0 || n > 1 << 24)
+    if (!d_tok || !d_seq || !d_score || W < 1 || W > ZZ_BEAM_MAXW || n < 0 || n > 1 << 24)
         ZZ_FAIL("zz_stack_beam_dev: bad arguments (1 <= W <= %d, 0 <= n <= 2^24)", ZZ_BEAM_MAXW);
-    const int64_t wsb = zz_beam_ws_bytes(1, W, k->V);
-    if (wsb < 0) ZZ_FAIL("zz_stack_beam_dev: a vocabulary of %d is declined", k->V);
+    if ((uintptr_t)d_tok % 4 || (uintptr_t)d_seq % 4 || (uintptr_t)d_score % 4)
+        ZZ_FAIL("zz_stack_beam_dev: misaligned pointer");
     const int64_t ld = (int64_t)n + 1;
     if (zz_ranges_meet(d_seq, 4 * ld * W, d_tok, 4) || zz_ranges_meet(d_seq, 4 * ld * W, d_score, 4 * W) ||
         zz_ranges_meet(d_score, 4 * W, d_tok, 4))
         ZZ_FAIL("zz_stack_beam_dev: an output overlaps another argument");
     if (!zz_lib_here("zz_stack_beam_dev")) return 0;
+    Stack *k = get_stack(id);
+    if (!k) ZZ_FAIL("zz_stack_beam_dev: no such stack");
+    const int64_t wsb = zz_beam_ws_bytes(1, W, k->V);
+    if (wsb < 0) ZZ_FAIL("zz_stack_beam_dev: a vocabulary of %d is declined", k->V);
     hipStream_t st = stream ? (hipStream_t)stream : zz_lib_stream();
     // [rows W x D | logits W x V | tokens, parents, chosen, finished: 16 each | workspace]
     const size_t rows = sizeof(float) * (size_t)W * k->D, lg = sizeof(float) * (size_t)W * k->V;
