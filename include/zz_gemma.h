@@ -104,8 +104,9 @@ int zz_stack_decode_dev(int stack, int *d_tok, int n, float *d_logits, int use_g
  * receives the beams' tokens, d_tok[0] first, the best beam first; d_score [W] their
  * accumulated log-probabilities. A beam that took `eos` (no token is -1) is finished and
  * repeats it. Tokens never leave the device. A call that needs more room than any
- * before allocates the search's rows and waits for the device. The outputs overlap each other
- * and d_tok nowhere. */
+ * before allocates the search's rows and waits for the device; a graph captured from a call
+ * ends with the rows that it was given. The outputs are written at the end, once nothing can
+ * decline any more; they overlap each other and d_tok nowhere. */
 int zz_stack_beam_dev(int stack, const int *d_tok, int W, int n, int eos, int *d_seq, float *d_score,
                       void *stream);
 

@@ -425,3 +425,40 @@ def test_stack_search(W, eos, flash):
         stack.close()
         head.close()
         close_all(b, m, d)
+
+
+@pytest.mark.parametrize("gone", ["block", "head"])
+def test_stack_search_declined(gone):
+    """A search that is declined on its way, because a block or the head is no longer there,
+    leaves the outputs as they were; longer and wider searches follow shorter ones."""
+    L = Z.make_layer("gemma", seed=41, E=16, K=4, D=512, MI=256)
+    b, m, d = gpu_block(L, Z.make_dense(L.D, 512, 40))
+    V, D = 1024, L.D
+    head = zz.Head(tied_head(V, D, 4), V, D, np.ones(D, np.float32), 1e-6, float(np.sqrt(D)), 30.0)
+    stack = zz.Stack([b], head)
+    try:
+        start = torch.tensor([17], dtype=torch.int32, device="cuda")
+
+        def search(W, n):
+            seq = torch.full((W, n + 1), -5, dtype=torch.int32, device="cuda")
+            score = torch.full((W,), -5.0, device="cuda")
+            try:
+                stack.beam_dev(start.data_ptr(), W, n, seq.data_ptr(), score.data_ptr(), stream=stream())
+                torch.cuda.synchronize()
+                return seq.cpu(), score.cpu(), None
+            except RuntimeError as e:
+                torch.cuda.synchronize()
+                return seq.cpu(), score.cpu(), str(e)
+
+        short, long = search(3, 2), search(3, 300)
+        assert short[2] is None and long[2] is None and bool((long[0] >= 0).all())
+        again = search(3, 2)
+        assert torch.equal(again[0], short[0]) and torch.equal(again[1], short[1])
+        (b if gone == "block" else head).close()
+        seq, score, why = search(3, 2)
+        assert why and ("gone" if gone == "block" else "zz_head") in why
+        assert bool((seq == -5).all()) and bool((score == -5.0).all())
+    finally:
+        stack.close()
+        head.close()
+        close_all(b, m, d)

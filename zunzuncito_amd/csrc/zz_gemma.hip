@@ -807,6 +807,14 @@ __global__ __launch_bounds__(64) void zz_beam_append_kernel(const int *token, in
     cur[w] = token[w];
 }
 
+// the outcome to the caller's rows: `all` tokens, W scores
+__global__ __launch_bounds__(256) void zz_beam_end_kernel(const int *seq, const float *score, int W, int64_t all,
+                                                          int *d_seq, float *d_score) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i < all) d_seq[i] = seq[i];
+    if (i < W) d_score[i] = score[i];
+}
+
 int zz_lib_here(const char *who);                                             // zz_fp8.hip
 int zz_ranges_meet(const void *a, int64_t n, const void *b, int64_t m);
 
@@ -826,35 +834,46 @@ extern "C" int zz_stack_beam_dev(int id, const int *d_tok, int W, int n, int eos
     const int64_t wsb = zz_beam_ws_bytes(1, W, k->V);
     if (wsb < 0) ZZ_FAIL("zz_stack_beam_dev: a vocabulary of %d is declined", k->V);
     hipStream_t st = stream ? (hipStream_t)stream : zz_lib_stream();
-    // [rows W x D | logits W x V | tokens, parents, chosen, finished: 16 each | workspace]
+    // [rows W x D | logits W x V | tokens, parents, chosen, scores, finished: 16 each | workspace |
+    // the search's tokens W x (n + 1)]. The search runs in its own rows: what declines on the way
+    // leaves the caller's as they were.
     const size_t rows = sizeof(float) * (size_t)W * k->D, lg = sizeof(float) * (size_t)W * k->V;
-    const size_t need = rows + lg + 256 + (size_t)wsb;
+    const size_t need = rows + lg + 320 + (size_t)wsb + 4 * (size_t)(ld * W);
     if (need > k->beam_cap) {
         ZZ_CHECK(hipDeviceSynchronize());
         if (k->beam) (void)hipFree(k->beam);
         k->beam = nullptr;
         k->beam_cap = 0;
         zz_lib_mem_bump();
-        ZZ_CHECK(hipMalloc(&k->beam, need));
+        if (hipMalloc(&k->beam, need) != hipSuccess) {
+            k->beam = nullptr;
+            (void)hipGetLastError();
+            ZZ_FAIL("zz_stack_beam_dev: device allocation failed");
+        }
         k->beam_cap = need;
     }
     float *h = (float *)k->beam, *logits = (float *)(k->beam + rows);
     int *cur = (int *)(k->beam + rows + lg), *parent = cur + 16, *token = parent + 16;
-    uint8_t *done = (uint8_t *)(token + 16);
+    float *score = (float *)(token + 16);
+    uint8_t *done = (uint8_t *)(score + 16);
     char *ws = (char *)(done + 64);
-    hipLaunchKernelGGL(zz_beam_begin_kernel, dim3(1), dim3(64), 0, st, d_tok, W, ld, d_seq, cur, d_score, done, eos);
+    int *seq = (int *)(ws + wsb);
+    hipLaunchKernelGGL(zz_beam_begin_kernel, dim3(1), dim3(64), 0, st, d_tok, W, ld, seq, cur, score, done, eos);
     for (int i = 0; i < n; i++) {
         if (!zz_head_embed_dev(k->head, cur, W, h, st) || !stack_blocks(k, h, W, st)) return 0;
         for (int w = 0; w < W; w += ZZ_DEC_MAXS) {
             const int m = W - w < ZZ_DEC_MAXS ? W - w : ZZ_DEC_MAXS;
             if (!zz_head_logits_dev(k->head, h + (size_t)w * k->D, m, logits + (size_t)w * k->V, nullptr, st)) return 0;
         }
-        if (!zz_beam_step_dev(ZZ_F32, logits, 0, 1, W, k->V, d_score, done, eos, eos >= 0 ? eos : 0, d_score, parent,
+        if (!zz_beam_step_dev(ZZ_F32, logits, 0, 1, W, k->V, score, done, eos, eos >= 0 ? eos : 0, score, parent,
                               token, done, ws, (size_t)wsb, st))
             return 0;
-        if (!zz_beam_reorder_dev(d_seq, d_seq, parent, 1, W, 1, 0, 4 * ld, 4 * ((int64_t)i + 1), st)) return 0;
-        hipLaunchKernelGGL(zz_beam_append_kernel, dim3(1), dim3(64), 0, st, token, W, ld, i + 1, d_seq, cur);
+        if (!zz_beam_reorder_dev(seq, seq, parent, 1, W, 1, 0, 4 * ld, 4 * ((int64_t)i + 1), st)) return 0;
+        hipLaunchKernelGGL(zz_beam_append_kernel, dim3(1), dim3(64), 0, st, token, W, ld, i + 1, seq, cur);
     }
+    if (hipGetLastError() != hipSuccess) ZZ_FAIL("zz_stack_beam_dev: launch failed");
+    hipLaunchKernelGGL(zz_beam_end_kernel, dim3((unsigned)((ld * W + 255) / 256)), dim3(256), 0, st, seq, score, W, ld * W,
+                       d_seq, d_score);
     if (hipGetLastError() != hipSuccess) ZZ_FAIL("zz_stack_beam_dev: launch failed");
     return 1;
 }
