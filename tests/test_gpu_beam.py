@@ -462,3 +462,21 @@ def test_stack_search_declined(gone):
         stack.close()
         head.close()
         close_all(b, m, d)
+
+
+@pytest.mark.parametrize("N, W, row", [(5, 3, 1 << 23), (2, 4, 9000001), (3, 8, 1 << 22), (1, 16, 5000013)])
+def test_reorder_past_the_caches(N, W, row):
+    """States of 64 MiB and more, for each number of rows that a thread holds, in place and not,
+    with bytes behind the last whole piece and with none."""
+    g = torch.Generator(device="cuda").manual_seed(W)
+    src = torch.randint(0, 255, (N, W, row), generator=g, dtype=torch.uint8, device="cuda")
+    par = torch.randint(0, W, (N, W), generator=g, dtype=torch.int32, device="cuda")
+    used = row - 1 if row % 2 else row
+    assert N * W * used >= 64 << 20
+    want = torch.stack([src[n, par[n].long(), :used] for n in range(N)])
+    dst = torch.full_like(src, 3)
+    for to in (dst, src):
+        last = to[:, :, used:].clone()
+        zz.beam_reorder_dev(to.data_ptr(), src.data_ptr(), par.data_ptr(), N, W, row_stride=row, row_bytes=used, stream=stream())
+        torch.cuda.synchronize()
+        assert torch.equal(to[:, :, :used], want) and torch.equal(to[:, :, used:], last)

@@ -515,3 +515,82 @@ def test_add_norm_ends_of_range(dtype, D):
         _, y = R.norm_rows(x, None, wt, 0.0)
         assert np.isfinite(y).all() and np.abs(y).max() > 0.1
         R.check_rows(y, qh, sh, R.norm_delta(D))
+
+
+def product_on(xq, xs, wq, ws, O, I, dtype):
+    """R.product and R.product_bound of a large result, in 64 bits on the device."""
+    x = torch.from_numpy(R.e4m3_value(xq)[:, :I] * np.repeat(xs.astype(np.float64).T, 128, 1)[:, :I]).cuda()
+    w = R.e4m3_value(wq) * np.repeat(np.repeat(ws.astype(np.float64), 128, 0)[:O], 128, 1)[:, :I]
+    w = torch.from_numpy(np.ascontiguousarray(w.T)).cuda()
+    want, mag = x @ w, x.abs() @ w.abs()
+    return want, R.product_bound(mag, 0.0, I, dtype) + R.HALF[dtype] * want.abs()
+
+
+# results of 64 MiB and more whose lines tiles write whole, which are stored past the caches: for
+# each type 64 x 128 and 128 x 128 tiles, and both with what is over a round in parts; no size a
+# tile divides
+@pytest.mark.parametrize("dtype, S, O, I, ldy", [
+    (F32, 8331, 2002, 129, 2016), (F32, 8903, 2066, 129, 2080), (F32, 2584, 7445, 515, 7456), (F32, 2949, 6845, 777, 6848),
+    (BF16, 4870, 6927, 129, 6944), (BF16, 7299, 4577, 129, 4608), (BF16, 6190, 6472, 513, 6496),
+    (BF16, 7041, 5281, 643, 5312)])
+def test_product_past_the_caches(dtype, S, O, I, ldy):
+    print("case", S, O, I, ldy, dtype, flush=True)
+    xq, xs, wq, ws = case(S, O, I, S)
+    m = zz.Fp8Matrix(O, I)
+    try:
+        m.upload(wq, ws)
+        Q, Sc = torch.from_numpy(xq).cuda(), torch.from_numpy(xs).cuda()
+        y = torch.full((S + 1, ldy), -3.0, dtype=dtype, device="cuda")
+        assert y.data_ptr() % 64 == 0 and ldy * y.element_size() % 64 == 0 and S * ldy * y.element_size() >= 64 << 20
+        m.matmul_dev(Q.data_ptr(), Sc.data_ptr(), S, y.data_ptr(), KIND[dtype], ldy=ldy, stream=stream())
+        torch.cuda.synchronize()
+        assert bool((y[:, O:] == -3.0).all()) and bool((y[S] == -3.0).all())
+        want, lim = product_on(xq, xs, wq, ws, O, I, dtype)
+        assert bool(((y[:S, :O].double() - want).abs_() <= lim).all())
+    finally:
+        m.close()
+
+
+@pytest.mark.parametrize("S, O, I, dtype", [(1, 65600, 1088, BF16), (8, 65600, 1088, BF16), (9, 65600, 1088, BF16),
+                                            (32, 65600, 1088, BF16), (5, 65600, 1200, F32), (32, 18432, 7168, BF16)])
+def test_product_large_matrices(S, O, I, dtype):
+    """Matrices past the caches, all of the result: in 16 bits, in both forms that are stored
+    past them, at both ends of their rows; with more columns, where another form is chosen."""
+    r = np.random.default_rng(S)
+    xq, xs, _, _ = case(S, 1, I, S)
+    wq = coded((O, I), S)
+    ws = np.exp(r.normal(-8, 1, (R.blocks(O), R.blocks(I)))).astype(np.float32)
+    m = zz.Fp8Matrix(O, I)
+    try:
+        m.upload(wq, ws)
+        Q, Sc = torch.from_numpy(xq).cuda(), torch.from_numpy(xs).cuda()
+        y = torch.full((S + 1, O), -3.0, dtype=dtype, device="cuda")
+        m.matmul_dev(Q.data_ptr(), Sc.data_ptr(), S, y.data_ptr(), KIND[dtype], stream=stream())
+        torch.cuda.synchronize()
+        assert bool((y[S] == -3.0).all())
+        want, lim = product_on(xq, xs, wq, ws, O, I, dtype)
+        assert bool(((y[:S].double() - want).abs_() <= lim).all())
+    finally:
+        m.close()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("D", [500, 1000, 2000, 2816, 5035])
+def test_add_norm_past_the_caches(dtype, D):
+    """A sum of 64 MiB and a few rows, with each number of threads and groups a row: all of the
+    sum, and some rows' codes."""
+    S = (64 << 20) // (D * (4 if dtype == F32 else 2)) + 3
+    g = torch.Generator(device="cuda").manual_seed(D)
+    x = torch.randn(S, D, generator=g, device="cuda").to(dtype)
+    res = torch.randn(S, D, generator=g, device="cuda").to(dtype)
+    w = 1 + 0.3 * torch.randn(D, generator=g, device="cuda")
+    q, s = buffers(S, D)
+    sm = torch.full((S + 1, D), -5.0, dtype=dtype, device="cuda")
+    zz.add_norm_fp8_dev(x.data_ptr(), res.data_ptr(), sm.data_ptr(), w.data_ptr(), S, D, 1e-6, q.data_ptr(), s.data_ptr(),
+                        KIND[dtype], stream=stream())
+    torch.cuda.synchronize()
+    assert torch.equal(sm[:S], (x.float() + res.float()).to(dtype)) and bool((sm[S] == -5.0).all())
+    qh, sh = taken(q, s, S, D)
+    at = [*range(9), S // 3, S // 2, *range(S - 9, S)]
+    _, y = R.norm_rows(x[at].cpu(), res[at].cpu(), w.cpu(), float(np.float32(1e-6)))
+    R.check_rows(y, qh[at], sh[:, at], R.norm_delta(D))
