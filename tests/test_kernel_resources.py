@@ -41,3 +41,12 @@ def test_matmul_sums_in_registers(kernels):
     mm = {k: v for k, v in kernels.items() if k.startswith("zz_matmul_f32_kernel<")}
     assert len(mm) == 32
     assert not [(k, v) for k, v in mm.items() if v[0] or v[1] > 512]
+
+
+def test_rows_product_beam_in_registers(kernels):
+    """No scratch in the kernels of the 8-bit rows, their product and beam search: the reordering
+    lost half its speed to it once."""
+    mine = {k: v for k, v in kernels.items() if k.startswith(("zz_add_norm_fp8", "zz_rows_fp8", "zz_fp8_", "zz_beam_"))}
+    assert len([k for k in mine if k.startswith("zz_add_norm_fp8_kernel<")]) == 20
+    assert len([k for k in mine if k.startswith("zz_beam_reorder_kernel<")]) == 6
+    assert not [(k, v) for k, v in mine.items() if v[0]]
