@@ -3,11 +3,12 @@
 //   total(w, t) = score[w] + ((L[w][t] - m[w]) - log(sum_t exp(L[w][t] - m[w]))), m the maximum
 // Within a row totals go by the logit, so a row's W best are found on the logits alone, as
 // 64-bit keys (order-preserving bits of the logit, then the lower token), and the sum of
-// exponentials belongs to the same pass over the data. Two launches:
+// exponentials belongs to the same pass over the data; within a chunk it is summed in f32 (up to
+// 32 terms a thread, then the wave's and the workgroup's), from there on in double. Two launches:
 //   zz_beam_part_kernel   a workgroup per (row, chunk of the vocabulary): the chunk's W
 //                         largest keys in order, its maximum and sum of exponentials
 //   zz_beam_merge_kernel  a workgroup per sequence: a wave per beam joins the chunks' lists
-//                         and sums (in double), then one wave picks the W best totals
+//                         and sums (in double), and finds its totals' places among all
 // or, for a small vocabulary, one: zz_beam_small_kernel, whose waves make their beams' lists
 // themselves. A step of 16 sequences of 8 beams over 262144 f32 logits takes 32 us, 134 MB at
 // 4.2 TB/s, 26 us of it in the first launch at 5.2 TB/s; in bf16 29 us. There it is the chain of
