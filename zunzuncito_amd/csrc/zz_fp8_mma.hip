@@ -7,7 +7,9 @@
 // to the largest and keep 13 bits behind it (2^-14 beside 1 is lost within 16 neighbours and
 // kept between them, measured), 1.5e-5 off in the 2-norm over normally distributed codes and
 // 1e-4 of the terms' magnitude at worst, where the f16 form is 1e-8 and 2e-7 off. They would
-// run at twice the rate.
+// run at twice the rate (8192^3 in a library 2.7 PFLOP/s, in f16 1.35). Results in bf16, whose own
+// rounding is a hundred times as large, would bear them, but take the same form. bf16 holds
+// every code too, and its library product is faster (1.48): not tried.
 //
 // A block of 128 columns is eight v_mfma_f32_32x32x16_f16 of 32 matrix rows times 32
 // activation rows; each of the 16 results a lane then enters the f32 accumulator by one fma
@@ -461,6 +463,11 @@ static bool launch_few(const ZzF8Mm &a, hipStream_t st) {
 // the best form of each, and up to 17 %. Any one form for all loses far more: the first and the
 // last but one take 4.8 and 25.6 us for 1 x 4224 x 2816, 295 and 109 for 4096 rows; without the
 // parts 4096 x 4224 x 2816 takes 107 us where it takes 95, 1000 x 4224 x 2816 36 for 30.
+// The model has no bandwidth in it and holds for what it was fitted to. For few rows of matrices
+// past the caches its times lie below what their bytes take (262144 x 4096: 131 us, where a read at
+// 7.1 TB/s takes 151), and from about 3700 columns on it prefers the third form, whose loads go
+// through the caches: 1 row of 262144 x 4096 180 us (6.0 TB/s), of 128256 x 7168 152 (6.1), of 18432
+// x 7168 30 (4.4), where the second form's past the caches reaches 6.9 at 262144 x 2816.
 struct ZzF8Form { int o, s, ks, per; float fix[4], slope[4]; int parts; float busy[3]; };
 static const ZzF8Form mm_forms[] = {
     {32, 32, 16, 1, {1.9f}, {2.0f}},
