@@ -26,7 +26,7 @@ TYPES = {"f32": torch.float32, "bf16": torch.bfloat16}
 
 def listed():
     return [
-        # one token on its way to 8 experts: two launches' latency
+        # one token on its way to 8 experts: a call's latency
         dict(name="dispatch_decode_1", kind="dispatch", tokens=1, top=8, experts=128, width=2816, dtype="f32", drop=0),
         # a serving batch with every fifth choice dropped (an expert at its capacity)
         dict(name="dispatch_batch_37", kind="dispatch", tokens=37, top=4, experts=32, width=2048, dtype="bf16", drop=5),
@@ -337,9 +337,9 @@ def _own(st):
         return dict(y=st.y)
     S, K, D = c["tokens"], c["top"], c["width"]
     if c["kind"] == "dispatch":
-        zz.experts_sort_dev(st.ids.data_ptr(), S, K, c["experts"], st.offs.data_ptr(), st.row.data_ptr(),
-                            st.pos.data_ptr(), st.ws.data_ptr(), st.ws.numel(), stream=stream)
-        zz.experts_gather_dev(st.x.data_ptr(), st.pos.data_ptr(), S, K, D, st.xs.data_ptr(), dtype=t, stream=stream)
+        zz.experts_dispatch_dev(st.ids.data_ptr(), S, K, c["experts"], st.offs.data_ptr(), st.row.data_ptr(),
+                                st.pos.data_ptr(), st.ws.data_ptr(), st.ws.numel(), d_x=st.x.data_ptr(), D=D,
+                                d_xs=st.xs.data_ptr(), dtype=t, stream=stream)
         return dict(offs=st.offs, row=st.row, pos=st.pos, xs=st.xs)
     if c["kind"] == "back":
         zz.experts_back_dev(st.y.data_ptr(), st.pos.data_ptr(), st.w.data_ptr(), S, K, D, st.out.data_ptr(),
