@@ -27,6 +27,11 @@
 #define ZZ_F32  0
 #define ZZ_BF16 1
 
+/* activations of a product's epilogue */
+#define ZZ_EP_NONE      0
+#define ZZ_EP_GELU_TANH 1   /* v / (1 + exp(-sqrt(8/pi) (v + 0.044715 v^3))), gelu in its tanh form */
+#define ZZ_EP_SILU      2   /* v / (1 + exp(-v)) */
+
 #ifdef __cplusplus
 extern "C" {
 #endif
@@ -77,6 +82,40 @@ int zz_fp8_matmul_dev(int mat, const uint8_t *d_q, const float *d_s, int S, int 
 /* Host form, synchronous: x [S, I] f32 is rounded as zz_rows_fp8_dev does and multiplied;
  * y [S, O] f32. */
 int zz_fp8_matmul(int mat, const float *x, float *y, int S);
+
+/* A resident table of E experts' matrices [O, I] (E = 1: one matrix), or with `gated` of E pairs
+ * of them, gate and up; returns its id, or -1. zz_fp8_destroy gives it back. 1 <= E <= 512, O
+ * and I as zz_fp8_create's, all codes together less than 2^38 bytes. An upload fills one matrix,
+ * part 0 the only or the gate's, part 1 the up's, codes and scales as zz_fp8_upload's, and under
+ * its conditions; a table whose uploads are not complete has no product. */
+int zz_fp8_create_experts(int E, int O, int I, int gated);
+int zz_fp8_upload_expert(int mat, int e, int part, const uint8_t *codes, const float *scales);
+int zz_fp8_upload_expert_dev(int mat, int e, int part, const uint8_t *d_codes, const float *d_scales);
+
+/* The product of one matrix (zz_fp8_create's, or a table's with E = 1) with an epilogue: v the
+ * sums of zz_fp8_matmul_dev (not rounded) plus bias, then
+ *   y = act(v) + res                                        a plain matrix
+ *   y = act(min(v_gate, clamp)) * clip(v_up, -clamp, clamp) + res       a gated pair
+ * in f32, rounded once to `dtype`. bias f32 [O], a gated pair's [2][O], gate's first (NULL:
+ * none); act ZZ_EP_*; clamp > 0, or 0 for none (a plain matrix takes none); res [S, O] of `dtype`,
+ * rows ldr apart (0: O; NULL: none), may be y itself, rows as far apart. The activations are of
+ * one hardware exponential and one reciprocal: off by up to (6 + 10 |a|) 2^-24 of the value, a
+ * the exponent, beside what v is off. A NaN stays one; act(-infinity) is NaN, infinity times
+ * 0. Other limits and promises as zz_fp8_matmul_dev's, S <= 2^20. y overlaps no other argument. */
+int zz_fp8_matmul_ep_dev(int mat, const uint8_t *d_q, const float *d_s, int S, const float *d_bias, int act,
+                         float clamp, const void *d_res, int64_t ldr, int dtype, void *d_y, int64_t ldy,
+                         void *stream);
+
+/* The same over a table of experts: rows offs[e] .. offs[e + 1] - 1 of y [P, O] are expert e's
+ * products, of the rows row[p] of the R rows in d_q, d_s (row NULL: of row p itself, R >= P).
+ * offs [E + 1] and row [P] are device memory (zz_experts_dispatch_dev makes them): offs ascends from
+ * 0 or more to P or less, rows of y outside it are left as they were; with an index outside 0 ..
+ * R-1 row 0 is taken. bias [E][O], gated [E][2][O]; res [P, O]. P, R <= 2^24; with d_row, R *
+ * zz_fp8_row_bytes(I) < 2^32. The form is chosen by P and E: rows' results do not depend on how
+ * many rows other experts have. */
+int zz_fp8_matmul_experts_dev(int mat, const uint8_t *d_q, const float *d_s, int R, const int *d_row,
+                              const int *d_offs, int P, const float *d_bias, int act, float clamp,
+                              const void *d_res, int64_t ldr, int dtype, void *d_y, int64_t ldy, void *stream);
 
 #ifdef __cplusplus
 }

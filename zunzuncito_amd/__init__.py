@@ -3,9 +3,10 @@
 The product is libzzmoe.so (HIP, gfx950), whose C ABI is include/zz_gpu.h (the
 engines' gpu.h, same symbols), include/zz_moe.h (the whole MoE block with
 experts resident in HBM), include/zz_gemma.h (gemma's feed-forward block and
-tied embedding / lm_head around it), include/zz_fp8.h (8-bit floating-point rows
-and matrices) and include/zz_beam.h (beam search's step). This module is a thin ctypes binding of that ABI for
-Python callers, tests and the benchmark. There is no CPU fallback here: when the
+tied embedding / lm_head around it), include/zz_fp8.h (8-bit floating-point rows,
+matrices and tables of experts), include/zz_experts.h (tokens to experts and back)
+and include/zz_beam.h (beam search's step). This module is a thin ctypes binding of
+that ABI for Python callers, tests and the benchmark. There is no CPU fallback here: when the
 library is missing or no gfx950 device is present, calls raise.
 """
 import ctypes as C
@@ -20,7 +21,9 @@ GPU_FMT_Q40, GPU_FMT_Q80, GPU_FMT_TQ2, GPU_FMT_Q4A = 1, 2, 3, 4
 ZZ_GATE_SOFTMAX_PES, ZZ_GATE_SIGMOID_BIAS, ZZ_GATE_SOFTMAX_TOPK, ZZ_GATE_DENSE = 0, 1, 2, 3
 ZZ_GATE_GROUPED = 4
 ZZ_F32, ZZ_BF16 = 0, 1
+ZZ_EP_NONE, ZZ_EP_GELU_TANH, ZZ_EP_SILU = 0, 1, 2
 ZZ_BEAM_MAXW, ZZ_BEAM_MAXV = 16, 524288
+ZZ_EXPERTS_MAXE, ZZ_EXPERTS_MAXK = 512, 16
 ZZ_ACT_GEGLU_TANH, ZZ_ACT_SWIGLU, ZZ_ACT_SWIGLU_CLAMP = 0, 1, 2
 
 # Every symbol the headers in include/ declare.
@@ -40,7 +43,9 @@ ABI_SYMBOLS = (
     "zz_stack_use_flash", "zz_moe_forward_dev_noalloc", "zz_router_expf", "zz_gpu_map_refreshes", "zz_moe_dots",
     "zz_fp8_row_bytes", "zz_add_norm_fp8_dev", "zz_rows_fp8_dev", "zz_fp8_create", "zz_fp8_destroy",
     "zz_fp8_upload", "zz_fp8_upload_dev", "zz_fp8_matmul_dev", "zz_fp8_matmul",
-    "zz_beam_ws_bytes", "zz_beam_step_dev", "zz_beam_reorder_dev", "zz_stack_beam_dev",
+    "zz_fp8_create_experts", "zz_fp8_upload_expert", "zz_fp8_upload_expert_dev", "zz_fp8_matmul_ep_dev",
+    "zz_fp8_matmul_experts_dev", "zz_experts_ws_bytes", "zz_experts_dispatch_dev", "zz_experts_back_dev",
+    "zz_experts_back_grad_dev", "zz_beam_ws_bytes", "zz_beam_step_dev", "zz_beam_reorder_dev", "zz_stack_beam_dev",
 )
 KERNELS = ("prep", "logits", "topk", "dispatch", "ffn_up", "ffn_down", "combine", "dec_route",
            "dec_down")
@@ -152,6 +157,17 @@ def lib():
     L.zz_fp8_upload_dev.argtypes = [i, p, p]
     L.zz_fp8_matmul_dev.argtypes = [i, p, p, i, i, p, l, p]
     L.zz_fp8_matmul.argtypes = [i, _f32p, _f32p, i]
+    f, n = C.c_float, C.c_size_t
+    L.zz_fp8_create_experts.argtypes = [i, i, i, i]
+    L.zz_fp8_upload_expert.argtypes = [i, i, i, _u8p, _f32p]
+    L.zz_fp8_upload_expert_dev.argtypes = [i, i, i, p, p]
+    L.zz_fp8_matmul_ep_dev.argtypes = [i, p, p, i, p, i, f, p, l, i, p, l, p]
+    L.zz_fp8_matmul_experts_dev.argtypes = [i, p, p, i, p, p, i, p, i, f, p, l, i, p, l, p]
+    L.zz_experts_ws_bytes.restype = l
+    L.zz_experts_ws_bytes.argtypes = [i, i, i]
+    L.zz_experts_dispatch_dev.argtypes = [p, i, i, i, p, p, p, i, p, l, i, p, l, p, n, p]
+    L.zz_experts_back_dev.argtypes = [i, p, l, p, p, i, i, i, p, l, p, l, p]
+    L.zz_experts_back_grad_dev.argtypes = [i, p, l, p, l, p, p, i, i, i, p, l, p, p]
     L.zz_beam_ws_bytes.restype = l
     L.zz_beam_ws_bytes.argtypes = [i, i, i]
     L.zz_beam_step_dev.argtypes = [i, p, l, i, i, i, p, p, i, i, p, p, p, p, p, C.c_size_t, p]
@@ -536,6 +552,13 @@ class Fp8Matrix:
         if not lib().zz_fp8_matmul_dev(self.id, d_q or None, d_s or None, S, dtype, d_y or None, ldy, stream or None):
             raise RuntimeError(f"zz_fp8_matmul_dev declined: {last_error()}")
 
+    def matmul_ep_dev(self, d_q, d_s, S, d_y, d_bias=0, act=ZZ_EP_NONE, clamp=0.0, d_res=0, dtype=ZZ_F32, ldr=0, ldy=0,
+                      stream=0):
+        """act(product + bias) + res, for a gated pair act(gate) * up + res (zz_fp8_matmul_ep_dev)."""
+        if not lib().zz_fp8_matmul_ep_dev(self.id, d_q or None, d_s or None, S, d_bias or None, act, clamp, d_res or None,
+                                          ldr, dtype, d_y or None, ldy, stream or None):
+            raise RuntimeError(f"zz_fp8_matmul_ep_dev declined: {last_error()}")
+
     def matmul(self, x):
         """Host x [S, I] f32, rounded to e4m3 rows, times the matrix; y [S, O]."""
         x = np.ascontiguousarray(x, np.float32)
@@ -550,6 +573,75 @@ class Fp8Matrix:
         if self.id >= 0:
             lib().zz_fp8_destroy(self.id)
             self.id = -1
+
+
+class Fp8Experts:
+    """A resident table of E e4m3 matrices [O, I], or of E gated pairs (zz_fp8_create_experts)."""
+
+    def __init__(self, E, O, I, gated=False):
+        self.E, self.O, self.I, self.parts = E, O, I, 2 if gated else 1
+        self.id = lib().zz_fp8_create_experts(E, O, I, 1 if gated else 0)
+        if self.id < 0:
+            raise RuntimeError(f"zz_fp8_create_experts declined: {last_error()}")
+
+    def upload(self, e, codes, scales, part=0):
+        """Host codes uint8 [O, I] and scales f32 [ceil(O/128), ceil(I/128)] of expert e; part 1:
+        the up matrix of a gated pair."""
+        codes = np.ascontiguousarray(codes, np.uint8)
+        scales = np.ascontiguousarray(scales, np.float32)
+        if codes.shape != (self.O, self.I) or scales.shape != (-(-self.O // 128), -(-self.I // 128)):
+            raise ValueError("codes [O, I] and scales [ceil(O/128), ceil(I/128)]")
+        if not lib().zz_fp8_upload_expert(self.id, e, part, _p(codes, _u8p), _p(scales, _f32p)):
+            raise RuntimeError(f"zz_fp8_upload_expert declined: {last_error()}")
+
+    def upload_dev(self, e, d_codes, d_scales, part=0):
+        if not lib().zz_fp8_upload_expert_dev(self.id, e, part, d_codes or None, d_scales or None):
+            raise RuntimeError(f"zz_fp8_upload_expert_dev declined: {last_error()}")
+
+    matmul_ep_dev = Fp8Matrix.matmul_ep_dev          # a table of one
+
+    def matmul_dev(self, d_q, d_s, R, d_row, d_offs, P, d_y, d_bias=0, act=ZZ_EP_NONE, clamp=0.0, d_res=0, dtype=ZZ_F32,
+                   ldr=0, ldy=0, stream=0):
+        """Each expert's rows times its matrix, with the epilogue of matmul_ep_dev
+        (zz_fp8_matmul_experts_dev): rows offs[e] .. offs[e+1]-1 of y [P, O] from the rows d_row
+        names (0: the rows themselves)."""
+        if not lib().zz_fp8_matmul_experts_dev(self.id, d_q or None, d_s or None, R, d_row or None, d_offs or None, P,
+                                               d_bias or None, act, clamp, d_res or None, ldr, dtype, d_y or None, ldy,
+                                               stream or None):
+            raise RuntimeError(f"zz_fp8_matmul_experts_dev declined: {last_error()}")
+
+    close = Fp8Matrix.close
+
+
+def experts_ws_bytes(S, K, E):
+    """Workspace bytes of one experts_dispatch_dev of these sizes."""
+    n = lib().zz_experts_ws_bytes(S, K, E)
+    if n < 0:
+        raise RuntimeError("zz_experts_ws_bytes declined: 1 <= S <= 2^20, 1 <= K <= 16, 1 <= E <= 512")
+    return n
+
+
+def experts_dispatch_dev(d_eidx, S, K, E, d_offs, d_row, d_pos, d_ws, ws_bytes, d_x=0, D=0, d_xs=0, dtype=ZZ_F32, ldx=0,
+                         ldxs=0, stream=0):
+    """The pairs of eidx [S, K] in the experts' order (zz_experts_dispatch_dev): offs [E + 1], row
+    [S * K], pos [S, K] int32; and with d_x the tokens' rows there, xs [S * K, D]."""
+    if not lib().zz_experts_dispatch_dev(d_eidx or None, S, K, E, d_offs or None, d_row or None, d_pos or None, dtype,
+                                         d_x or None, ldx, D, d_xs or None, ldxs, d_ws or None, ws_bytes, stream or None):
+        raise RuntimeError(f"zz_experts_dispatch_dev declined: {last_error()}")
+
+
+def experts_back_dev(d_y, d_pos, d_w, S, K, D, d_out, d_res=0, dtype=ZZ_F32, ldy=0, ldr=0, ldo=0, stream=0):
+    """out[s] = res[s] + sum_j w[s, j] y[pos[s, j]] (zz_experts_back_dev); d_w 0: ones."""
+    if not lib().zz_experts_back_dev(dtype, d_y or None, ldy, d_pos or None, d_w or None, S, K, D, d_res or None, ldr,
+                                     d_out or None, ldo, stream or None):
+        raise RuntimeError(f"zz_experts_back_dev declined: {last_error()}")
+
+
+def experts_back_grad_dev(d_dout, d_y, d_pos, d_w, S, K, D, d_dy, d_dw, dtype=ZZ_F32, ldg=0, ldy=0, lddy=0, stream=0):
+    """dy and dw [S, K] of experts_back_dev from dout (zz_experts_back_grad_dev); d_dw 0: not formed."""
+    if not lib().zz_experts_back_grad_dev(dtype, d_dout or None, ldg, d_y or None, ldy, d_pos or None, d_w or None, S, K, D,
+                                          d_dy or None, lddy, d_dw or None, stream or None):
+        raise RuntimeError(f"zz_experts_back_grad_dev declined: {last_error()}")
 
 
 def beam_ws_bytes(N, W, V):

@@ -16,7 +16,7 @@ HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 SOURCES = ["zz_api.hip", "zz_route.hip", "zz_ffn.hip", "zz_matmul.hip", "zz_quant.hip", "zz_mma_up.hip", "zz_mma_down.hip", "zz_decode.hip",
            "zz_gemma.hip", "zz_container.hip", "zz_flash.hip", "zz_fp8.hip", "zz_fp8_rows.hip",
-           "zz_fp8_mma.hip", "zz_beam.hip"]
+           "zz_fp8_mma.hip", "zz_fp8_ep.hip", "zz_fp8_gated.hip", "zz_experts.hip", "zz_beam.hip"]
 
 FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",

@@ -1,0 +1,433 @@
+// zz_experts.hip -- tokens to experts and back (include/zz_experts.h): the stable sort of the
+// (token, slot) pairs by expert, the rows' copies, the weighted way back and its gradient.
+//
+// All of it moves rows and is bound by their bytes; the sort is bound by latency. A lane owns 8
+// consecutive elements of a token's row (16 bytes of it, copied) and goes through the token's K
+// pairs, so a token's row is read or written once and its K partners once each.
+#include "zz_common.h"
+#include "zz_kernels.h"
+#include "zz_fp8_dev.h"
+#include "../../include/zz_experts.h"
+
+#define ZZ_FAIL(...)               \
+    do {                           \
+        zz_set_error(__VA_ARGS__); \
+        return 0;                  \
+    } while (0)
+
+#define XP_FEW 1024                 // pairs that every workgroup looks through by itself
+#define XP_ONE 8192                 // pairs that one workgroup sorts
+#define XP_CHUNKS 256               // chunks of the others' sort
+
+struct XpArgs {
+    const int *eidx;
+    int S, K, E, n;                 // n = S * K
+    int *offs, *row, *pos;
+    int chunk, chunks;              // pairs of a chunk, a multiple of 1024
+    int *count;                     // [chunks][E]
+    const uint8_t *x;               // rows as bytes, null: none
+    uint8_t *xs;
+    int64_t ldx, ldxs;              // bytes
+    int bytes;                      // of a row
+};
+
+// `bytes` (a multiple of 2) of 16 bytes at any address
+__device__ __forceinline__ zz_u4 xp_load(const uint8_t *p, int bytes) {
+    if (bytes >= 16) return *(const zz_u4any *)p;
+    zz_u4 v = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < 7; i++)
+        if (2 * i + 2 <= bytes) v[i / 2] |= (unsigned)*(const uint16_t *)(p + 2 * i) << (16 * (i & 1));
+    return v;
+}
+template <bool NT>
+__device__ __forceinline__ void xp_store(uint8_t *p, zz_u4 v, int bytes) {
+    if (bytes >= 16) {
+        if constexpr (NT) __builtin_nontemporal_store((zz_u4any)v, (zz_u4any *)p);
+        else *(zz_u4any *)p = v;
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 7; i++)
+        if (2 * i + 2 <= bytes) *(uint16_t *)(p + 2 * i) = (uint16_t)(v[i / 2] >> (16 * (i & 1)));
+}
+
+// exclusive prefix sums of v[0 .. E) into offs[0 .. E] by one wave
+template <typename PUT>
+__device__ __forceinline__ void xp_offsets(const int *v, int E, PUT put) {
+    constexpr int N = ZZ_EXPERTS_MAXE / 64;
+    const int l = threadIdx.x & 63, per = (E + 63) / 64;
+    int c[N], sum = 0;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const int e = l * per + i;
+        c[i] = i < per && e < E ? v[e] : 0;
+        sum += c[i];
+    }
+    const int upto = zz_wave_incl_scan_add(sum);
+    int at = upto - sum;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const int e = l * per + i;
+        if (i < per && e < E) put(e, at);
+        at += c[i];
+    }
+    if (l == 63) put(E, upto);
+}
+
+// Few pairs, one launch: a workgroup per token finds its pairs' positions by counting the pairs
+// before them, one more the offsets.
+__global__ __launch_bounds__(256) void zz_xp_few_kernel(XpArgs a) {
+    __shared__ int hist[ZZ_EXPERTS_MAXE], part[4][ZZ_EXPERTS_MAXK], where[ZZ_EXPERTS_MAXK];
+    const int tid = threadIdx.x, w = zz_wave_id(), l = tid & 63, s = blockIdx.x;
+    int id[XP_FEW / 256];
+#pragma unroll
+    for (int i = 0; i < XP_FEW / 256; i++) id[i] = tid + 256 * i < a.n ? a.eidx[tid + 256 * i] : -1;
+    if (s == a.S) {
+        for (int e = tid; e < a.E; e += 256) hist[e] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < XP_FEW / 256; i++)
+            if ((unsigned)id[i] < (unsigned)a.E) atomicAdd(&hist[id[i]], 1);
+        __syncthreads();
+        if (w == 0) xp_offsets(hist, a.E, [&](int e, int v) { a.offs[e] = v; });
+        return;
+    }
+    int mine = 0;
+    for (int k = 0; k < a.K; k++) {
+        const int e = a.eidx[s * a.K + k], at = s * a.K + k;
+        int c = 0;
+#pragma unroll
+        for (int i = 0; i < XP_FEW / 256; i++)
+            c += __builtin_popcountll(__ballot((unsigned)id[i] < (unsigned)a.E && (id[i] < e || (id[i] == e && tid + 256 * i < at))));
+        if (l == k) mine = c;
+    }
+    if (l < a.K) part[w][l] = mine;
+    __syncthreads();
+    if (tid < a.K) {
+        const int e = a.eidx[s * a.K + tid];
+        const int p = (unsigned)e < (unsigned)a.E ? part[0][tid] + part[1][tid] + part[2][tid] + part[3][tid] : -1;
+        a.pos[s * a.K + tid] = where[tid] = p;
+        if (p >= 0) a.row[p] = s;
+    }
+    if (!a.x) return;
+    __syncthreads();
+    for (int b = 16 * tid; b < a.bytes; b += 4096) {
+        const zz_u4 v = xp_load(a.x + s * a.ldx + b, a.bytes - b);
+        for (int k = 0; k < a.K; k++)
+            if (where[k] >= 0) xp_store<false>(a.xs + where[k] * a.ldxs + b, v, a.bytes - b);
+    }
+}
+
+// how many pairs of each expert a chunk has
+__global__ __launch_bounds__(1024) void zz_xp_count_kernel(XpArgs a) {
+    __shared__ int hist[ZZ_EXPERTS_MAXE];
+    const int tid = threadIdx.x, end = min(a.n, (int)(blockIdx.x + 1) * a.chunk);
+    for (int e = tid; e < a.E; e += 1024) hist[e] = 0;
+    __syncthreads();
+    for (int i = blockIdx.x * a.chunk + tid; i < end; i += 1024) {
+        const int e = a.eidx[i];
+        if ((unsigned)e < (unsigned)a.E) atomicAdd(&hist[e], 1);
+    }
+    __syncthreads();
+    for (int e = tid; e < a.E; e += 1024) a.count[blockIdx.x * a.E + e] = hist[e];
+}
+
+// The positions of a chunk's pairs. Each of 16 waves has a run of them: how many of an expert lie
+// in the waves before is added up in LDS; within a wave's 64 pairs, the lanes with the same expert
+// are found by a ballot for each bit of the id. Nothing depends on the order of atomics.
+template <bool ONE>
+__global__ __launch_bounds__(1024) void zz_xp_place_kernel(XpArgs a) {
+    __shared__ int wcnt[16][ZZ_EXPERTS_MAXE], total[ZZ_EXPERTS_MAXE], pre[ZZ_EXPERTS_MAXE], base[ZZ_EXPERTS_MAXE + 1];
+    const int tid = threadIdx.x, w = zz_wave_id(), l = tid & 63, E = a.E;
+    const int per = a.chunk / 16, first = blockIdx.x * a.chunk + w * per, end = min(a.n, first + per);
+    for (int i = tid; i < 16 * ZZ_EXPERTS_MAXE; i += 1024) (&wcnt[0][0])[i] = 0;
+    for (int e = tid; e < E; e += 1024) total[e] = pre[e] = 0;
+    __syncthreads();
+    for (int i = first + l; i < end; i += 64) {
+        const int e = a.eidx[i];
+        if ((unsigned)e < (unsigned)E) atomicAdd(&wcnt[w][e], 1);
+    }
+    if constexpr (!ONE) {                                 // the other chunks' pairs
+        const int lanes = (E + 63) & ~63, groups = 1024 / lanes, e = tid % lanes, g = tid / lanes;
+        if (e < E && g < groups) {
+            int all = 0, before = 0;
+            for (int c = g; c < a.chunks; c += groups) {
+                const int v = a.count[c * E + e];
+                all += v;
+                before += c < (int)blockIdx.x ? v : 0;
+            }
+            atomicAdd(&total[e], all);
+            atomicAdd(&pre[e], before);
+        }
+    }
+    __syncthreads();
+    if (tid < E) {
+        int t = 0;
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            const int v = wcnt[i][tid];
+            wcnt[i][tid] = t;
+            t += v;
+        }
+        if constexpr (ONE) total[tid] = t;
+    }
+    __syncthreads();
+    if (w == 0)
+        xp_offsets(total, E, [&](int e, int v) {
+            base[e] = v;
+            if (blockIdx.x == 0) a.offs[e] = v;
+        });
+    __syncthreads();
+    const int bits = 32 - __builtin_clz(E);               // of an id, 0 .. E - 1
+    for (int i0 = first; i0 < end; i0 += 64) {
+        const int i = i0 + l, e = i < end ? a.eidx[i] : -1;
+        const bool ok = (unsigned)e < (unsigned)E;
+        unsigned long long same = __ballot(ok);
+        for (int b = 0; b < bits; b++) {
+            const unsigned long long m = __ballot(e >> b & 1);
+            same &= e >> b & 1 ? m : ~m;
+        }
+        const int rank = __builtin_popcountll(same & ((1ull << l) - 1));
+        int p = -1;
+        if (ok) {
+            const int before = wcnt[w][e];
+            p = base[e] + (ONE ? 0 : pre[e]) + before + rank;
+            asm volatile("" ::: "memory");                // all have read it
+            if (rank == 0) wcnt[w][e] = before + __builtin_popcountll(same);
+            a.row[p] = i / a.K;
+        }
+        asm volatile("" ::: "memory");
+        if (i < end) a.pos[i] = p;
+    }
+}
+
+// the tokens' rows to their positions
+template <bool NT>
+__global__ __launch_bounds__(256) void zz_xp_rows_kernel(XpArgs a) {
+    const int units = (a.bytes + 15) / 16;
+    const unsigned id = blockIdx.x * 256u + threadIdx.x;
+    const int s = id / units, b = 16 * (id - s * units);
+    if (s >= a.S) return;
+    const zz_u4 v = xp_load(a.x + s * a.ldx + b, a.bytes - b);
+    for (int k = 0; k < a.K; k++) {
+        const int p = a.pos[s * a.K + k];
+        if (p >= 0) xp_store<NT>(a.xs + p * a.ldxs + b, v, a.bytes - b);
+    }
+}
+
+struct XpBack {
+    const void *y, *res, *dout;
+    const int *pos;
+    const float *w;
+    void *out, *dy;
+    float *dw;
+    int64_t ldy, ldr, ldo, ldg, lddy;   // elements
+    int S, K, D, n;
+};
+
+// the position of pair i, -1 for none
+__device__ __forceinline__ int xp_pos(const XpBack &a, int i) {
+    const int p = a.pos[i];
+    return (unsigned)p < (unsigned)a.n ? p : -1;
+}
+
+template <typename T, bool NT>
+__global__ __launch_bounds__(256) void zz_xp_back_kernel(XpBack a) {
+    const int units = (a.D + 7) / 8;
+    const unsigned id = blockIdx.x * 256u + threadIdx.x;
+    const int s = id / units, e = 8 * (id - s * units), n = a.D - e;
+    if (s >= a.S) return;
+    float v[8];
+    if (a.res) {
+        zz_get8(v, (const T *)a.res + s * a.ldr + e, n, false);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = 0.0f;
+    }
+    for (int k = 0; k < a.K; k++) {
+        const int p = xp_pos(a, s * a.K + k);
+        if (p < 0) continue;
+        const float w = a.w ? a.w[s * a.K + k] : 1.0f;
+        float t[8];
+        zz_get8(t, (const T *)a.y + p * a.ldy + e, n, false);
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = fmaf(w, t[j], v[j]);
+    }
+    zz_put8<NT>((T *)a.out + s * a.ldo + e, v, n);
+}
+
+// A workgroup per token: its lanes keep 8 elements of dout and go through the K rows.
+template <typename T, bool NT>
+__global__ __launch_bounds__(256) void zz_xp_grad_kernel(XpBack a) {
+    __shared__ float part[4][ZZ_EXPERTS_MAXK];
+    const int tid = threadIdx.x, w = zz_wave_id(), l = tid & 63, s = blockIdx.x;
+    for (int k = 0; k < a.K; k++) {
+        const int p = xp_pos(a, s * a.K + k);
+        float dot = 0.0f;
+        if (p >= 0) {
+            const float wt = a.w ? a.w[s * a.K + k] : 1.0f;
+            for (int e = 8 * tid; e < a.D; e += 2048) {
+                float g[8], t[8];
+                zz_get8(g, (const T *)a.dout + s * a.ldg + e, a.D - e, false);
+                if (a.dw) {
+                    zz_get8(t, (const T *)a.y + p * a.ldy + e, a.D - e, false);
+#pragma unroll
+                    for (int j = 0; j < 8; j++) dot = fmaf(g[j], t[j], dot);
+                }
+#pragma unroll
+                for (int j = 0; j < 8; j++) t[j] = wt * g[j];
+                zz_put8<NT>((T *)a.dy + p * a.lddy + e, t, a.D - e);
+            }
+        }
+        dot = zz_wave_sum(dot);
+        if (l == 0) part[w][k] = dot;
+    }
+    __syncthreads();
+    if (a.dw && tid < a.K) a.dw[s * a.K + tid] = (part[0][tid] + part[1][tid]) + (part[2][tid] + part[3][tid]);
+}
+
+// ------------------------------------------------------------------ host side
+int zz_lib_here(const char *who);                                             // zz_fp8.hip
+int zz_ranges_meet(const void *a, int64_t n, const void *b, int64_t m);
+
+static bool xp_sizes(int S, int K, int E) {
+    return S >= 1 && S <= 1 << 20 && K >= 1 && K <= ZZ_EXPERTS_MAXK && E >= 1 && E <= ZZ_EXPERTS_MAXE;
+}
+
+// pairs of a chunk: at most XP_CHUNKS chunks of whole thousands
+static int xp_chunk(int n) {
+    if (n <= XP_ONE) return (n + 1023) / 1024 * 1024;
+    const int c = ((n + XP_CHUNKS - 1) / XP_CHUNKS + 1023) / 1024 * 1024;
+    return c < 4096 ? 4096 : c;
+}
+
+extern "C" int64_t zz_experts_ws_bytes(int S, int K, int E) {
+    if (!xp_sizes(S, K, E)) return -1;
+    const int n = S * K;
+    return n <= XP_ONE ? 16 : (int64_t)((n + xp_chunk(n) - 1) / xp_chunk(n)) * E * 4;
+}
+
+// a range of memory; n = 0: none
+struct XpRange { const void *p; int64_t n; };
+static int64_t xp_span(int64_t ld, int64_t rows, int D, int esz) { return ((rows - 1) * ld + D) * esz; }
+
+// whether one of `out` has a byte in common with one of `in` or with another of `out`
+static bool xp_overlap(const XpRange *out, int no, const XpRange *in, int ni) {
+    for (int i = 0; i < no; i++) {
+        for (int j = 0; j < ni; j++)
+            if (out[i].n && in[j].n && zz_ranges_meet(out[i].p, out[i].n, in[j].p, in[j].n)) return true;
+        for (int j = 0; j < i; j++)
+            if (out[i].n && out[j].n && zz_ranges_meet(out[i].p, out[i].n, out[j].p, out[j].n)) return true;
+    }
+    return false;
+}
+
+// a row distance: 0 becomes D; false where rows would overlap
+static bool xp_ld(int64_t *ld, int D) {
+    if (!*ld) *ld = D;
+    return *ld >= D && *ld <= (int64_t)1 << 36;           // 2^24 rows' bytes stay under 2^62
+}
+
+extern "C" int zz_experts_dispatch_dev(const int *d_eidx, int S, int K, int E, int *d_offs, int *d_row, int *d_pos,
+                                       int dtype, const void *d_x, int64_t ldx, int D, void *d_xs, int64_t ldxs,
+                                       void *d_ws, size_t ws_bytes, void *stream) {
+    const char *who = "zz_experts_dispatch_dev";
+    if (!xp_sizes(S, K, E)) ZZ_FAIL("%s: S <= 2^20, K <= 16, E <= 512", who);
+    if (!d_eidx || !d_offs || !d_row || !d_pos || !d_ws || (d_x && !d_xs)) ZZ_FAIL("%s: bad arguments", who);
+    if (((uintptr_t)d_eidx | (uintptr_t)d_offs | (uintptr_t)d_row | (uintptr_t)d_pos | (uintptr_t)d_ws) % 4)
+        ZZ_FAIL("%s: misaligned pointer", who);
+    if (ws_bytes < (size_t)zz_experts_ws_bytes(S, K, E)) ZZ_FAIL("%s: the workspace is too small", who);
+    const int n = S * K, esz = dtype == ZZ_F32 ? 4 : 2;
+    if (d_x) {
+        if (dtype != ZZ_F32 && dtype != ZZ_BF16) ZZ_FAIL("%s: dtype %d declined", who, dtype);
+        if (D < 1 || D > ZZ_MAXD) ZZ_FAIL("%s: 1 <= D <= %d", who, ZZ_MAXD);
+        if (!xp_ld(&ldx, D) || !xp_ld(&ldxs, D)) ZZ_FAIL("%s: rows closer than their width", who);
+        if (((uintptr_t)d_x | (uintptr_t)d_xs) % esz) ZZ_FAIL("%s: misaligned pointer", who);
+    }
+    const int64_t nxs = d_x ? xp_span(ldxs, n, D, esz) : 0;
+    const XpRange out[] = {{d_offs, 4 * (int64_t)(E + 1)}, {d_row, 4 * (int64_t)n}, {d_pos, 4 * (int64_t)n},
+                           {d_ws, zz_experts_ws_bytes(S, K, E)}, {d_xs, nxs}};
+    const XpRange in[] = {{d_eidx, 4 * (int64_t)n}, {d_x, d_x ? xp_span(ldx, S, D, esz) : 0}};
+    if (xp_overlap(out, 5, in, 2)) ZZ_FAIL("%s: an output overlaps another argument", who);
+    if (!zz_lib_here(who)) return 0;
+    hipStream_t st = stream ? (hipStream_t)stream : zz_lib_stream();
+    XpArgs a;
+    a.eidx = d_eidx; a.S = S; a.K = K; a.E = E; a.n = n; a.offs = d_offs; a.row = d_row; a.pos = d_pos;
+    a.chunk = xp_chunk(n); a.chunks = (n + a.chunk - 1) / a.chunk; a.count = (int *)d_ws;
+    a.x = (const uint8_t *)d_x; a.xs = (uint8_t *)d_xs; a.ldx = ldx * esz; a.ldxs = ldxs * esz; a.bytes = D * esz;
+    if (n <= XP_FEW) {
+        hipLaunchKernelGGL(zz_xp_few_kernel, dim3(S + 1), dim3(256), 0, st, a);
+    } else {
+        if (n <= XP_ONE) {
+            hipLaunchKernelGGL(zz_xp_place_kernel<true>, dim3(1), dim3(1024), 0, st, a);
+        } else {
+            hipLaunchKernelGGL(zz_xp_count_kernel, dim3(a.chunks), dim3(1024), 0, st, a);
+            hipLaunchKernelGGL(zz_xp_place_kernel<false>, dim3(a.chunks), dim3(1024), 0, st, a);
+        }
+        if (d_x) {
+            const int64_t t = (int64_t)S * ((a.bytes + 15) / 16);
+            const auto k = nxs >= ZZ_NT_BYTES ? zz_xp_rows_kernel<true> : zz_xp_rows_kernel<false>;
+            hipLaunchKernelGGL(k, dim3((unsigned)((t + 255) / 256)), dim3(256), 0, st, a);
+        }
+    }
+    if (hipGetLastError() != hipSuccess) ZZ_FAIL("%s: launch failed", who);
+    return 1;
+}
+
+extern "C" int zz_experts_back_dev(int dtype, const void *d_y, int64_t ldy, const int *d_pos, const float *d_w, int S,
+                                   int K, int D, const void *d_res, int64_t ldr, void *d_out, int64_t ldo, void *stream) {
+    const char *who = "zz_experts_back_dev";
+    if (dtype != ZZ_F32 && dtype != ZZ_BF16) ZZ_FAIL("%s: dtype %d declined", who, dtype);
+    if (!xp_sizes(S, K, 1) || D < 1 || D > ZZ_MAXD) ZZ_FAIL("%s: S <= 2^20, K <= 16, D <= %d", who, ZZ_MAXD);
+    if (!d_y || !d_pos || !d_out) ZZ_FAIL("%s: bad arguments", who);
+    const int n = S * K, esz = dtype == ZZ_F32 ? 4 : 2;
+    if (!xp_ld(&ldy, D) || !xp_ld(&ldo, D) || (d_res && !xp_ld(&ldr, D))) ZZ_FAIL("%s: rows closer than their width", who);
+    if (((uintptr_t)d_y | (uintptr_t)d_res | (uintptr_t)d_out) % esz || ((uintptr_t)d_pos | (uintptr_t)d_w) % 4)
+        ZZ_FAIL("%s: misaligned pointer", who);
+    const bool own = d_res == d_out && ldr == ldo;
+    const XpRange out = {d_out, xp_span(ldo, S, D, esz)};
+    const XpRange in[] = {{d_y, xp_span(ldy, n, D, esz)}, {d_pos, 4 * (int64_t)n}, {d_w, d_w ? 4 * (int64_t)n : 0},
+                          {d_res, d_res && !own ? xp_span(ldr, S, D, esz) : 0}};
+    if (xp_overlap(&out, 1, in, 4)) ZZ_FAIL("%s: out overlaps another argument", who);
+    if (!zz_lib_here(who)) return 0;
+    XpBack a{};
+    a.y = d_y; a.ldy = ldy; a.pos = d_pos; a.w = d_w; a.S = S; a.K = K; a.D = D; a.n = n; a.res = d_res; a.ldr = ldr;
+    a.out = d_out; a.ldo = ldo;
+    const int64_t t = (int64_t)S * ((D + 7) / 8);
+    const bool nt = out.n >= ZZ_NT_BYTES;
+    const auto k = dtype == ZZ_F32 ? nt ? zz_xp_back_kernel<float, true> : zz_xp_back_kernel<float, false>
+                                   : nt ? zz_xp_back_kernel<zz_bf16, true> : zz_xp_back_kernel<zz_bf16, false>;
+    hipLaunchKernelGGL(k, dim3((unsigned)((t + 255) / 256)), dim3(256), 0, stream ? (hipStream_t)stream : zz_lib_stream(), a);
+    if (hipGetLastError() != hipSuccess) ZZ_FAIL("%s: launch failed", who);
+    return 1;
+}
+
+extern "C" int zz_experts_back_grad_dev(int dtype, const void *d_dout, int64_t ldg, const void *d_y, int64_t ldy,
+                                        const int *d_pos, const float *d_w, int S, int K, int D, void *d_dy, int64_t lddy,
+                                        float *d_dw, void *stream) {
+    const char *who = "zz_experts_back_grad_dev";
+    if (dtype != ZZ_F32 && dtype != ZZ_BF16) ZZ_FAIL("%s: dtype %d declined", who, dtype);
+    if (!xp_sizes(S, K, 1) || D < 1 || D > ZZ_MAXD) ZZ_FAIL("%s: S <= 2^20, K <= 16, D <= %d", who, ZZ_MAXD);
+    if (!d_dout || !d_pos || !d_dy || (d_dw && !d_y)) ZZ_FAIL("%s: bad arguments", who);
+    const int n = S * K, esz = dtype == ZZ_F32 ? 4 : 2;
+    if (!xp_ld(&ldg, D) || !xp_ld(&lddy, D) || (d_dw && !xp_ld(&ldy, D))) ZZ_FAIL("%s: rows closer than their width", who);
+    if (((uintptr_t)d_dout | (uintptr_t)d_dy | (d_dw ? (uintptr_t)d_y : 0)) % esz ||
+        ((uintptr_t)d_pos | (uintptr_t)d_w | (uintptr_t)d_dw) % 4)
+        ZZ_FAIL("%s: misaligned pointer", who);
+    const bool own = d_dy == d_y && lddy == ldy;
+    const XpRange out[] = {{d_dy, xp_span(lddy, n, D, esz)}, {d_dw, d_dw ? 4 * (int64_t)n : 0}};
+    const XpRange in[] = {{d_dout, xp_span(ldg, S, D, esz)}, {d_pos, 4 * (int64_t)n}, {d_w, d_w ? 4 * (int64_t)n : 0},
+                          {d_y, d_dw && !own ? xp_span(ldy, n, D, esz) : 0}};
+    if (xp_overlap(out, 2, in, 4)) ZZ_FAIL("%s: an output overlaps another argument", who);
+    if (!zz_lib_here(who)) return 0;
+    XpBack a{};
+    a.dout = d_dout; a.ldg = ldg; a.y = d_y; a.ldy = ldy; a.pos = d_pos; a.w = d_w; a.S = S; a.K = K; a.D = D; a.n = n;
+    a.dy = d_dy; a.lddy = lddy; a.dw = d_dw;
+    const bool nt = out[0].n >= ZZ_NT_BYTES;
+    const auto k = dtype == ZZ_F32 ? nt ? zz_xp_grad_kernel<float, true> : zz_xp_grad_kernel<float, false>
+                                   : nt ? zz_xp_grad_kernel<zz_bf16, true> : zz_xp_grad_kernel<zz_bf16, false>;
+    hipLaunchKernelGGL(k, dim3(S), dim3(256), 0, stream ? (hipStream_t)stream : zz_lib_stream(), a);
+    if (hipGetLastError() != hipSuccess) ZZ_FAIL("%s: launch failed", who);
+    return 1;
+}

@@ -17,6 +17,7 @@
 
 #define ZZ_F8_MAXS (1 << 20)
 #define ZZ_F8_MAXNORM 8192
+#define ZZ_F8_MAXP (1 << 24)
 
 // the library is up and its device is the current one; the last check of a call, so that
 // what is wrong with its arguments is named without a device too
@@ -101,15 +102,21 @@ extern "C" int zz_rows_fp8_dev(int dtype, const void *d_x, int64_t ldx, int S, i
 }
 
 // ------------------------------------------------------------------ resident matrices
+// a table of E matrices [O, I], or of E gated pairs; one plain matrix is a table of one
 struct Fp8Mat {
-    int O, I;
-    uint8_t *w = nullptr;           // packed codes (zz_fp8_dev.h)
-    float *ws = nullptr;
-    bool loaded = false;
+    int E, O, I, parts;             // parts: 1, gated 2
+    uint8_t *w = nullptr;           // packed codes (zz_fp8_dev.h), an expert's `wbytes` apart
+    float *ws = nullptr;            // [E][parts][ceil(O/128)][ceil(I/128)]
+    std::vector<char> loaded;       // [E][parts]
+    int missing;                    // of them
 };
 static std::vector<Fp8Mat *> g_mats;
 
-static size_t packed_bytes(const Fp8Mat *m) { return (size_t)((m->O + 31) / 32) * zz_f8_nb(m->I) * 4096; }
+static size_t wbytes(int O, int I, int parts) {
+    const int gc = 32 / parts;      // rows of a matrix in a group of 32
+    return (size_t)((O + gc - 1) / gc) * zz_f8_nb(I) * 4096;
+}
+static size_t wbytes(const Fp8Mat *m) { return wbytes(m->O, m->I, m->parts); }
 static size_t scale_count(const Fp8Mat *m) { return (size_t)zz_f8_nb(m->O) * zz_f8_nb(m->I); }
 
 static void free_mat(Fp8Mat *m) {
@@ -125,32 +132,52 @@ static Fp8Mat *get_mat(int id) {
     return g_mats[id];
 }
 
-extern "C" int zz_fp8_create(int O, int I) {
-    if (O < 1 || O > 1 << 24 || I < 1 || I > 1 << 16 || (int64_t)O * I >= (int64_t)1 << 35) {
-        zz_set_error("zz_fp8_create: bad shape (O <= 2^24, I <= 65536, O * I < 2^35)");
-        return -1;
-    }
-    if (!zz_lib_here("zz_fp8_create")) return -1;
+static int create(const char *who, int E, int O, int I, int parts) {
+    if (!zz_lib_here(who)) return -1;
     size_t id = 0;
     while (id < g_mats.size() && g_mats[id]) id++;
     Fp8Mat *m = nullptr;
     try {
         if (id == g_mats.size()) g_mats.push_back(nullptr);
         m = new Fp8Mat();
+        m->loaded.assign((size_t)E * parts, 0);
     } catch (const std::bad_alloc &) {
-        zz_set_error("zz_fp8_create: out of memory");
+        delete m;
+        zz_set_error("%s: out of memory", who);
         return -1;
     }
+    m->E = E;
     m->O = O;
     m->I = I;
-    if (hipMalloc(&m->w, packed_bytes(m)) != hipSuccess || hipMalloc(&m->ws, 4 * scale_count(m)) != hipSuccess) {
+    m->parts = parts;
+    m->missing = E * parts;
+    if (hipMalloc(&m->w, E * wbytes(m)) != hipSuccess ||
+        hipMalloc(&m->ws, 4 * E * parts * scale_count(m)) != hipSuccess) {
         (void)hipGetLastError();
-        zz_set_error("zz_fp8_create: device allocation failed");
+        zz_set_error("%s: device allocation failed", who);
         free_mat(m);
         return -1;
     }
     g_mats[id] = m;
     return (int)id;
+}
+
+extern "C" int zz_fp8_create(int O, int I) {
+    if (O < 1 || O > 1 << 24 || I < 1 || I > 1 << 16 || (int64_t)O * I >= (int64_t)1 << 35) {
+        zz_set_error("zz_fp8_create: bad shape (O <= 2^24, I <= 65536, O * I < 2^35)");
+        return -1;
+    }
+    return create("zz_fp8_create", 1, O, I, 1);
+}
+
+extern "C" int zz_fp8_create_experts(int E, int O, int I, int gated) {
+    const int parts = gated ? 2 : 1;
+    if (E < 1 || E > ZZ_F8_MAXE || O < 1 || O > 1 << 24 || I < 1 || I > 1 << 16 || (int64_t)O * I >= (int64_t)1 << 35 ||
+        (uint64_t)E * wbytes(O, I, parts) >= (uint64_t)1 << 38) {
+        zz_set_error("zz_fp8_create_experts: bad shape (E <= 512, O <= 2^24, I <= 65536, O * I < 2^35, all less than 2^38)");
+        return -1;
+    }
+    return create("zz_fp8_create_experts", E, O, I, parts);
 }
 
 extern "C" void zz_fp8_destroy(int id) {
@@ -161,40 +188,78 @@ extern "C" void zz_fp8_destroy(int id) {
     g_mats[id] = nullptr;
 }
 
-static int upload_mat(Fp8Mat *m, const uint8_t *d_codes, const void *scales, hipMemcpyKind kind) {
+// one matrix of the table, from codes on the device and scales on either side
+static int upload_mat(Fp8Mat *m, int e, int part, const uint8_t *d_codes, const void *scales, hipMemcpyKind kind) {
     hipStream_t st = zz_lib_stream();
-    m->loaded = false;
-    ZZ_CHECK(hipMemcpyAsync(m->ws, scales, 4 * scale_count(m), kind, st));
-    if (!zz_launch_fp8_pack(d_codes, m->O, m->I, m->w, st)) ZZ_FAIL("zz_fp8_upload: launch failed");
+    char &have = m->loaded[(size_t)e * m->parts + part];
+    m->missing += have;
+    have = 0;
+    float *ws = m->ws + ((size_t)e * m->parts + part) * scale_count(m);
+    ZZ_CHECK(hipMemcpyAsync(ws, scales, 4 * scale_count(m), kind, st));
+    if (!zz_launch_fp8_pack(d_codes, m->O, m->I, m->parts == 2 ? part : -1, m->w + e * wbytes(m), st))
+        ZZ_FAIL("zz_fp8_upload: launch failed");
     ZZ_CHECK(hipStreamSynchronize(st));
-    m->loaded = true;
+    have = 1;
+    m->missing--;
     return 1;
+}
+
+static int upload_host(const char *who, Fp8Mat *m, int e, int part, const uint8_t *codes, const float *scales) {
+    uint8_t *d = nullptr;
+    const size_t n = (size_t)m->O * m->I;
+    if (hipMalloc(&d, n) != hipSuccess) {
+        (void)hipGetLastError();
+        ZZ_FAIL("%s: device allocation failed", who);
+    }
+    const int ok = hipMemcpy(d, codes, n, hipMemcpyHostToDevice) == hipSuccess &&
+                   upload_mat(m, e, part, d, scales, hipMemcpyHostToDevice);
+    (void)hipFree(d);
+    if (!ok) ZZ_FAIL("%s: failed", who);
+    return 1;
+}
+
+// a matrix that is no table
+static Fp8Mat *plain_mat(int id) {
+    Fp8Mat *m = get_mat(id);
+    return m && m->E == 1 && m->parts == 1 ? m : nullptr;
 }
 
 extern "C" int zz_fp8_upload(int id, const uint8_t *codes, const float *scales) {
     if (!codes || !scales) ZZ_FAIL("zz_fp8_upload: bad arguments");
     if (!zz_lib_here("zz_fp8_upload")) return 0;
-    Fp8Mat *m = get_mat(id);
+    Fp8Mat *m = plain_mat(id);
     if (!m) ZZ_FAIL("zz_fp8_upload: no such matrix");
-    uint8_t *d = nullptr;
-    const size_t n = (size_t)m->O * m->I;
-    if (hipMalloc(&d, n) != hipSuccess) {
-        (void)hipGetLastError();
-        ZZ_FAIL("zz_fp8_upload: device allocation failed");
-    }
-    const int ok = hipMemcpy(d, codes, n, hipMemcpyHostToDevice) == hipSuccess &&
-                   upload_mat(m, d, scales, hipMemcpyHostToDevice);
-    (void)hipFree(d);
-    if (!ok) ZZ_FAIL("zz_fp8_upload: failed");
-    return 1;
+    return upload_host("zz_fp8_upload", m, 0, 0, codes, scales);
 }
 
 extern "C" int zz_fp8_upload_dev(int id, const uint8_t *d_codes, const float *d_scales) {
     if (!d_codes || !d_scales || (uintptr_t)d_scales % 4) ZZ_FAIL("zz_fp8_upload_dev: bad arguments");
     if (!zz_lib_here("zz_fp8_upload_dev")) return 0;
-    Fp8Mat *m = get_mat(id);
+    Fp8Mat *m = plain_mat(id);
     if (!m) ZZ_FAIL("zz_fp8_upload_dev: no such matrix");
-    return upload_mat(m, d_codes, d_scales, hipMemcpyDeviceToDevice);
+    return upload_mat(m, 0, 0, d_codes, d_scales, hipMemcpyDeviceToDevice);
+}
+
+static Fp8Mat *expert_mat(const char *who, int id, int e, int part) {
+    if (!zz_lib_here(who)) return nullptr;
+    Fp8Mat *m = get_mat(id);
+    if (m && e >= 0 && e < m->E && part >= 0 && part < m->parts) return m;
+    zz_set_error("%s: no such table, expert or part", who);
+    return nullptr;
+}
+
+extern "C" int zz_fp8_upload_expert(int id, int e, int part, const uint8_t *codes, const float *scales) {
+    const char *who = "zz_fp8_upload_expert";
+    if (!codes || !scales) ZZ_FAIL("%s: bad arguments", who);
+    Fp8Mat *m = expert_mat(who, id, e, part);
+    return m ? upload_host(who, m, e, part, codes, scales) : 0;
+}
+
+extern "C" int zz_fp8_upload_expert_dev(int id, int e, int part, const uint8_t *d_codes, const float *d_scales) {
+    const char *who = "zz_fp8_upload_expert_dev";
+    if (!d_codes || !d_scales || (uintptr_t)d_scales % 4) ZZ_FAIL("%s: bad arguments", who);
+    Fp8Mat *m = expert_mat(who, id, e, part);
+    return m ? upload_mat(m, e, part, d_codes, d_scales, hipMemcpyDeviceToDevice) : 0;
 }
 
 extern "C" int zz_fp8_matmul_dev(int id, const uint8_t *d_q, const float *d_s, int S, int dtype, void *d_y,
@@ -206,8 +271,8 @@ extern "C" int zz_fp8_matmul_dev(int id, const uint8_t *d_q, const float *d_s, i
     if ((uintptr_t)d_q % 16 || (uintptr_t)d_s % 4 || (uintptr_t)d_y % esz)
         ZZ_FAIL("zz_fp8_matmul_dev: misaligned pointer");
     if (!zz_lib_here("zz_fp8_matmul_dev")) return 0;
-    Fp8Mat *m = get_mat(id);
-    if (!m || !m->loaded) ZZ_FAIL("zz_fp8_matmul_dev: no such matrix, or it has no weights yet");
+    Fp8Mat *m = plain_mat(id);
+    if (!m || m->missing) ZZ_FAIL("zz_fp8_matmul_dev: no such matrix, or it has no weights yet");
     if (!ldy) ldy = m->O;
     if (ldy < m->O) ZZ_FAIL("zz_fp8_matmul_dev: rows of y closer than their width");
     if ((int64_t)S * m->O >= (int64_t)1 << 37) ZZ_FAIL("zz_fp8_matmul_dev: S * O < 2^37");
@@ -223,8 +288,8 @@ extern "C" int zz_fp8_matmul_dev(int id, const uint8_t *d_q, const float *d_s, i
 extern "C" int zz_fp8_matmul(int id, const float *x, float *y, int S) {
     if (!x || !y || S < 1 || S > ZZ_F8_MAXS) ZZ_FAIL("zz_fp8_matmul: bad arguments (1 <= S <= 2^20)");
     if (!zz_lib_here("zz_fp8_matmul")) return 0;
-    Fp8Mat *m = get_mat(id);
-    if (!m || !m->loaded) ZZ_FAIL("zz_fp8_matmul: no such matrix, or it has no weights yet");
+    Fp8Mat *m = plain_mat(id);
+    if (!m || m->missing) ZZ_FAIL("zz_fp8_matmul: no such matrix, or it has no weights yet");
     if ((int64_t)S * zz_f8_nb(m->I) > 1 << 27) ZZ_FAIL("zz_fp8_matmul: S * ceil(I/128) <= 2^27");
     hipStream_t st = zz_lib_stream();
     float *dx = nullptr, *ds = nullptr, *dy = nullptr;
@@ -244,6 +309,80 @@ extern "C" int zz_fp8_matmul(int id, const float *x, float *y, int S) {
     for (void *p : ps)
         if (p) (void)hipFree(p);
     return ok;                      // the failing step said why
+}
+
+// ------------------------------------------------------------------ with an epilogue, and experts
+// what both calls check without a device
+static int ep_common(const char *who, const ZzF8EpCall &c) {
+    if (c.dtype != ZZ_F32 && c.dtype != ZZ_BF16) ZZ_FAIL("%s: dtype %d declined", who, c.dtype);
+    if (c.act < ZZ_EP_NONE || c.act > ZZ_EP_SILU) ZZ_FAIL("%s: activation %d declined", who, c.act);
+    if (!(c.clamp >= 0.0f) || isinf(c.clamp)) ZZ_FAIL("%s: clamp has to be finite and not negative", who);
+    const int64_t far = (int64_t)1 << 36;                 // P rows' bytes stay under 2^62
+    if (!c.q || !c.s || !c.y || c.ldy < 0 || c.ldy > far || c.ldr < 0 || c.ldr > far) ZZ_FAIL("%s: bad arguments", who);
+    const int esz = c.dtype == ZZ_F32 ? 4 : 2;
+    if ((uintptr_t)c.q % 16 || (uintptr_t)c.s % 4 || (uintptr_t)c.y % esz || (uintptr_t)c.res % esz ||
+        (uintptr_t)c.bias % 4 || (uintptr_t)c.row % 4 || (uintptr_t)c.offs % 4)
+        ZZ_FAIL("%s: misaligned pointer", who);
+    return 1;
+}
+
+static int ep_run(const char *who, Fp8Mat *m, ZzF8EpCall &c, void *stream) {
+    const int esz = c.dtype == ZZ_F32 ? 4 : 2, nb = zz_f8_nb(m->I);
+    if (m->parts == 1 && c.clamp > 0.0f) ZZ_FAIL("%s: a clamp is a gated pair's", who);
+    if (!c.ldy) c.ldy = m->O;
+    if (!c.ldr) c.ldr = m->O;
+    if (c.ldy < m->O || (c.res && c.ldr < m->O)) ZZ_FAIL("%s: rows closer than their width", who);
+    if ((int64_t)c.P * m->O >= (int64_t)1 << 37) ZZ_FAIL("%s: results of 2^37 elements or more", who);
+    if (c.row && (uint64_t)c.R * zz_fp8_row_bytes(m->I) >= (uint64_t)1 << 32)
+        ZZ_FAIL("%s: rows by index within 2^32 bytes", who);
+    const int64_t ny = span(c.ldy, c.P, m->O, esz);
+    const bool own = c.res == c.y && c.ldr == c.ldy;
+    int bad = zz_ranges_meet(c.y, ny, c.q, c.R * zz_fp8_row_bytes(m->I)) || zz_ranges_meet(c.y, ny, c.s, (int64_t)nb * c.R * 4);
+    if (c.bias) bad |= zz_ranges_meet(c.y, ny, c.bias, (int64_t)c.E * m->parts * m->O * 4);
+    if (c.res && !own) bad |= zz_ranges_meet(c.y, ny, c.res, span(c.ldr, c.P, m->O, esz));
+    if (c.row) bad |= zz_ranges_meet(c.y, ny, c.row, (int64_t)c.P * 4);
+    if (c.offs) bad |= zz_ranges_meet(c.y, ny, c.offs, (int64_t)(c.E + 1) * 4);
+    if (bad) ZZ_FAIL("%s: y overlaps another argument", who);
+    c.m = ZzF8Mat{m->O, m->I, m->w, m->ws};
+    c.we = (int64_t)wbytes(m);
+    c.wsu = (int)scale_count(m);
+    c.wse = m->parts * c.wsu;
+    hipStream_t st = stream ? (hipStream_t)stream : zz_lib_stream();
+    if (!(m->parts == 2 ? zz_launch_fp8_gated(c, st) : zz_launch_fp8_ep(c, st))) ZZ_FAIL("%s: launch failed", who);
+    return 1;
+}
+
+extern "C" int zz_fp8_matmul_ep_dev(int id, const uint8_t *d_q, const float *d_s, int S, const float *d_bias, int act,
+                                    float clamp, const void *d_res, int64_t ldr, int dtype, void *d_y, int64_t ldy,
+                                    void *stream) {
+    const char *who = "zz_fp8_matmul_ep_dev";
+    ZzF8EpCall c{};
+    c.q = d_q; c.s = d_s; c.R = c.P = S; c.E = 1; c.bias = d_bias; c.res = d_res; c.ldr = ldr; c.act = act;
+    c.clamp = clamp; c.dtype = dtype; c.y = d_y; c.ldy = ldy;
+    if (!ep_common(who, c)) return 0;
+    if (S < 1 || S > ZZ_F8_MAXS) ZZ_FAIL("%s: bad arguments (1 <= S <= 2^20)", who);
+    if (!zz_lib_here(who)) return 0;
+    Fp8Mat *m = get_mat(id);
+    if (!m || m->E != 1 || m->missing) ZZ_FAIL("%s: no such matrix, or it has no weights yet", who);
+    return ep_run(who, m, c, stream);
+}
+
+extern "C" int zz_fp8_matmul_experts_dev(int id, const uint8_t *d_q, const float *d_s, int R, const int *d_row,
+                                         const int *d_offs, int P, const float *d_bias, int act, float clamp,
+                                         const void *d_res, int64_t ldr, int dtype, void *d_y, int64_t ldy,
+                                         void *stream) {
+    const char *who = "zz_fp8_matmul_experts_dev";
+    ZzF8EpCall c{};
+    c.q = d_q; c.s = d_s; c.R = R; c.P = P; c.row = d_row; c.offs = d_offs; c.bias = d_bias; c.res = d_res;
+    c.ldr = ldr; c.act = act; c.clamp = clamp; c.dtype = dtype; c.y = d_y; c.ldy = ldy;
+    if (!ep_common(who, c)) return 0;
+    if (!d_offs || P < 1 || P > ZZ_F8_MAXP || R < 1 || R > ZZ_F8_MAXP) ZZ_FAIL("%s: bad arguments (1 <= P, R <= 2^24)", who);
+    if (!d_row && R < P) ZZ_FAIL("%s: without an index R >= P", who);
+    if (!zz_lib_here(who)) return 0;
+    Fp8Mat *m = get_mat(id);
+    if (!m || m->missing) ZZ_FAIL("%s: no such table, or it has experts without weights", who);
+    c.E = m->E;
+    return ep_run(who, m, c, stream);
 }
 
 // released by gpu_shutdown (zz_api.hip)

@@ -5,6 +5,7 @@
 
 #define ZZ_F8B 128                  // elements under one scale
 #define ZZ_F8MAX 448.0f             // largest e4m3 value
+#define ZZ_F8_MAXE 512              // experts of a table
 #define ZZ_F8FLOOR 0x1p-100f        // a block's largest magnitude counts as at least this
 
 // element types of the unquantised side, as in include/zz_fp8.h
@@ -111,6 +112,30 @@ struct ZzF8Mat {
 };
 __host__ __device__ __forceinline__ int zz_f8_nb(int n) { return (n + ZZ_F8B - 1) / ZZ_F8B; }
 
-int zz_launch_fp8_pack(const uint8_t *codes, int O, int I, uint8_t *dst, hipStream_t st);
+// part: -1 a plain matrix; 0, 1 gate's or up's half of a gated pair, whose 32-row groups are 16
+// rows of each (zz_fp8_mma.h)
+int zz_launch_fp8_pack(const uint8_t *codes, int O, int I, int part, uint8_t *dst, hipStream_t st);
 int zz_launch_fp8_matmul(const ZzF8Mat &m, const uint8_t *q, const float *s, int S, int dtype, void *y,
                          int64_t ldy, hipStream_t st);
+
+// The product with an epilogue, and over a table of experts (zz_fp8_ep.h)
+struct ZzF8EpCall {
+    ZzF8Mat m;                  // the first expert's; O columns of y
+    int64_t we;                 // bytes of an expert's codes
+    int wse, wsu;               // floats of an expert's scales, of gate's before up's
+    const uint8_t *q;
+    const float *s;
+    int R, P;                   // rows of q, rows of y
+    const int *row, *offs;      // each may be null
+    int E;
+    const float *bias;
+    const void *res;
+    int64_t ldr;
+    int act;
+    float clamp;
+    int dtype;
+    void *y;
+    int64_t ldy;
+};
+int zz_launch_fp8_ep(const ZzF8EpCall &c, hipStream_t st);
+int zz_launch_fp8_gated(const ZzF8EpCall &c, hipStream_t st);
