@@ -93,25 +93,33 @@ __global__ __launch_bounds__(64 * NW) void zz_fp8_few_ep_kernel(ZzF8Ep a) {
     zz_fp8_few<T, G, RG, RS, NW, PF, NT>(a, part, blockIdx.x % OT * RG, st * 32 * RS);
 }
 
-// Tiles of 32 RO WO packed rows x 32 RS WS rows, XCD by XCD in the order of the experts, so that
-// an expert's codes are read into one XCD's L2.
-template <typename T, int G, int RO, int RS, int WO, int WS, int KS, int NS, bool NT>
-__global__ __launch_bounds__(64 * WO * WS * KS, 2) void zz_fp8_tiles_ep_kernel(ZzF8Ep a) {
-    typedef ZzF8Async<RO, RS, WO, WS, KS, NS> C;
-    extern __shared__ __attribute__((aligned(1024))) char lds[];
-    constexpr int OC = C::O / 32 * zz_f8_gw<G>;
+// A workgroup's tile of 32 TG packed rows x TS rows: its column and row tile, the arguments made
+// its expert's. Tiles go XCD by XCD in the order of the experts, so that an expert's codes are read
+// into one XCD's L2.
+template <int G, typename T, int TG, int TS>
+__device__ __forceinline__ bool zz_f8_place(ZzF8Ep &a, int *ot, int *st) {
+    constexpr int OC = TG * zz_f8_gw<G>;
     const int OT = (a.m.O + OC - 1) / OC;
-    int id = blockIdx.x, ot, st;
+    int id = blockIdx.x;
     if (a.offs) {
         ZzF8Found f;
-        if (!zz_f8_find<C::S, true>(a, OT, id, f)) return;
+        if (!zz_f8_find<TS, true>(a, OT, id, f)) return false;
         zz_f8_expert<G, T>(a, f);
         id -= f.before * OT;
     } else {
         id = id % 8 * (gridDim.x / 8) + id / 8;
-        if (id >= (a.S + C::S - 1) / C::S * OT) return;
+        if (id >= (a.S + TS - 1) / TS * OT) return false;
     }
-    zz_fp8_at(id, OT, (a.S + C::S - 1) / C::S, &ot, &st);
+    zz_fp8_at(id, OT, (a.S + TS - 1) / TS, ot, st);
+    return true;
+}
+
+template <typename T, int G, int RO, int RS, int WO, int WS, int KS, int NS, bool NT>
+__global__ __launch_bounds__(64 * WO * WS * KS, 2) void zz_fp8_tiles_ep_kernel(ZzF8Ep a) {
+    typedef ZzF8Async<RO, RS, WO, WS, KS, NS> C;
+    extern __shared__ __attribute__((aligned(1024))) char lds[];
+    int ot, st;
+    if (!zz_f8_place<G, T, C::O / 32, C::S>(a, &ot, &st)) return;
     zz_fp8_tile<T, G, RO, RS, WO, WS, KS, NS, NT>(a, lds, ot * C::O / 32, st * C::S);
 }
 
@@ -121,29 +129,35 @@ static inline int64_t ep_tiles(const ZzF8EpCall &c, int ts) {
     return (c.P + m * (ts - 1)) / ts;
 }
 
+// whether a launch in one dimension holds n workgroups of `threads`
+static inline bool ep_fits(int64_t n, int threads) { return n * threads <= 0xffffffffll; }
+
 template <typename T, int G, int RG, int RS, int NW, bool PF, bool NT>
 static bool launch_few_ep(const ZzF8EpCall &c, const ZzF8Ep &a, hipStream_t st) {
     constexpr int OC = RG * zz_f8_gw<G>;
     const int64_t n = ep_tiles(c, 32 * RS) * ((a.m.O + OC - 1) / OC);
-    if (n * 64 * NW > 0xffffffffll) return false;         // a launch's threads in one dimension
+    if (!ep_fits(n, 64 * NW)) return false;
     hipLaunchKernelGGL((zz_fp8_few_ep_kernel<T, G, RG, RS, NW, PF, NT>), dim3((unsigned)n), dim3(64 * NW), NW * RG * RS * 4096, st, a);
     return true;
 }
 
-template <typename T, int G, int RO, int RS, int WO, int WS, int KS, int NS, bool CANNT>
-static bool launch_tiles_ep(const ZzF8EpCall &c, const ZzF8Ep &a, hipStream_t st) {
-    typedef ZzF8Async<RO, RS, WO, WS, KS, NS> C;
+template <typename C, int G>
+static bool launch_tiles_ep(const ZzF8EpCall &c, const ZzF8Ep &a, void (*kernel)(ZzF8Ep), hipStream_t st) {
     constexpr int OC = C::O / 32 * zz_f8_gw<G>;
     const int64_t n = (ep_tiles(c, C::S) * ((a.m.O + OC - 1) / OC) + 7) / 8 * 8;
-    if (n * C::NT > 0xffffffffll) return false;           // a launch's threads in one dimension
-    // large results past the caches where tiles write whole lines, as zz_fp8_mma.hip's
-    const bool nt = CANNT && c.P * a.ldy * (int64_t)sizeof(T) >= ZZ_NT_BYTES && (uintptr_t)a.y % 64 == 0 &&
-                    a.ldy * sizeof(T) % 64 == 0;
-    const auto k = nt ? zz_fp8_tiles_ep_kernel<T, G, RO, RS, WO, WS, KS, NS, CANNT>
-                      : zz_fp8_tiles_ep_kernel<T, G, RO, RS, WO, WS, KS, NS, false>;
-    hipLaunchKernelGGL(k, dim3((unsigned)n), dim3(C::NT), C::LDS, st, a);
+    if (!ep_fits(n, C::NT)) return false;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)n), dim3(C::NT), C::LDS, st, a);
     return true;
 }
+
+template <typename T, int G, int RO, int RS, int WO, int WS, int KS, int NS, bool CANNT>
+static bool launch_async_ep(const ZzF8EpCall &c, const ZzF8Ep &a, hipStream_t st) {
+    typedef ZzF8Async<RO, RS, WO, WS, KS, NS> C;
+    return launch_tiles_ep<C, G>(c, a, CANNT && a.nt ? zz_fp8_tiles_ep_kernel<T, G, RO, RS, WO, WS, KS, NS, CANNT>
+                                                     : zz_fp8_tiles_ep_kernel<T, G, RO, RS, WO, WS, KS, NS, false>, st);
+}
+
+#include "zz_fp8_wide.h"
 
 template <typename T, int G>
 static bool launch_ep(const ZzF8EpCall &c, hipStream_t st) {
@@ -151,10 +165,12 @@ static bool launch_ep(const ZzF8EpCall &c, hipStream_t st) {
     a.m = c.m; a.q = c.q; a.s = c.s; a.S = c.P; a.nb = zz_f8_nb(c.m.I); a.y = c.y; a.ldy = c.ldy;
     a.R = c.R; a.row = c.row; a.bias = c.bias; a.res = c.res; a.ldr = c.ldr; a.act = c.act; a.clamp = c.clamp;
     a.offs = c.offs; a.E = c.E; a.P = c.P; a.we = c.we; a.wse = c.wse; a.wsu = c.wsu;
+    // large results past the caches where tiles write whole lines, as zz_fp8_mma.hip's
+    a.nt = c.P * a.ldy * (int64_t)sizeof(T) >= ZZ_NT_BYTES && (uintptr_t)a.y % 64 == 0 && a.ldy * sizeof(T) % 64 == 0;
     // the rows of an expert, were they spread evenly
     const int m = c.offs ? (c.E < c.P ? c.E : c.P) : 1, per = (c.P + m - 1) / m;
     const int O = G * c.m.O;                              // packed rows
-    const int v = zz_fp8_form(O, per, m, a.nb);
+    const int v = zz_fp8_form(O, per, m, a.nb, sizeof(T) == 2 ? ZZ_F8_FORMS_BF16 : ZZ_F8_FORMS_F32);
     const bool nt = per <= 32 && (int64_t)m * O * c.m.I >= ZZ_NT_BYTES;
     bool ok = false;
     if (v == 0) ok = launch_few_ep<T, G, 1, 1, 16, false, false>(c, a, st);
@@ -162,11 +178,18 @@ static bool launch_ep(const ZzF8EpCall &c, hipStream_t st) {
     else if (v == 1 && nt) ok = launch_few_ep<T, G, 2, 1, 4, true, true>(c, a, st);
     else if (v == 1) ok = launch_few_ep<T, G, 1, 1, 4, true, false>(c, a, st);
     else if (v == 2) ok = launch_few_ep<T, G, 2, 1, 8, false, false>(c, a, st);
-    else if (v == 3) ok = launch_tiles_ep<T, G, 1, 1, 2, 1, 2, 2, false>(c, a, st);
-    else if (v == 4) ok = launch_tiles_ep<T, G, 1, 2, 2, 1, 4, 2, false>(c, a, st);
-    else if (v == 5) ok = launch_tiles_ep<T, G, 1, 2, 2, 1, 2, 2, false>(c, a, st);
-    else if (v == 6) ok = launch_tiles_ep<T, G, 1, 1, 2, 2, 1, 3, false>(c, a, st);
-    else if (v <= 8) ok = launch_tiles_ep<T, G, 1, 2, 2, 2, 1, 2, true>(c, a, st);
-    // the largest tiles also where the smaller ones are more than a launch holds
-    return ok || launch_tiles_ep<T, G, 2, 2, 2, 2, 1, 2, true>(c, a, st);
+    else if (v == 3) ok = launch_async_ep<T, G, 1, 1, 2, 1, 2, 2, false>(c, a, st);
+    else if (v == 4) ok = launch_async_ep<T, G, 1, 2, 2, 1, 4, 2, false>(c, a, st);
+    else if (v == 5) ok = launch_async_ep<T, G, 1, 2, 2, 1, 2, 2, false>(c, a, st);
+    if (ok) return true;
+    // the largest tiles also where smaller ones are more than a launch holds
+    if constexpr (sizeof(T) == 2) {
+        if (v == 11 && launch_wide<G, 1, 1, 2, 2, 2, 4>(c, a, st)) return true;
+        if (v == 12 && launch_wide<G, 2, 1, 2, 2, 2, 3>(c, a, st)) return true;
+        return launch_wide<G, 2, 1, 2, 4, 2, 4>(c, a, st);
+    } else {
+        if (v == 6 && launch_async_ep<T, G, 1, 1, 2, 2, 1, 3, false>(c, a, st)) return true;
+        if (v == 7 && launch_async_ep<T, G, 1, 2, 2, 2, 1, 2, true>(c, a, st)) return true;
+        return launch_async_ep<T, G, 2, 2, 2, 2, 1, 2, true>(c, a, st);
+    }
 }

@@ -99,6 +99,7 @@ struct ZzF8Ep : ZzF8Mm {
     int64_t ldr;
     int act;                    // ZZ_EP_*
     float clamp;
+    int nt;                     // large tiles' results are stored past the caches
     const int *offs;            // [E + 1], or null: one matrix for all rows
     int E, P;
     int64_t we;                 // bytes of an expert's codes
@@ -125,18 +126,47 @@ __device__ __forceinline__ int zz_f8_row(const A &a, int t) {
     }
 }
 
+// N (4 or 8) elements at any address as f32, n of them inside
+template <int N, typename T>
+__device__ __forceinline__ void zz_f8_load(float (&v)[N], const T *p, int n) {
+    if (n >= N) {
+        if constexpr (N == 4 && sizeof(T) == 2) {
+            const zz_u2any a = *(const zz_u2any *)p;
+#pragma unroll
+            for (int j = 0; j < 4; j++) v[j] = __uint_as_float(j & 1 ? a[j >> 1] & 0xffff0000u : a[j >> 1] << 16);
+        } else {
+#pragma unroll
+            for (int q = 0; q < N * (int)sizeof(T) / 16; q++) {
+                const zz_u4 a = *((const zz_u4any *)p + q);
+#pragma unroll
+                for (int j = 0; j < 16 / (int)sizeof(T); j++)
+                    if constexpr (sizeof(T) == 4) v[4 * q + j] = __uint_as_float(a[j]);
+                    else v[8 * q + j] = __uint_as_float(j & 1 ? a[j >> 1] & 0xffff0000u : a[j >> 1] << 16);
+            }
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < N; i++) v[i] = i < n ? zz_f32_of(p[i]) : 0.0f;
+}
+
 // N sums (gated: and up's) of columns o .. o + n - 1 to results: bias, activation, gate, residual
 // (res: the row's at column o). One hardware exponential and one reciprocal a result; sums that
 // are NaN stay so.
 template <int G, int N, typename T>
 __device__ __forceinline__ void zz_f8_end(const ZzF8Ep &a, float (&v)[N], float (&u)[N], int o, int n, const T *res) {
-    if (a.bias)
+    float t[N];
+    if (a.bias) {
+        zz_f8_load(t, a.bias + o, n);
 #pragma unroll
-        for (int i = 0; i < N; i++)
-            if (i < n) {
-                v[i] += a.bias[o + i];
-                if constexpr (G == 2) u[i] += a.bias[a.m.O + o + i];
-            }
+        for (int i = 0; i < N; i++) v[i] += t[i];
+        if constexpr (G == 2) {
+            zz_f8_load(t, a.bias + a.m.O + o, n);
+#pragma unroll
+            for (int i = 0; i < N; i++) u[i] += t[i];
+        }
+    }
+    if (a.res) zz_f8_load(t, res, n);
     if constexpr (G == 2)
         if (a.clamp > 0.0f)
 #pragma unroll
@@ -156,8 +186,7 @@ __device__ __forceinline__ void zz_f8_end(const ZzF8Ep &a, float (&v)[N], float 
         for (int i = 0; i < N; i++) v[i] *= u[i];
     if (a.res)
 #pragma unroll
-        for (int i = 0; i < N; i++)
-            if (i < n) v[i] += zz_f32_of(res[i]);
+        for (int i = 0; i < N; i++) v[i] += t[i];
 }
 
 // Few rows: a workgroup per RG groups of 32 matrix rows and RS tiles of 32 activation rows;
@@ -282,6 +311,28 @@ __device__ __forceinline__ void zz_wait_vm() {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
+// A matrix's scales, one of 64 blocks in each lane: a round takes its own from there by a readlane,
+// where a load just before the round's wait for its codes would be waited for with them (512 x 4224 x
+// 2816 took 26.4 us with that and takes 25.1). The loads are waited for where they are made, so
+// that nothing waits for them elsewhere.
+struct ZzF8Scales {
+    const float *p;
+    int nb, base = 0;
+    float v;
+    __device__ __forceinline__ ZzF8Scales(const float *from, int n) : p(from), nb(n) { load(); }
+    __device__ __forceinline__ void load() {
+        v = p[min(base + (int)(threadIdx.x & 63), nb - 1)];
+        asm volatile("" : "+v"(v));
+    }
+    __device__ __forceinline__ float of(int b) {           // b ascending, less than nb
+        if (b >= base + 64) {
+            base = b & ~63;
+            load();
+        }
+        return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), b & 63));
+    }
+};
+
 // Many rows: a workgroup owns a tile of 32*RO*WO matrix rows times 32*RS*WS activation rows.
 // KS groups of WO*WS waves take every KS-th block of 128 columns; a wave owns RO x RS tiles of
 // 32 x 32. Blocks arrive in LDS NS - 1 rounds ahead without passing registers: matrix codes in
@@ -349,6 +400,7 @@ __device__ __forceinline__ void zz_fp8_tile(const A &a, char *lds, int gt, int t
         for (int i = 0; i < C::XI; i++) zz_dma16(xsrc + (size_t)b * ZZ_F8B, xo[i], d + C::WB + (w * C::XI + i) * 1024);
         zz_dma4(ssrc + (size_t)b * rs, so, d + C::WB + C::XB + w % SI * 256);
     };
+    ZzF8Scales wsl(wsp, nb), wul(wup, nb);
     zz_v16f acc[RO][RS];
 #pragma unroll
     for (int i = 0; i < RO; i++)
@@ -361,7 +413,6 @@ __device__ __forceinline__ void zz_fp8_tile(const A &a, char *lds, int gt, int t
     int slot = 0, into = NS - 1;
     for (int it = 0; it < rounds; it++) {
         const int b = it * KS + kg;
-        const float wsc = b < nb ? wsp[b] : 0.0f, wsc2 = G == 2 && b < nb ? wup[b] : 0.0f;
         // round it has arrived for this wave; behind the barrier, for all, and the one before it
         // is read
         if (it + NS - 2 < rounds) zz_wait_vm<C::DMA *(NS - 2)>();
@@ -374,6 +425,7 @@ __device__ __forceinline__ void zz_fp8_tile(const A &a, char *lds, int gt, int t
         slot = slot + 1 == NS ? 0 : slot + 1;
         into = into + 1 == NS ? 0 : into + 1;
         if (KS > 1 && b >= nb) continue;
+        const float wsc = wsl.of(b), wsc2 = G == 2 ? wul.of(b) : wsc;
         float sc[RS], sc2[RS];
 #pragma unroll
         for (int j = 0; j < RS; j++) {
@@ -459,5 +511,8 @@ __device__ __forceinline__ void zz_fp8_at(int id, int OT, int ST, int *ot, int *
 }
 
 // The form that is expected to take the shortest for `tables` products of S rows each
-// (zz_fp8_mma.hip)
-int zz_fp8_form(int O, int S, int tables, int nb);
+// (zz_fp8_mma.hip), of all plain ones, or of those with an epilogue and results in f32 or bf16
+#define ZZ_F8_FORMS_PLAIN 0
+#define ZZ_F8_FORMS_F32   1
+#define ZZ_F8_FORMS_BF16  2
+int zz_fp8_form(int O, int S, int tables, int nb, int of);

@@ -136,19 +136,24 @@ static const ZzF8Form mm_forms[] = {
     {64, 128, 1, 3, {3.4f, 6.0f, 4.0f}, {0.74f, 0.96f, 1.49f}, 2, {0.2f, 0.05f, 0.10f}},
     {128, 128, 1, 2, {4.5f, 7.8f}, {1.04f, 1.59f}},
     {128, 128, 1, 2, {4.5f, 7.8f}, {1.04f, 1.59f}, 4, {1.6f, 0.03f, 0.13f}},
+    // zz_fp8_wide.h's, from 512 and 2816 columns with one to `per` workgroups on each CU
+    {64, 64, 1, 4, {3.6f, 4.7f, 6.0f, 6.5f}, {0.46f, 0.49f, 0.53f, 0.73f}},
+    {128, 64, 1, 3, {5.1f, 6.5f, 7.9f}, {0.52f, 0.58f, 0.88f}},
+    {128, 128, 1, 2, {6.5f, 9.2f}, {0.63f, 0.94f}},
 };
-int zz_fp8_form(int O, int S, int tables, int nb) {
+int zz_fp8_form(int O, int S, int tables, int nb, int of) {
     int best = 0;
     float least = INFINITY;
     // up to 32 rows the first three: the others' tiles are half empty
-    for (int v = 0; v < (S <= 32 ? 3 : (int)(sizeof mm_forms / sizeof *mm_forms)); v++) {
+    for (int v = 0; v < (S <= 32 ? 3 : of == ZZ_F8_FORMS_BF16 ? 14 : 11); v++) {
         const ZzF8Form &f = mm_forms[v];
+        if ((of == ZZ_F8_FORMS_BF16 && v >= 6 && v < 11) || (of && f.parts)) continue;
         int64_t n = (int64_t)((O + f.o - 1) / f.o) * ((S + f.s - 1) / f.s) * tables;
         const int r = (nb + f.ks - 1) / f.ks, cap = 256 * f.per;
         float t = 0.0f;
         if (f.parts) {
             const int parts = (int)(n % 256) * f.parts;
-            if (!parts || parts > 256 || tables > 1) continue;
+            if (!parts || parts > 256) continue;
             n -= n % 256;
             t = n % cap ? f.busy[0] + (f.busy[1] + f.busy[2] * parts / 256.0f) * r : 2.9f + 0.49f * r;
         }
@@ -165,7 +170,7 @@ int zz_fp8_form(int O, int S, int tables, int nb) {
 
 template <typename T>
 static bool launch_mm(const ZzF8Mm &a, hipStream_t st) {
-    const int v = zz_fp8_form(a.m.O, a.S, 1, a.nb);
+    const int v = zz_fp8_form(a.m.O, a.S, 1, a.nb, ZZ_F8_FORMS_PLAIN);
     if (v == 0) return launch_few<T, 1, 1, 16, false, false>(a, st);
     // a large matrix, read once, past the caches; the activation rows come from the L2 for each
     // workgroup again, which 64 matrix rows a workgroup halve (200000 x 2816: 4 rows 85 us and 89
