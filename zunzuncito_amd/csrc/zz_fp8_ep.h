@@ -159,6 +159,22 @@ static bool launch_async_ep(const ZzF8EpCall &c, const ZzF8Ep &a, hipStream_t st
 
 #include "zz_fp8_wide.h"
 
+// The form for m matrices of `per` rows each, O packed rows, nb blocks: zz_fp8_form's choice, but
+// for many experts of few rows. How the rows are spread is not known here, and a router's choice is
+// skewed: some experts have many times the average, and with tiles of 32 rows their matrices are
+// read that many times, while tiles that are nearly empty cost little (their rows are one, read
+// from the caches). Over a Zipf spread with 128 experts of 1408 x 2816 (gated, bf16): 1024 pairs
+// in 64 x 64 tiles 17 us and in 32 x 32 31 (64 x 32: 33), 4096 pairs in 128 x 64 29 and in 64 x 32 85;
+// 2816 x 704 in f32: 1024 pairs in 64 x 128 16 and 29, 4096 34 and 78. Up to 4 rows an expert the
+// few-row form stays the best: 128 pairs 11.9 us (64 x 32 14.8), 512 19. With fewer than 2048
+// workgroups of it there are too few tiles: 1136 pairs of 47 experts, 1044 x 1664 in f32, 13.8 and
+// 16.1. Over 60 cases from perf/more_operators.py's ranges this lies 6 % behind the best form of each.
+static int ep_form(int O, int per, int m, int nb, bool bf16) {
+    if (m > 1 && per <= 32 && (int64_t)m * ((O + 31) / 32) > 2048)
+        return per <= 4 ? 1 : !bf16 ? 7 : per < 12 ? 11 : 12;
+    return zz_fp8_form(O, per, m, nb, bf16 ? ZZ_F8_FORMS_BF16 : ZZ_F8_FORMS_F32);
+}
+
 template <typename T, int G>
 static bool launch_ep(const ZzF8EpCall &c, hipStream_t st) {
     ZzF8Ep a;
@@ -167,13 +183,16 @@ static bool launch_ep(const ZzF8EpCall &c, hipStream_t st) {
     a.offs = c.offs; a.E = c.E; a.P = c.P; a.we = c.we; a.wse = c.wse; a.wsu = c.wsu;
     // large results past the caches where tiles write whole lines, as zz_fp8_mma.hip's
     a.nt = c.P * a.ldy * (int64_t)sizeof(T) >= ZZ_NT_BYTES && (uintptr_t)a.y % 64 == 0 && a.ldy * sizeof(T) % 64 == 0;
-    // the rows of an expert, were they spread evenly
+    // the experts that can have rows, and each one's rows, were they spread evenly
     const int m = c.offs ? (c.E < c.P ? c.E : c.P) : 1, per = (c.P + m - 1) / m;
     const int O = G * c.m.O;                              // packed rows
-    const int v = zz_fp8_form(O, per, m, a.nb, sizeof(T) == 2 ? ZZ_F8_FORMS_BF16 : ZZ_F8_FORMS_F32);
+    const int v = ep_form(O, per, m, a.nb, sizeof(T) == 2);
+    // matrices past the caches are read past them too, as zz_fp8_mma.hip's; several of them by four
+    // waves a workgroup (128 pairs of 128 experts, 1408 x 2816: 11.9 us, by eight 17.5)
     const bool nt = per <= 32 && (int64_t)m * O * c.m.I >= ZZ_NT_BYTES;
     bool ok = false;
     if (v == 0) ok = launch_few_ep<T, G, 1, 1, 16, false, false>(c, a, st);
+    else if (v == 1 && nt && m > 1) ok = launch_few_ep<T, G, 1, 1, 4, true, true>(c, a, st);
     else if (v == 1 && nt && per <= 8) ok = launch_few_ep<T, G, 1, 1, 8, true, true>(c, a, st);
     else if (v == 1 && nt) ok = launch_few_ep<T, G, 2, 1, 4, true, true>(c, a, st);
     else if (v == 1) ok = launch_few_ep<T, G, 1, 1, 4, true, false>(c, a, st);
