@@ -31,6 +31,10 @@ struct XpArgs {
     int bytes;                      // of a row
 };
 
+// A row's last unit, where its width leaves a rest, ends where the row ends and begins inside the
+// unit before: vector loads all the same (element by element, a few lanes held their waves up: the
+// way back of 8192 x 4 rows of 1087 bf16 took XXX us and takes YYY).
+//
 // `bytes` (a multiple of 2) of 16 bytes at any address
 __device__ __forceinline__ zz_u4 xp_load(const uint8_t *p, int bytes) {
     if (bytes >= 16) return *(const zz_u4any *)p;
@@ -93,9 +97,10 @@ __global__ __launch_bounds__(256) void zz_xp_few_kernel(XpArgs a) {
         if (w == 0) xp_offsets(hist, a.E, [&](int e, int v) { a.offs[e] = v; });
         return;
     }
+    const int ids = l < a.K ? a.eidx[s * a.K + l] : -1;   // the token's own
     int mine = 0;
     for (int k = 0; k < a.K; k++) {
-        const int e = a.eidx[s * a.K + k], at = s * a.K + k;
+        const int e = __builtin_amdgcn_readlane(ids, k), at = s * a.K + k;
         int c = 0;
 #pragma unroll
         for (int i = 0; i < XP_FEW / 256; i++)
@@ -105,14 +110,14 @@ __global__ __launch_bounds__(256) void zz_xp_few_kernel(XpArgs a) {
     if (l < a.K) part[w][l] = mine;
     __syncthreads();
     if (tid < a.K) {
-        const int e = a.eidx[s * a.K + tid];
-        const int p = (unsigned)e < (unsigned)a.E ? part[0][tid] + part[1][tid] + part[2][tid] + part[3][tid] : -1;
+        const int p = (unsigned)ids < (unsigned)a.E ? part[0][tid] + part[1][tid] + part[2][tid] + part[3][tid] : -1;
         a.pos[s * a.K + tid] = where[tid] = p;
         if (p >= 0) a.row[p] = s;
     }
     if (!a.x) return;
     __syncthreads();
-    for (int b = 16 * tid; b < a.bytes; b += 4096) {
+    for (int u = 16 * tid; u < a.bytes; u += 4096) {
+        const int b = max(min(u, a.bytes - 16), 0);
         const zz_u4 v = xp_load(a.x + s * a.ldx + b, a.bytes - b);
         for (int k = 0; k < a.K; k++)
             if (where[k] >= 0) xp_store<false>(a.xs + where[k] * a.ldxs + b, v, a.bytes - b);
@@ -135,23 +140,35 @@ __global__ __launch_bounds__(1024) void zz_xp_count_kernel(XpArgs a) {
 
 // The positions of a chunk's pairs. Each of 16 waves has a run of them: how many of an expert lie
 // in the waves before is added up in LDS; within a wave's 64 pairs, the lanes with the same expert
-// are found by a ballot for each bit of the id. Nothing depends on the order of atomics.
+// are found by a ballot for each bit of the id. Nothing depends on the order of atomics. A wave's
+// pairs are requested 256 at a time, and the first 256 kept for the second pass.
 template <bool ONE>
 __global__ __launch_bounds__(1024) void zz_xp_place_kernel(XpArgs a) {
     __shared__ int wcnt[16][ZZ_EXPERTS_MAXE], total[ZZ_EXPERTS_MAXE], pre[ZZ_EXPERTS_MAXE], base[ZZ_EXPERTS_MAXE + 1];
     const int tid = threadIdx.x, w = zz_wave_id(), l = tid & 63, E = a.E;
     const int per = a.chunk / 16, first = blockIdx.x * a.chunk + w * per, end = min(a.n, first + per);
-    for (int i = tid; i < 16 * ZZ_EXPERTS_MAXE; i += 1024) (&wcnt[0][0])[i] = 0;
+    int id[4];
+    auto take = [&](int from) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) id[i] = from + 64 * i + l < end ? a.eidx[from + 64 * i + l] : -1;
+    };
+    take(first);
     for (int e = tid; e < E; e += 1024) total[e] = pre[e] = 0;
+#pragma unroll
+    for (int i = 0; i < 16; i++)
+        if (tid < E) wcnt[i][tid] = 0;
     __syncthreads();
-    for (int i = first + l; i < end; i += 64) {
-        const int e = a.eidx[i];
-        if ((unsigned)e < (unsigned)E) atomicAdd(&wcnt[w][e], 1);
+    for (int i0 = first; i0 < end; i0 += 256) {
+        if (i0 != first) take(i0);
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if ((unsigned)id[i] < (unsigned)E) atomicAdd(&wcnt[w][id[i]], 1);
     }
     if constexpr (!ONE) {                                 // the other chunks' pairs
         const int lanes = (E + 63) & ~63, groups = 1024 / lanes, e = tid % lanes, g = tid / lanes;
         if (e < E && g < groups) {
             int all = 0, before = 0;
+#pragma unroll 4
             for (int c = g; c < a.chunks; c += groups) {
                 const int v = a.count[c * E + e];
                 all += v;
@@ -180,25 +197,30 @@ __global__ __launch_bounds__(1024) void zz_xp_place_kernel(XpArgs a) {
         });
     __syncthreads();
     const int bits = 32 - __builtin_clz(E);               // of an id, 0 .. E - 1
-    for (int i0 = first; i0 < end; i0 += 64) {
-        const int i = i0 + l, e = i < end ? a.eidx[i] : -1;
-        const bool ok = (unsigned)e < (unsigned)E;
-        unsigned long long same = __ballot(ok);
-        for (int b = 0; b < bits; b++) {
-            const unsigned long long m = __ballot(e >> b & 1);
-            same &= e >> b & 1 ? m : ~m;
+    if (per > 256) take(first);
+    for (int i0 = first; i0 < end; i0 += 256) {
+        if (i0 != first) take(i0);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int at = i0 + 64 * i + l, e = id[i];
+            const bool ok = (unsigned)e < (unsigned)E;
+            unsigned long long same = __ballot(ok);
+            for (int b = 0; b < bits; b++) {
+                const unsigned long long m = __ballot(e >> b & 1);
+                same &= e >> b & 1 ? m : ~m;
+            }
+            const int rank = __builtin_popcountll(same & ((1ull << l) - 1));
+            int p = -1;
+            if (ok) {
+                const int before = wcnt[w][e];
+                p = base[e] + (ONE ? 0 : pre[e]) + before + rank;
+                asm volatile("" ::: "memory");            // all have read it
+                if (rank == 0) wcnt[w][e] = before + __builtin_popcountll(same);
+                a.row[p] = at / a.K;
+            }
+            asm volatile("" ::: "memory");
+            if (at < end) a.pos[at] = p;
         }
-        const int rank = __builtin_popcountll(same & ((1ull << l) - 1));
-        int p = -1;
-        if (ok) {
-            const int before = wcnt[w][e];
-            p = base[e] + (ONE ? 0 : pre[e]) + before + rank;
-            asm volatile("" ::: "memory");                // all have read it
-            if (rank == 0) wcnt[w][e] = before + __builtin_popcountll(same);
-            a.row[p] = i / a.K;
-        }
-        asm volatile("" ::: "memory");
-        if (i < end) a.pos[i] = p;
     }
 }
 
@@ -207,9 +229,10 @@ template <bool NT>
 __global__ __launch_bounds__(256) void zz_xp_rows_kernel(XpArgs a) {
     const int units = (a.bytes + 15) / 16;
     const unsigned id = blockIdx.x * 256u + threadIdx.x;
-    const int s = id / units, b = 16 * (id - s * units);
+    const int s = id / units, b = max(min(16 * (int)(id - s * units), a.bytes - 16), 0);
     if (s >= a.S) return;
     const zz_u4 v = xp_load(a.x + s * a.ldx + b, a.bytes - b);
+#pragma unroll 8
     for (int k = 0; k < a.K; k++) {
         const int p = a.pos[s * a.K + k];
         if (p >= 0) xp_store<NT>(a.xs + p * a.ldxs + b, v, a.bytes - b);
@@ -232,59 +255,168 @@ __device__ __forceinline__ int xp_pos(const XpBack &a, int i) {
     return (unsigned)p < (unsigned)a.n ? p : -1;
 }
 
+// 8 elements as they lie in memory, and as f32
+template <typename T> struct XpRaw { zz_u4 w[sizeof(T) / 2]; };
+template <typename T>
+__device__ __forceinline__ XpRaw<T> xp_raw(const T *p) {
+    XpRaw<T> r;
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; i++) r.w[i] = *((const zz_u4any *)p + i);
+    return r;
+}
+template <typename T>
+__device__ __forceinline__ float xp_of(const XpRaw<T> &r, int j) {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(r.w[j >> 2][j & 3]);
+    else return __uint_as_float(j & 1 ? r.w[0][j >> 1] & 0xffff0000u : r.w[0][j >> 1] << 16);
+}
+// a lane's unit of a row: 8 elements from e, of which the first `skip` are another lane's
+struct XpUnit { int e, skip; };
+__device__ __forceinline__ XpUnit xp_unit(int u, int D) {
+    const int e = min(8 * u, D - 8);
+    return {e, 8 * u - e};
+}
+template <bool NT, typename T>
+__device__ __forceinline__ void xp_put(T *p, const float (&v)[8], int skip) {
+    if (!skip) {
+        zz_put8<NT>(p, v, 8);
+        return;
+    }
+#pragma unroll
+    for (int j = 1; j < 8; j++)
+        if (j >= skip) zz_put(p + j, v[j]);
+}
+
+// Rows of fewer than 8 elements: a lane per element.
+template <typename T>
+__global__ __launch_bounds__(256) void zz_xp_back_narrow_kernel(XpBack a) {
+    const unsigned id = blockIdx.x * 256u + threadIdx.x;
+    const int s = id / a.D, e = id - s * a.D;
+    if (s >= a.S) return;
+    float v = a.res ? zz_f32_of(((const T *)a.res)[s * a.ldr + e]) : 0.0f;
+    for (int k = 0; k < a.K; k++) {
+        const int p = xp_pos(a, s * a.K + k);
+        if (p >= 0) v = fmaf(a.w ? a.w[s * a.K + k] : 1.0f, zz_f32_of(((const T *)a.y)[p * a.ldy + e]), v);
+    }
+    zz_put((T *)a.out + s * a.ldo + e, v);
+}
+
+// 8 rows are on their way at once.
 template <typename T, bool NT>
 __global__ __launch_bounds__(256) void zz_xp_back_kernel(XpBack a) {
     const int units = (a.D + 7) / 8;
     const unsigned id = blockIdx.x * 256u + threadIdx.x;
-    const int s = id / units, e = 8 * (id - s * units), n = a.D - e;
+    const int s = id / units;
     if (s >= a.S) return;
+    const XpUnit u = xp_unit(id - s * units, a.D);
     float v[8];
     if (a.res) {
-        zz_get8(v, (const T *)a.res + s * a.ldr + e, n, false);
+        const XpRaw<T> r = xp_raw((const T *)a.res + s * a.ldr + u.e);
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = xp_of(r, j);
     } else {
 #pragma unroll
         for (int j = 0; j < 8; j++) v[j] = 0.0f;
     }
-    for (int k = 0; k < a.K; k++) {
-        const int p = xp_pos(a, s * a.K + k);
-        if (p < 0) continue;
-        const float w = a.w ? a.w[s * a.K + k] : 1.0f;
-        float t[8];
-        zz_get8(t, (const T *)a.y + p * a.ldy + e, n, false);
+    for (int k0 = 0; k0 < a.K; k0 += 8) {
+        int p[8];
+        float w[8];
+        XpRaw<T> r[8];
 #pragma unroll
-        for (int j = 0; j < 8; j++) v[j] = fmaf(w, t[j], v[j]);
+        for (int k = 0; k < 8; k++) p[k] = k0 + k < a.K ? xp_pos(a, s * a.K + k0 + k) : -1;
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+            if (p[k] >= 0) {
+                r[k] = xp_raw((const T *)a.y + p[k] * a.ldy + u.e);
+                w[k] = a.w ? a.w[s * a.K + k0 + k] : 1.0f;
+            }
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+            if (p[k] >= 0)
+#pragma unroll
+                for (int j = 0; j < 8; j++) v[j] = fmaf(w[k], xp_of(r[k], j), v[j]);
     }
-    zz_put8<NT>((T *)a.out + s * a.ldo + e, v, n);
+    xp_put<NT>((T *)a.out + s * a.ldo + u.e, v, u.skip);
 }
 
-// A workgroup per token: its lanes keep 8 elements of dout and go through the K rows.
-template <typename T, bool NT>
+// TPR lanes per token (a row of at most 8 TPR elements, or 256): they keep 8 elements of dout and go
+// through the token's rows, 4 of them on their way at once; a row's sum is joined over the lanes.
+template <typename T, int TPR, bool NT>
 __global__ __launch_bounds__(256) void zz_xp_grad_kernel(XpBack a) {
     __shared__ float part[4][ZZ_EXPERTS_MAXK];
-    const int tid = threadIdx.x, w = zz_wave_id(), l = tid & 63, s = blockIdx.x;
-    for (int k = 0; k < a.K; k++) {
-        const int p = xp_pos(a, s * a.K + k);
-        float dot = 0.0f;
-        if (p >= 0) {
-            const float wt = a.w ? a.w[s * a.K + k] : 1.0f;
-            for (int e = 8 * tid; e < a.D; e += 2048) {
-                float g[8], t[8];
-                zz_get8(g, (const T *)a.dout + s * a.ldg + e, a.D - e, false);
-                if (a.dw) {
-                    zz_get8(t, (const T *)a.y + p * a.ldy + e, a.D - e, false);
+    const int tid = threadIdx.x % TPR, units = (a.D + 7) / 8, l = threadIdx.x & 63;
+    const int s = TPR == 256 ? blockIdx.x : blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
+    const bool here = s < a.S;
+    for (int k0 = 0; k0 < a.K; k0 += 4) {
+        int p[4];
+        float w[4], dot[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                    for (int j = 0; j < 8; j++) dot = fmaf(g[j], t[j], dot);
+        for (int k = 0; k < 4; k++) {
+            p[k] = here && k0 + k < a.K ? xp_pos(a, s * a.K + k0 + k) : -1;
+            w[k] = p[k] >= 0 && a.w ? a.w[s * a.K + k0 + k] : 1.0f;
+        }
+        if (a.D >= 8) {
+            for (int q = tid; q < units && here; q += TPR) {
+                const XpUnit u = xp_unit(q, a.D);
+                const XpRaw<T> g = xp_raw((const T *)a.dout + s * a.ldg + u.e);
+                XpRaw<T> y[4];
+                if (a.dw)
+#pragma unroll
+                    for (int k = 0; k < 4; k++)
+                        if (p[k] >= 0) y[k] = xp_raw((const T *)a.y + p[k] * a.ldy + u.e);
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+                    if (p[k] >= 0) {
+                        float t[8];
+#pragma unroll
+                        for (int j = 0; j < 8; j++) {
+                            if (a.dw && j >= u.skip) dot[k] = fmaf(xp_of(g, j), xp_of(y[k], j), dot[k]);
+                            t[j] = w[k] * xp_of(g, j);
+                        }
+                        xp_put<NT>((T *)a.dy + p[k] * a.lddy + u.e, t, u.skip);
+                    }
+            }
+        } else if (tid < a.D && here) {
+            const float g = zz_f32_of(((const T *)a.dout)[s * a.ldg + tid]);
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                if (p[k] >= 0) {
+                    if (a.dw) dot[k] = g * zz_f32_of(((const T *)a.y)[p[k] * a.ldy + tid]);
+                    zz_put((T *)a.dy + p[k] * a.lddy + tid, w[k] * g);
                 }
+        }
 #pragma unroll
-                for (int j = 0; j < 8; j++) t[j] = wt * g[j];
-                zz_put8<NT>((T *)a.dy + p * a.lddy + e, t, a.D - e);
+        for (int k = 0; k < 4; k++) {
+            dot[k] = zz_group_sum<TPR < 64 ? TPR : 64>(dot[k]);
+            if (k0 + k >= a.K) continue;
+            if constexpr (TPR == 256) {
+                if (l == 0) part[zz_wave_id()][k0 + k] = dot[k];
+            } else if (tid == 0 && here && a.dw) {
+                a.dw[s * a.K + k0 + k] = dot[k];
             }
         }
-        dot = zz_wave_sum(dot);
-        if (l == 0) part[w][k] = dot;
     }
-    __syncthreads();
-    if (a.dw && tid < a.K) a.dw[s * a.K + tid] = (part[0][tid] + part[1][tid]) + (part[2][tid] + part[3][tid]);
+    if constexpr (TPR == 256) {
+        __syncthreads();
+        if (a.dw && tid < a.K) a.dw[s * a.K + tid] = (part[0][tid] + part[1][tid]) + (part[2][tid] + part[3][tid]);
+    }
+}
+
+template <typename T>
+static void xp_launch_back(const XpBack &a, bool nt, hipStream_t st) {
+    const int64_t t = (int64_t)a.S * (a.D < 8 ? a.D : (a.D + 7) / 8);
+    const auto k = a.D < 8 ? zz_xp_back_narrow_kernel<T> : nt ? zz_xp_back_kernel<T, true> : zz_xp_back_kernel<T, false>;
+    hipLaunchKernelGGL(k, dim3((unsigned)((t + 255) / 256)), dim3(256), 0, st, a);
+}
+template <typename T, int TPR>
+static void xp_launch_grad(const XpBack &a, bool nt, hipStream_t st) {
+    const auto k = nt ? zz_xp_grad_kernel<T, TPR, true> : zz_xp_grad_kernel<T, TPR, false>;
+    hipLaunchKernelGGL(k, dim3((a.S + 256 / TPR - 1) / (256 / TPR)), dim3(256), 0, st, a);
+}
+template <typename T>
+static void xp_launch_grad(const XpBack &a, bool nt, hipStream_t st) {
+    if (a.D <= 128) xp_launch_grad<T, 16>(a, nt, st);
+    else if (a.D <= 1024) xp_launch_grad<T, 64>(a, nt, st);
+    else xp_launch_grad<T, 256>(a, nt, st);
 }
 
 // ------------------------------------------------------------------ host side
@@ -394,11 +526,8 @@ extern "C" int zz_experts_back_dev(int dtype, const void *d_y, int64_t ldy, cons
     XpBack a{};
     a.y = d_y; a.ldy = ldy; a.pos = d_pos; a.w = d_w; a.S = S; a.K = K; a.D = D; a.n = n; a.res = d_res; a.ldr = ldr;
     a.out = d_out; a.ldo = ldo;
-    const int64_t t = (int64_t)S * ((D + 7) / 8);
-    const bool nt = out.n >= ZZ_NT_BYTES;
-    const auto k = dtype == ZZ_F32 ? nt ? zz_xp_back_kernel<float, true> : zz_xp_back_kernel<float, false>
-                                   : nt ? zz_xp_back_kernel<zz_bf16, true> : zz_xp_back_kernel<zz_bf16, false>;
-    hipLaunchKernelGGL(k, dim3((unsigned)((t + 255) / 256)), dim3(256), 0, stream ? (hipStream_t)stream : zz_lib_stream(), a);
+    hipStream_t st = stream ? (hipStream_t)stream : zz_lib_stream();
+    dtype == ZZ_F32 ? xp_launch_back<float>(a, out.n >= ZZ_NT_BYTES, st) : xp_launch_back<zz_bf16>(a, out.n >= ZZ_NT_BYTES, st);
     if (hipGetLastError() != hipSuccess) ZZ_FAIL("%s: launch failed", who);
     return 1;
 }
@@ -424,10 +553,9 @@ extern "C" int zz_experts_back_grad_dev(int dtype, const void *d_dout, int64_t l
     XpBack a{};
     a.dout = d_dout; a.ldg = ldg; a.y = d_y; a.ldy = ldy; a.pos = d_pos; a.w = d_w; a.S = S; a.K = K; a.D = D; a.n = n;
     a.dy = d_dy; a.lddy = lddy; a.dw = d_dw;
+    hipStream_t st = stream ? (hipStream_t)stream : zz_lib_stream();
     const bool nt = out[0].n >= ZZ_NT_BYTES;
-    const auto k = dtype == ZZ_F32 ? nt ? zz_xp_grad_kernel<float, true> : zz_xp_grad_kernel<float, false>
-                                   : nt ? zz_xp_grad_kernel<zz_bf16, true> : zz_xp_grad_kernel<zz_bf16, false>;
-    hipLaunchKernelGGL(k, dim3(S), dim3(256), 0, stream ? (hipStream_t)stream : zz_lib_stream(), a);
+    dtype == ZZ_F32 ? xp_launch_grad<float>(a, nt, st) : xp_launch_grad<zz_bf16>(a, nt, st);
     if (hipGetLastError() != hipSuccess) ZZ_FAIL("%s: launch failed", who);
     return 1;
 }
