@@ -55,7 +55,8 @@ int zz_experts_back_dev(int dtype, const void *d_y, int64_t ldy, const int *d_po
 /* The way back's gradient, dout [S, D] being that of out (and of res):
  *   dy[pos[s][j]] = w[s][j] * dout[s]            rounded once to `dtype`
  *   dw[s][j]      = sum_d dout[s][d] * y[pos[s][j]][d]     f32, 0 for a pair without a position
- * The sum over d is made of f32 sums of up to 8 * ceil(D / 2048) products each, joined in pairs.
+ * The sum over d is made of f32 sums of up to max(16, 8 ceil(D / 2048)) products each, joined in
+ * pairs.
  * Rows of dy that pos does not name are left as they were; pos names a row once at most. dw
  * (NULL: not formed, y then unread and may be NULL); w NULL: ones. dout [S, D] rows ldg apart,
  * dy rows lddy. dy may be y itself, rows as far apart; outputs overlap nothing else. */

@@ -56,9 +56,9 @@ def grad(dout, y, pos, w):
 
 
 def dw_bound(mag, D):
-    """A lane's chain of 8 products for each 2048 columns, the wave's six and the waves' two
-    joining additions."""
-    return (8 * -(-D // 2048) + 9) * U * mag
+    """A lane's chain of up to 16 products, from 1025 columns on of 8 for each 2048, the wave's six
+    and the waves' two joining additions."""
+    return (max(16, 8 * -(-D // 2048)) + 9) * U * mag
 
 
 def activated(v, act):
