@@ -317,6 +317,33 @@ def test_gradients_against_differences():
         assert abs(float(diff) - float(dx[s, d])) <= (K + 1) * X.U * float(mag) + 1e-12
 
 
+@pytest.mark.parametrize("dtype, S, D", [(F32, 3000, 8192), (BF16, 9001, 4099)])
+def test_way_past_the_caches(dtype, S, D):
+    """Rows of 64 MiB and more, which are stored past the caches: copies, a sum of two rows and the
+    gradient, whose values are exact or of one rounding."""
+    K = 2
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn(S, D, generator=g, device="cuda").to(dtype)
+    ids = torch.randint(0, 40, (S, K), generator=g, device="cuda", dtype=torch.int32)
+    n = S * K
+    offs, row, pos = (torch.empty(k, dtype=torch.int32, device="cuda") for k in (41, n, n))
+    ws = torch.empty(zz.experts_ws_bytes(S, K, 40), dtype=torch.uint8, device="cuda")
+    xs = torch.full((n + 1, D), 7.0, dtype=dtype, device="cuda")
+    zz.experts_dispatch_dev(ptr(ids), S, K, 40, ptr(offs), ptr(row), ptr(pos), ptr(ws), ws.numel(), d_x=ptr(x), D=D, d_xs=ptr(xs),
+                            dtype=KIND[dtype], stream=stream())
+    assert torch.equal(xs[:n], x[row.long()]) and (xs[n] == 7.0).all()
+    out = torch.full((S + 1, D), 7.0, dtype=dtype, device="cuda")
+    zz.experts_back_dev(ptr(xs), ptr(pos), 0, S, K, D, ptr(out), d_res=ptr(x), dtype=KIND[dtype], stream=stream())
+    assert torch.equal(out[:S], (x.float() + x.float() + x.float()).to(dtype)) and (out[S] == 7.0).all()
+    w = torch.rand(S, K, generator=g, device="cuda")
+    dy = torch.full((n + 1, D), 7.0, dtype=dtype, device="cuda")
+    zz.experts_back_grad_dev(ptr(x), 0, ptr(pos), ptr(w), S, K, D, ptr(dy), 0, dtype=KIND[dtype], stream=stream())
+    p = pos.view(S, K).long()
+    for j in range(K):
+        assert torch.equal(dy[p[:, j]], (w[:, j:j + 1] * x.float()).to(dtype))
+    assert (dy[n] == 7.0).all()
+
+
 # ------------------------------------------------------------------ products
 def codes(shape, seed, small=False):
     """e4m3 codes without NaN; small: of magnitude up to 2, so that sums reach the activations' bend."""
@@ -353,15 +380,18 @@ class Case:
                     self.mat.upload(e, self.wq[e, p].numpy(), self.ws[e, p].numpy(), part=p)
         self.q, self.s, self.b = self.xq.cuda(), self.xs.cuda(), self.bias.cuda() if bias else None
 
-    def want(self, e, at, out, act, clamp, bias=True, res=True):
-        """(y, bound) of expert e's product of the rows `at`, which are rows `out` of y"""
+    def want(self, e, at, out, act, clamp, bias=True, res=True, cols=None):
+        """(y, bound) of expert e's product of the rows `at`, which are rows `out` of y; cols: of whole
+        blocks of 128 columns alone, a slice"""
+        cols = cols or slice(0, self.O)
+        n, blocks = cols.stop - cols.start, slice(cols.start // 128, R.blocks(cols.stop))
         xq, xs = self.xq[at].numpy(), self.xs[:, at].numpy()
-        sums, mags = zip(*(R.product(xq, xs, self.wq[e, p].numpy(), self.ws[e, p].numpy(), self.O, self.I) for p in range(self.G)))
-        b = self.bias[e].numpy() if bias and self.bias is not None else None
-        r = self.res.float().cpu()[out].numpy() if res and self.res is not None else None
-        cut = [0.0, 0.0]                         # results in bf16 may come from the 8-bit instructions
-        if self.dtype == BF16:
-            cut = [X.eights(xq, xs, self.wq[e, p].numpy(), self.ws[e, p].numpy(), self.O, self.I) for p in range(self.G)]
+        w = [(xq, xs, self.wq[e, p, cols].numpy(), self.ws[e, p, blocks].numpy(), n, self.I) for p in range(self.G)]
+        sums, mags = zip(*(R.product(*a) for a in w))
+        b = self.bias[e][:, cols].numpy() if bias and self.bias is not None else None
+        r = self.res[out.cuda()][:, cols].float().cpu().numpy() if res and self.res is not None else None
+        # results in bf16 may come from the 8-bit instructions
+        cut = [X.eights(*a) for a in w] if self.dtype == BF16 else [0.0, 0.0]
         return X.epilogue(sums, mags, self.I, b, act, clamp, r, R.HALF[self.dtype], cut)
 
 
@@ -400,6 +430,90 @@ def test_epilogue(S, O, I, gated):
                 assert torch.equal(y[:S], again[:S])
         finally:
             c.mat.close()
+
+
+def picked(n, k=12):
+    """The first rows, the last and some between."""
+    return torch.arange(n) if n <= 3 * k else torch.unique(torch.cat([torch.arange(k), torch.arange(n - k, n), torch.arange(k, n, n // k)]))
+
+
+# sizes that between them take every form that a product's rows, columns and type choose from, with
+# three blocks of columns at least, and matrices that are read past the caches
+@pytest.mark.parametrize("dtype, gated, S, O, I", [
+    (F32, False, 34, 4169, 576), (F32, False, 480, 4146, 385), (F32, False, 65, 5447, 796), (F32, False, 517, 1973, 257),
+    (F32, False, 361, 1352, 514), (F32, False, 1090, 3600, 257), (F32, False, 736, 4157, 259), (F32, True, 1, 4247, 529),
+    (F32, True, 137, 5631, 392), (F32, True, 37, 4162, 810), (F32, True, 33, 4284, 649), (F32, True, 37, 4234, 526),
+    (F32, True, 518, 3466, 260), (F32, True, 455, 3107, 263), (BF16, False, 1764, 1194, 263), (BF16, False, 1926, 1555, 259),
+    (BF16, False, 1239, 5017, 260), (BF16, False, 33, 4212, 533), (BF16, False, 326, 5533, 291), (BF16, False, 66, 5540, 813),
+    (BF16, False, 66, 5769, 561), (BF16, True, 265, 3817, 258), (BF16, True, 262, 5067, 257), (BF16, True, 641, 4548, 259),
+    (BF16, True, 145, 5608, 279), (BF16, True, 35, 4114, 808), (BF16, True, 35, 4220, 529), (F32, False, 3, 65600, 1088),
+    (F32, False, 20, 65600, 1088), (BF16, True, 3, 32800, 1088), (BF16, True, 20, 32800, 1088)])
+def test_epilogue_in_every_form(dtype, gated, S, O, I):
+    print("case", S, O, I, gated, dtype, flush=True)
+    c = Case(1, O, I, gated, S, S, S + O + I, dtype, size=0.3)
+    try:
+        act, clamp = (2, 0.8) if gated else (1, 0.0)
+        y = torch.full((S + 1, O), 9.0, dtype=dtype, device="cuda")
+        c.mat.matmul_ep_dev(ptr(c.q), ptr(c.s), S, ptr(y), d_bias=ptr(c.b), act=act, clamp=clamp, d_res=ptr(c.res),
+                            dtype=KIND[dtype], stream=stream())
+        at = picked(S)
+        for lo in (0, O // 256 * 128, O // 128 * 128):
+            cols = slice(lo, min(lo + 256, O))
+            near(y[at.cuda()][:, cols], *c.want(0, at, at, act, clamp, cols=cols))
+        assert (y[S] == 9.0).all()
+    finally:
+        c.mat.close()
+
+
+# as above, for tables of experts and a skewed spread of the rows
+@pytest.mark.parametrize("dtype, gated, E, P, O, I", [
+    (F32, False, 53, 55, 1802, 713), (F32, False, 137, 195, 34, 609), (F32, False, 51, 3492, 143, 667), (F32, False, 38, 1235, 213, 770),
+    (F32, False, 26, 851, 291, 586), (F32, False, 428, 1965, 139, 280), (F32, False, 6, 395, 4274, 263), (F32, True, 17, 17, 2646, 752),
+    (F32, True, 44, 3190, 72, 606), (F32, True, 8, 36, 4324, 267), (F32, True, 38, 2504, 321, 317), (BF16, False, 222, 242, 462, 657),
+    (BF16, False, 302, 1300, 213, 259), (BF16, False, 344, 3885, 180, 314), (BF16, False, 31, 2019, 1774, 267),
+    (BF16, False, 68, 2274, 100, 555), (BF16, True, 11, 11, 3736, 828), (BF16, True, 13, 55, 2628, 266),
+    (BF16, True, 259, 3277, 116, 376), (BF16, True, 45, 3158, 518, 292), (BF16, True, 5, 323, 1655, 258)])
+def test_experts_in_every_form(dtype, gated, E, P, O, I):
+    print("case", E, P, O, I, gated, dtype, flush=True)
+    n = max(1, P // 2)
+    c = Case(E, O, I, gated, n, P, E + P, dtype, size=0.4)
+    try:
+        offs = spread(P, E, "skew", E + P)
+        at = torch.randint(0, n, (P,), generator=torch.Generator().manual_seed(P))
+        row, D = at.int().cuda(), offs.cuda()
+        act, clamp = (1, 0.0) if gated else (2, 0.0)
+        y = torch.full((P + 1, O), 9.0, dtype=dtype, device="cuda")
+        c.mat.matmul_dev(ptr(c.q), ptr(c.s), n, ptr(row), ptr(D), P, ptr(y), d_bias=ptr(c.b), act=act, d_res=ptr(c.res),
+                         dtype=KIND[dtype], stream=stream())
+        o = offs.tolist()
+        some = [e for e in range(E) if o[e] < o[e + 1]]
+        for e in some[:3] + some[-3:] + some[3:-3:max(1, len(some) // 12)]:
+            out = o[e] + picked(o[e + 1] - o[e])
+            lo = max(0, (O - 1) // 128 * 128 - 128) if e % 2 else 0
+            cols = slice(lo, min(lo + 256, O))
+            near(y[out.cuda()][:, cols], *c.want(e, at[out], out, act, clamp, cols=cols))
+        assert (y[o[E]:] == 9.0).all()
+    finally:
+        c.mat.close()
+
+
+@pytest.mark.parametrize("dtype, gated, S, O, I", [(F32, False, 4100, 4224, 130), (F32, True, 4100, 4224, 130),
+                                                   (BF16, False, 8300, 4224, 130), (BF16, True, 8300, 4224, 130)])
+def test_epilogue_large_result(dtype, gated, S, O, I):
+    """Results of 64 MiB and more are stored past the caches where rows begin at whole lines, and
+    are what they are elsewhere."""
+    print("case", S, O, I, gated, dtype, flush=True)
+    c = Case(1, O, I, gated, S, 1, 5, dtype, res=False)
+    try:
+        a = torch.full((S + 1, O), 9.0, dtype=dtype, device="cuda")
+        b = torch.full(((S + 1) * O + 1,), 9.0, dtype=dtype, device="cuda")[1:].view(S + 1, O)
+        for y in (a, b):
+            c.mat.matmul_ep_dev(ptr(c.q), ptr(c.s), S, y.data_ptr(), d_bias=ptr(c.b), act=1, dtype=KIND[dtype], stream=stream())
+        assert torch.equal(a, b) and (a[S] == 9.0).all()
+        at = picked(S)
+        near(a[at.cuda()][:, :256], *c.want(0, at, at, 1, 0.0, cols=slice(0, 256)))
+    finally:
+        c.mat.close()
 
 
 @pytest.mark.parametrize("gated", [False, True])
@@ -482,6 +596,33 @@ def test_epilogue_edges(gated):
                     near(y, *big.want(0, torch.arange(S), torch.arange(S), act, 3.0 if gated else 0.0))
             finally:
                 big.mat.close()
+        finally:
+            c.mat.close()
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("S, O, I", [(1764, 1194, 263), (1926, 1555, 259), (1239, 5017, 260), (517, 1973, 257)])
+def test_epilogue_edges_in_tiles(S, O, I, gated):
+    """The same in the tiles of larger products: a NaN code, bias or residual and an infinite scale
+    stay in their row or column."""
+    for dtype in (F32, BF16):
+        print("case", S, O, I, gated, dtype, flush=True)
+        c = Case(1, O, I, gated, S, S, 11, dtype)
+        try:
+            out = []
+            q, s, b, r = c.q.clone(), c.s.clone(), c.b.clone(), c.res.clone()
+            for k in range(2):
+                y = torch.empty(S, O, dtype=dtype, device="cuda")
+                c.mat.matmul_ep_dev(ptr(q), ptr(s), S, ptr(y), d_bias=ptr(b), act=2, clamp=0.5 if gated else 0.0, d_res=ptr(r),
+                                    dtype=KIND[dtype], stream=stream())
+                out.append(y)
+                q[70, 5], b[0, 0, 133], r[9, 40], s[0, S - 1] = 0xFF, NAN, NAN, INF
+            y, z = out
+            bad = torch.zeros(S, O, dtype=torch.bool, device="cuda")
+            bad[70], bad[:, 133], bad[9, 40] = True, True, True
+            assert z[bad].isnan().all()
+            bad[S - 1] = True
+            assert torch.equal(z[~bad], y[~bad]) and y.isfinite().all()
         finally:
             c.mat.close()
 

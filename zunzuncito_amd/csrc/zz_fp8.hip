@@ -188,15 +188,15 @@ extern "C" void zz_fp8_destroy(int id) {
     g_mats[id] = nullptr;
 }
 
-// one matrix of the table, from codes on the device and scales on either side
-static int upload_mat(Fp8Mat *m, int e, int part, const uint8_t *d_codes, const void *scales, hipMemcpyKind kind) {
+// one matrix of the table, from codes on the device and scales there (one launch) or on the host
+static int upload_mat(Fp8Mat *m, int e, int part, const uint8_t *d_codes, const float *scales, bool host) {
     hipStream_t st = zz_lib_stream();
     char &have = m->loaded[(size_t)e * m->parts + part];
     m->missing += have;
     have = 0;
     float *ws = m->ws + ((size_t)e * m->parts + part) * scale_count(m);
-    ZZ_CHECK(hipMemcpyAsync(ws, scales, 4 * scale_count(m), kind, st));
-    if (!zz_launch_fp8_pack(d_codes, m->O, m->I, m->parts == 2 ? part : -1, m->w + e * wbytes(m), st))
+    if (host) ZZ_CHECK(hipMemcpyAsync(ws, scales, 4 * scale_count(m), hipMemcpyHostToDevice, st));
+    if (!zz_launch_fp8_pack(d_codes, m->O, m->I, m->parts == 2 ? part : -1, m->w + e * wbytes(m), host ? nullptr : scales, ws, st))
         ZZ_FAIL("zz_fp8_upload: launch failed");
     ZZ_CHECK(hipStreamSynchronize(st));
     have = 1;
@@ -212,7 +212,7 @@ static int upload_host(const char *who, Fp8Mat *m, int e, int part, const uint8_
         ZZ_FAIL("%s: device allocation failed", who);
     }
     const int ok = hipMemcpy(d, codes, n, hipMemcpyHostToDevice) == hipSuccess &&
-                   upload_mat(m, e, part, d, scales, hipMemcpyHostToDevice);
+                   upload_mat(m, e, part, d, scales, true);
     (void)hipFree(d);
     if (!ok) ZZ_FAIL("%s: failed", who);
     return 1;
@@ -237,7 +237,7 @@ extern "C" int zz_fp8_upload_dev(int id, const uint8_t *d_codes, const float *d_
     if (!zz_lib_here("zz_fp8_upload_dev")) return 0;
     Fp8Mat *m = plain_mat(id);
     if (!m) ZZ_FAIL("zz_fp8_upload_dev: no such matrix");
-    return upload_mat(m, 0, 0, d_codes, d_scales, hipMemcpyDeviceToDevice);
+    return upload_mat(m, 0, 0, d_codes, d_scales, false);
 }
 
 static Fp8Mat *expert_mat(const char *who, int id, int e, int part) {
@@ -259,7 +259,7 @@ extern "C" int zz_fp8_upload_expert_dev(int id, int e, int part, const uint8_t *
     const char *who = "zz_fp8_upload_expert_dev";
     if (!d_codes || !d_scales || (uintptr_t)d_scales % 4) ZZ_FAIL("%s: bad arguments", who);
     Fp8Mat *m = expert_mat(who, id, e, part);
-    return m ? upload_mat(m, e, part, d_codes, d_scales, hipMemcpyDeviceToDevice) : 0;
+    return m ? upload_mat(m, e, part, d_codes, d_scales, false) : 0;
 }
 
 extern "C" int zz_fp8_matmul_dev(int id, const uint8_t *d_q, const float *d_s, int S, int dtype, void *d_y,

@@ -113,8 +113,8 @@ struct ZzF8Mat {
 __host__ __device__ __forceinline__ int zz_f8_nb(int n) { return (n + ZZ_F8B - 1) / ZZ_F8B; }
 
 // part: -1 a plain matrix; 0, 1 gate's or up's half of a gated pair, whose 32-row groups are 16
-// rows of each (zz_fp8_mma.h)
-int zz_launch_fp8_pack(const uint8_t *codes, int O, int I, int part, uint8_t *dst, hipStream_t st);
+// rows of each (zz_fp8_mma.h). scales (null: not copied) go to ws
+int zz_launch_fp8_pack(const uint8_t *codes, int O, int I, int part, uint8_t *dst, const float *scales, float *ws, hipStream_t st);
 int zz_launch_fp8_matmul(const ZzF8Mat &m, const uint8_t *q, const float *s, int S, int dtype, void *y,
                          int64_t ldy, hipStream_t st);
 

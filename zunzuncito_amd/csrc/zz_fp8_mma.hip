@@ -42,10 +42,12 @@ __global__ __launch_bounds__(256, 2) void zz_fp8_tiles_kernel(ZzF8Mm a, int whol
 }
 
 // one 16-byte piece of the packed layout per thread; part 0, 1: gate's, up's rows of a gated pair
-// (-1: a plain matrix), the other's left as they are
+// (-1: a plain matrix), the other's left as they are. The first threads copy the scales, of which
+// there are fewer than pieces.
 __global__ __launch_bounds__(256) void zz_fp8_pack_kernel(const uint8_t *src, int O, int I, int nb, uint8_t *dst,
-                                                          int64_t n, int part) {
+                                                          int64_t n, int part, const float *scales, float *ws, int ns) {
     const int64_t p = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (p < ns) ws[p] = scales[p];
     if (p >= n) return;
     const int l = (int)(p & 63), pc = (int)(p >> 6) & 3;
     const int64_t gb = p >> 8, g = gb / nb;
@@ -69,10 +71,11 @@ __global__ __launch_bounds__(256) void zz_fp8_pack_kernel(const uint8_t *src, in
     *(uint4 *)(dst + 16 * p) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-int zz_launch_fp8_pack(const uint8_t *codes, int O, int I, int part, uint8_t *dst, hipStream_t st) {
+int zz_launch_fp8_pack(const uint8_t *codes, int O, int I, int part, uint8_t *dst, const float *scales, float *ws, hipStream_t st) {
     const int nb = zz_f8_nb(I), gc = part < 0 ? 32 : 16;
     const int64_t n = (int64_t)((O + gc - 1) / gc) * nb * 256;
-    hipLaunchKernelGGL(zz_fp8_pack_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, codes, O, I, nb, dst, n, part);
+    hipLaunchKernelGGL(zz_fp8_pack_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, codes, O, I, nb, dst, n, part,
+                       scales, ws, scales ? zz_f8_nb(O) * nb : 0);
     return hipGetLastError() == hipSuccess;
 }
 
