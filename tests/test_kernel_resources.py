@@ -50,3 +50,12 @@ def test_rows_product_beam_in_registers(kernels):
     assert len([k for k in mine if k.startswith("zz_add_norm_fp8_kernel<")]) == 20
     assert len([k for k in mine if k.startswith("zz_beam_reorder_kernel<")]) == 6
     assert not [(k, v) for k, v in mine.items() if v[0]]
+
+
+def test_experts_in_registers(kernels):
+    """No scratch in the sort, the rows' ways and the gradient, nor in a product with an epilogue,
+    whose search for its expert indexes registers."""
+    mine = {k: v for k, v in kernels.items() if k.startswith(("zz_xp_", "zz_fp8_few_ep", "zz_fp8_tiles_ep", "zz_fp8_wide"))}
+    assert len([k for k in mine if k.startswith("zz_xp_grad_kernel<")]) == 12
+    assert len([k for k in mine if k.startswith("zz_fp8_wide_kernel<")]) == 6
+    assert not [(k, v) for k, v in mine.items() if v[0]]
