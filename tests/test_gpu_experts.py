@@ -686,6 +686,110 @@ def test_experts(E, P, O, I, gated, kind):
                 c.mat.close()
 
 
+@pytest.mark.parametrize("dtype, gated, E, P, O, I, ldy", [
+    (F32, False, 3, 20, 70, 300, 1 << 28), (BF16, True, 3, 20, 70, 300, 1 << 28), (F32, True, 2, 700, 130, 260, 1 << 23),
+    (BF16, False, 2, 700, 130, 260, 1 << 23), (F32, False, 2, 9000, 140, 130, 1 << 19), (BF16, True, 2, 9000, 140, 130, 1 << 19)])
+def test_experts_far_rows(dtype, gated, E, P, O, I, ldy):
+    """Rows of y whose elements pass 2^32, from few rows and in tiles."""
+    assert P * ldy > 1 << 32
+    c = Case(E, O, I, gated, P, P, 3, dtype, res=False)
+    y = torch.empty(P, ldy, dtype=dtype, device="cuda")
+    try:
+        offs = [0] + [P // 3] * (E - 1) + [P]
+        D = torch.tensor(offs, dtype=torch.int32).cuda()
+        y[-1].fill_(9.0)
+        for first in (True, False):              # then with itself as the residual
+            if not first:
+                y[:, :O] = torch.randn(P, O, generator=torch.Generator().manual_seed(8)).to(dtype).cuda()
+                c.res = y[:, :O].clone()
+            c.mat.matmul_dev(ptr(c.q), ptr(c.s), P, 0, ptr(D), P, ptr(y), d_bias=ptr(c.b), act=2, dtype=KIND[dtype], ldy=ldy,
+                             d_res=0 if first else ptr(y), ldr=ldy, stream=stream())
+            torch.cuda.synchronize()
+            for e in (0, E - 1):
+                at = torch.unique(torch.cat([torch.arange(offs[e], offs[e + 1])[k] for k in (slice(0, 3), slice(-4, None))]))
+                near(y[at.cuda(), :O], *c.want(e, at, at, 2, 0.0))
+            assert (y[-1, O:] == 9.0).all()
+    finally:
+        c.mat.close()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_experts_far_codes(dtype):
+    """Codes of the rows, and of the table, that pass 2^32 bytes; the last of them."""
+    I, O, E, P = 1 << 16, 33, 3, 70000
+    c = Case(E, O, I, False, 256, 256, 6, dtype, res=False)
+    q, s = c.q.repeat(P // 256 + 1, 1)[:P], c.s.repeat(1, P // 256 + 1)[:, :P].contiguous()
+    y = torch.empty(P, O, dtype=dtype, device="cuda")
+    try:
+        assert q.numel() > 1 << 32
+        offs = [0, 0, 100, P]
+        D = torch.tensor(offs, dtype=torch.int32).cuda()
+        c.mat.matmul_dev(ptr(q), ptr(s), P, 0, ptr(D), P, ptr(y), d_bias=ptr(c.b), act=1, dtype=KIND[dtype], stream=stream())
+        torch.cuda.synchronize()
+        for e, at in ((1, [0, 99]), (2, [100, 65535, 65536, P - 1])):
+            at = torch.tensor(at)
+            near(y[at.cuda()], *c.want(e, at % 256, at, 1, 0.0))
+    finally:
+        c.mat.close()
+    del q, s, y
+    O, E, P = 4096, 20, 45
+    c = Case(1, O, I, False, P, P, 6, dtype, res=False)
+    t = zz.Fp8Experts(E, O, I)
+    try:
+        zero, w, ws = torch.zeros(O, I, dtype=torch.uint8, device="cuda"), c.wq[0, 0].cuda(), c.ws[0, 0].cuda()
+        torch.cuda.synchronize()
+        for e in range(E):
+            t.upload_dev(e, ptr(w if e == E - 1 else zero), ptr(ws))
+        b = c.b.expand(E, 1, O).contiguous()
+        y = torch.empty(P, O, dtype=dtype, device="cuda")
+        for n in (2, P):                         # of the last expert; the others' are the bias alone
+            D = torch.tensor([0] * 5 + [P - n] * 15 + [P], dtype=torch.int32).cuda()
+            t.matmul_dev(ptr(c.q), ptr(c.s), P, 0, ptr(D), P, ptr(y), d_bias=ptr(b), dtype=KIND[dtype], stream=stream())
+            torch.cuda.synchronize()
+            at = torch.tensor([P - n, P - 1])
+            cols = slice(O - 128, O)
+            near(y[at.cuda(), cols], *c.want(0, at, at, 0, 0.0, cols=cols))
+            assert torch.equal(y[:P - n], c.b.view(O).to(dtype).expand(P - n, O))
+    finally:
+        c.mat.close()
+        t.close()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("gated", [False, True])
+def test_experts_most_rows(dtype, gated):
+    """2^24 rows of 512 experts, and 2^20 of one matrix: codes of 1 and scales of whole numbers, exact."""
+    E, P, O, I = 512, 1 << 24, 3, 5
+    t = zz.Fp8Experts(E, O, I, gated)
+    one = zz.Fp8Experts(1, O, I, gated)
+    try:
+        w = np.full((O, I), 0x38, np.uint8)
+        for e in range(E):
+            for p in range(2 if gated else 1):
+                t.upload(e, w, np.full((1, 1), 1.0 if p else e + 1.0, np.float32), part=p)
+                if e == 0:
+                    one.upload(0, w, np.ones((1, 1), np.float32), part=p)
+        q = torch.full((P, 128), 0x38, dtype=torch.uint8, device="cuda")
+        at = torch.arange(P, device="cuda")
+        s = (at % 7 + 1).float()
+        cut = torch.sort(torch.randint(0, P + 1, (E + 1,), generator=torch.Generator().manual_seed(3)))[0].int().cuda()
+        y = torch.full((P, O), 9.0, dtype=dtype, device="cuda")
+        e = torch.searchsorted(cut.long(), at, right=True) - 1
+        for row in (None, (P - 1 - at).int()):
+            t.matmul_dev(ptr(q), ptr(s), P, ptr(row), ptr(cut), P, ptr(y), dtype=KIND[dtype], stream=stream())
+            v = 5.0 * (s if row is None else s.flip(0))
+            want = ((e + 1) * v * (v if gated else 1.0)).to(dtype)
+            want = torch.where((e >= 0) & (e < E), want, 9.0)
+            assert torch.equal(y, want[:, None].expand(P, O))
+        S = 1 << 20
+        one.matmul_ep_dev(ptr(q), ptr(s), S, ptr(y), dtype=KIND[dtype], stream=stream())
+        v = 5.0 * s[:S]
+        assert torch.equal(y[:S], (v * (v if gated else 1.0)).to(dtype)[:, None].expand(S, O))
+    finally:
+        t.close()
+        one.close()
+
+
 def test_experts_rows_alone():
     """A row's result does not depend on how many rows other experts have, nor on where it lies."""
     E, P, O, I = 6, 400, 90, 300
