@@ -79,15 +79,16 @@ __device__ __forceinline__ void zz_fp8_wide(const ZzF8Ep &a, char *lds, int gt, 
     const bool by_row = a.row != nullptr;
     const uint8_t *xsrc = a.q + (by_row ? 0 : (size_t)t0 * nb * ZZ_F8B);
     const float *ssrc = a.s + (by_row ? 0 : t0);
-    auto at = [&](int t) {
-        const int in = min(t, last);
-        return (unsigned)(by_row ? zz_f8_row<G>(a, t0 + in) : in);
-    };
-    unsigned xo[C::XI];
+    ZzF8Scales wsl(wsp, nb), wul(wup, nb);
+    unsigned xo[C::XI + 1];
+#pragma unroll
+    for (int i = 0; i < C::XI; i++) xo[i] = min((w * C::XI + i) * 8 + (l >> 3), last);
+    xo[C::XI] = min(w * 64 + l, last);
+    zz_f8_rows<G>(a, t0, xo);
+    const unsigned so = 4 * xo[C::XI];
 #pragma unroll
     for (int i = 0; i < C::XI; i++)
-        xo[i] = at((w * C::XI + i) * 8 + (l >> 3)) * nb * ZZ_F8B + 16 * ((l & 7) ^ ((((w * C::XI + i) & 1) << 2) | (l >> 4)));
-    const unsigned so = 4 * at(w * 64 + l);
+        xo[i] = xo[i] * nb * ZZ_F8B + 16 * ((l & 7) ^ ((((w * C::XI + i) & 1) << 2) | (l >> 4)));
     auto fetch = [&](int b) {
         const unsigned d = lb + (b & 1) * C::STAGE;
 #pragma unroll
@@ -96,7 +97,6 @@ __device__ __forceinline__ void zz_fp8_wide(const ZzF8Ep &a, char *lds, int gt, 
         for (int i = 0; i < C::XI; i++) zz_dma16(xsrc + (size_t)b * ZZ_F8B, xo[i], d + C::WB + (w * C::XI + i) * 1024);
         if (w < C::SI) zz_dma4(ssrc + (size_t)b * a.R, so, d + C::WB + C::XB + w * 256);
     };
-    ZzF8Scales wsl(wsp, nb), wul(wup, nb);
     zz_v16f acc[RO], p[RO];
 #pragma unroll
     for (int i = 0; i < RO; i++) acc[i] = p[i] = zz_f8_zero();
@@ -106,6 +106,8 @@ __device__ __forceinline__ void zz_fp8_wide(const ZzF8Ep &a, char *lds, int gt, 
         for (int k = 0; k < 16; k++) acc[i][k] = fmaf(p[i][k], k < 8 ? sc : sc2, acc[i][k]);
     };
     fetch(0);
+    wsl.ready();
+    wul.ready();
     for (int b = 0; b < nb; b++) {
         // block b has arrived for this wave; behind the barrier, for all, and the one before it is read
         zz_wait_vm<0>();
