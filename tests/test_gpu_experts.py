@@ -465,6 +465,25 @@ def test_epilogue_in_every_form(dtype, gated, S, O, I):
         c.mat.close()
 
 
+# each tile's rounds, which go in threes and keep the scales of 64 blocks, at their ends
+@pytest.mark.parametrize("nb", [1, 2, 3, 4, 5, 65, 67])
+@pytest.mark.parametrize("gated, S, O", [(False, 2401, 1031), (False, 610, 4897), (False, 2182, 2691), (True, 641, 1930),
+                                         (True, 898, 1682), (True, 2182, 1346)])
+def test_epilogue_in_tiles_of_any_depth(gated, S, O, nb):
+    I = 128 * nb - 3
+    c = Case(1, O, I, gated, S, S, S + nb, BF16, size=0.3, res=False)
+    try:
+        y = torch.full((S + 1, O), 9.0, dtype=BF16, device="cuda")
+        c.mat.matmul_ep_dev(ptr(c.q), ptr(c.s), S, ptr(y), d_bias=ptr(c.b), act=2, dtype=KIND[BF16], stream=stream())
+        at = picked(S)
+        for lo in (0, O // 128 * 128):
+            cols = slice(lo, min(lo + 128, O))
+            near(y[at.cuda()][:, cols], *c.want(0, at, at, 2, 0.0, cols=cols))
+        assert (y[S] == 9.0).all()
+    finally:
+        c.mat.close()
+
+
 # as above, for tables of experts and a skewed spread of the rows
 @pytest.mark.parametrize("dtype, gated, E, P, O, I", [
     (F32, False, 53, 55, 1802, 713), (F32, False, 137, 195, 34, 609), (F32, False, 51, 3492, 143, 667), (F32, False, 38, 1235, 213, 770),

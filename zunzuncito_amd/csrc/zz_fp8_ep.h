@@ -203,9 +203,9 @@ static bool launch_ep(const ZzF8EpCall &c, hipStream_t st) {
     if (ok) return true;
     // the largest tiles also where smaller ones are more than a launch holds
     if constexpr (sizeof(T) == 2) {
-        if (v == 11 && launch_wide<G, 1, 2, 2, 4>(c, a, st)) return true;
-        if (v == 12 && launch_wide<G, 2, 2, 2, 3>(c, a, st)) return true;
-        return launch_wide<G, 2, 2, 4, 4>(c, a, st);
+        if (v == 11 && launch_wide<G, 2, 2, 2>(c, a, st)) return true;
+        if (v == 12 && launch_wide<G, 2, 4, 3>(c, a, st)) return true;
+        return launch_wide<G, 4, 4, 2>(c, a, st);
     } else {
         if (v == 6 && launch_async_ep<T, G, 1, 1, 2, 2, 1, 3, false>(c, a, st)) return true;
         if (v == 7 && launch_async_ep<T, G, 1, 2, 2, 2, 1, 2, true>(c, a, st)) return true;

@@ -140,9 +140,9 @@ static const ZzF8Form mm_forms[] = {
     {128, 128, 1, 2, {4.5f, 7.8f}, {1.04f, 1.59f}},
     {128, 128, 1, 2, {4.5f, 7.8f}, {1.04f, 1.59f}, 4, {1.6f, 0.03f, 0.13f}},
     // zz_fp8_wide.h's, from 512 and 2816 columns with one to `per` workgroups on each CU
-    {64, 64, 1, 4, {3.6f, 4.7f, 6.0f, 6.5f}, {0.46f, 0.49f, 0.53f, 0.73f}},
-    {128, 64, 1, 3, {5.1f, 6.5f, 7.9f}, {0.52f, 0.58f, 0.88f}},
-    {128, 128, 1, 2, {6.5f, 9.2f}, {0.63f, 0.94f}},
+    {64, 64, 1, 4, {4.6f, 5.6f, 6.5f, 6.9f}, {0.41f, 0.45f, 0.48f, 0.62f}},
+    {128, 64, 1, 3, {5.1f, 6.6f, 7.6f}, {0.46f, 0.58f, 0.81f}},
+    {128, 128, 1, 2, {7.8f, 9.2f}, {0.63f, 0.93f}},
 };
 int zz_fp8_form(int O, int S, int tables, int nb, int of) {
     int best = 0;

@@ -10,15 +10,20 @@
 // results, which would show it, and few rows, whose time is the matrix's bytes, keep
 // zz_fp8_mma.h's f16 products.
 //
-// Without the conversions and at twice the rate: 8192 x 2816 x 2112 64 us (1.52 PFLOP/s) where the
-// f16 tiles take 115; 2048 x 4224 x 2816 gated 39.5 for 71; 32768 rows of 128 experts, 1408 x 2816,
-// 160 for 263. What bounds them is the way of the codes into LDS: the last without it takes 126 us,
-// without the matrix instructions 157 (their clock is 1.9 GHz then; busy 39 %). Measured and not
-// better, 128 x 128 tiles at 160: 256 x 256, one workgroup a CU (166; 12 % faster where the tiles
-// come out even, 20 % slower where not), 64 x 64 a wave (170), operands of the next block read
-// ahead over the barrier (170), later lines touched for the L2 (199 and more).
+// Without the conversions and at twice the rate: 8192 x 2816 x 2112 65 us (1.50 PFLOP/s) where the
+// f16 tiles take 115; 2048 x 4224 x 2816 gated 36.4 for 71; 32768 rows of 128 experts, 1408 x 2816,
+// 153 for 263. What bounds them is the way of the codes to the matrix cores, which are 40 % busy at
+// 1.9 GHz: 32 KB a block for 128 x 128, and 128 bytes a cycle of LDS. So a wave keeps 32 packed
+// rows times all rows of the tile: its part of the matrix lies in operand order, no other wave wants
+// it, and it comes straight into registers, past LDS, which then holds more blocks. With the matrix
+// through LDS and waves of 64 x 32 the same three took 63.5, 37.6 and 153, but 128 experts of 256
+// rows each 224 for 197, 64 of 512 188 for 169, 64 rows each 125 for 120. Measured and not better,
+// 128 x 128 at 164: 256 x 256 (166) and 256 x 128 (184), 64 x 64 a wave (170), a third workgroup on a
+// CU (spills), the row operands' next block read over the barrier (170), later lines touched for the
+// L2 (199 and more), the XCDs' parts cut by the matrices they read (171: more workgroups without a tile).
 #pragma once
 #include "zz_fp8_mma.h"
+#include <type_traits>
 
 typedef int zz_i8 __attribute__((ext_vector_type(8)));
 __device__ __forceinline__ zz_i8 zz_f8_pair(const char *a, const char *b) {
@@ -44,37 +49,30 @@ __device__ __forceinline__ void zz_f8_store_bf16(zz_bf16 *p, const float (&v)[8]
         if (e < n) p[e].u = (uint16_t)(w[e / 2] >> (16 * (e & 1)));
 }
 
-// WO x WS waves of RO groups of 32 packed rows times 32 rows each
-template <int RO, int WO, int WS>
+// WO waves of 32 packed rows times 32 RS rows each
+template <int RS, int WO>
 struct ZzF8Wide {
-    static constexpr int GW = WO * WS, NT = 64 * GW, O = 32 * RO * WO, S = 32 * WS;
-    static constexpr int WB = O * 128, XB = S * 128, SI = (S + 63) / 64, STAGE = WB + XB + SI * 256;
+    static constexpr int NT = 64 * WO, O = 32 * WO, S = 32 * RS;
+    static constexpr int XB = S * 128, SI = (S + 63) / 64, STAGE = XB + SI * 256;
     static constexpr int LDS = 2 * STAGE > O * S * 4 ? 2 * STAGE : O * S * 4;    // two blocks, or the result
-    static constexpr int WI = O / 8 / GW, XI = S / 8 / GW;                       // a wave's requests a block
-    static_assert(O / 8 % GW == 0 && S / 8 % GW == 0 && SI <= GW, "whole requests a wave");
+    static constexpr int XI = S / 8 / WO;                                        // a wave's requests a block
+    static_assert(S / 8 % WO == 0 && SI <= WO, "whole requests a wave");
 };
 
-// One tile: the result's rows from t0, the matrix's groups from gt. Blocks arrive in LDS as in
-// zz_fp8_tile, one round ahead. A product's 16 results enter the sums while the next one runs, the
-// last one's of a block behind the next barrier (with one group a wave, its own).
-template <int G, int RO, int WO, int WS>
+// One tile: the result's rows from t0, the matrix's groups from gt. The rows' blocks arrive in LDS
+// as in zz_fp8_tile, one round ahead; the matrix's in registers, two rounds ahead. A product's 16
+// results enter the sums while the next one runs, the last one's of a block behind the next barrier.
+template <int G, int RS, int WO>
 __device__ __forceinline__ void zz_fp8_wide(const ZzF8Ep &a, char *lds, int gt, int t0) {
     constexpr int GC = zz_f8_gw<G>;
-    typedef ZzF8Wide<RO, WO, WS> C;
-    const int tid = threadIdx.x, l = tid & 63, r = l & 31, h = l >> 5, nb = a.nb;
-    const int w = zz_wave_id(), wo = w % WO, ws = w / WO;
-    const int g0 = gt + wo * RO, gl = (a.m.O + GC - 1) / GC - 1, last = a.S - 1 - t0;
-    const float *wsp = a.m.ws + (size_t)(min(g0, gl) / (128 / GC)) * nb, *wup = wsp;
+    typedef ZzF8Wide<RS, WO> C;
+    const int tid = threadIdx.x, l = tid & 63, r = l & 31, h = l >> 5, nb = a.nb, w = zz_wave_id();
+    const int gl = (a.m.O + GC - 1) / GC - 1, g0 = min(gt + w, gl), last = a.S - 1 - t0;
+    const float *wsp = a.m.ws + (size_t)(g0 / (128 / GC)) * nb, *wup = wsp;
     if constexpr (G == 2) wup += a.wsu;
     const unsigned lb = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
-    // this wave's requests: matrix pieces w*WI .. (4 a group), row octets w*XI .., the first waves'
-    // 64 scales
-    const uint8_t *wsrc[C::WI];
-#pragma unroll
-    for (int i = 0; i < C::WI; i++) {
-        const int pc = w * C::WI + i;
-        wsrc[i] = a.m.w + (size_t)min(gt + pc / 4, gl) * nb * 4096 + pc % 4 * 1024;
-    }
+    const uint8_t *wsrc = a.m.w + (size_t)g0 * nb * 4096;
+    // this wave's requests: row octets w*XI .., the first waves' 64 scales
     // (rows by index lie within 2^32 bytes of the first)
     const bool by_row = a.row != nullptr;
     const uint8_t *xsrc = a.q + (by_row ? 0 : (size_t)t0 * nb * ZZ_F8B);
@@ -92,69 +90,108 @@ __device__ __forceinline__ void zz_fp8_wide(const ZzF8Ep &a, char *lds, int gt, 
     auto fetch = [&](int b) {
         const unsigned d = lb + (b & 1) * C::STAGE;
 #pragma unroll
-        for (int i = 0; i < C::WI; i++) zz_dma16(wsrc[i] + (size_t)b * 4096, l * 16, d + (w * C::WI + i) * 1024);
-#pragma unroll
-        for (int i = 0; i < C::XI; i++) zz_dma16(xsrc + (size_t)b * ZZ_F8B, xo[i], d + C::WB + (w * C::XI + i) * 1024);
-        if (w < C::SI) zz_dma4(ssrc + (size_t)b * a.R, so, d + C::WB + C::XB + w * 256);
+        for (int i = 0; i < C::XI; i++) zz_dma16(xsrc + (size_t)b * ZZ_F8B, xo[i], d + (w * C::XI + i) * 1024);
+        if (w < C::SI) zz_dma4(ssrc + (size_t)b * a.R, so, d + C::XB + w * 256);
     };
-    zz_v16f acc[RO], p[RO];
+    struct Codes { zz_u4 v[4]; } w0, w1, w2;
+    auto ask = [&](Codes &c, int b) {                     // behind the last block: its data, not used
+        const uint8_t *from = wsrc + (size_t)min(b, nb - 1) * 4096 + l * 16;
 #pragma unroll
-    for (int i = 0; i < RO; i++) acc[i] = p[i] = zz_f8_zero();
+        for (int k = 0; k < 4; k++) c.v[k] = *(const zz_u4 *)(from + k * 1024);
+    };
+    zz_v16f acc[RS], p[2] = {zz_f8_zero(), zz_f8_zero()};
+#pragma unroll
+    for (int j = 0; j < RS; j++) acc[j] = zz_f8_zero();
     float late = 0.0f, late2 = 0.0f;
-    auto add = [&](int i, float sc, float sc2) {
+    auto add = [&](int j, float sc, float sc2) {
 #pragma unroll
-        for (int k = 0; k < 16; k++) acc[i][k] = fmaf(p[i][k], k < 8 ? sc : sc2, acc[i][k]);
+        for (int k = 0; k < 16; k++) acc[j][k] = fmaf(p[j & 1][k], k < 8 ? sc : sc2, acc[j][k]);
+        asm volatile("" : "+v"(acc[j]));                  // here, not where the sums are read next
     };
-    fetch(0);
-    wsl.ready();
-    wul.ready();
-    for (int b = 0; b < nb; b++) {
+    // A round requests the next block's rows, then the codes of the matrix for the one after it:
+    // before block b what may be on its way are the four requests for the codes of block b + 1, the
+    // youngest. LEFT is their number, 0 behind which nothing was requested.
+    auto round = [&](int b, Codes &wc, auto LEFT, auto next) {
         // block b has arrived for this wave; behind the barrier, for all, and the one before it is read
-        zz_wait_vm<0>();
+        zz_wait_vm<LEFT.value>();
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        zz_i8 wv[2];
+#pragma unroll
+        for (int k = 0; k < 4; k++) asm volatile("" : "+v"(wc.v[k]));
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            const zz_u4 u = wc.v[2 * k], v = wc.v[2 * k + 1];
+            wv[k] = zz_i8{(int)u.x, (int)u.y, (int)u.z, (int)u.w, (int)v.x, (int)v.y, (int)v.z, (int)v.w};
+        }
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
         if (b + 1 < nb) fetch(b + 1);
+        asm volatile("" ::: "memory");
+        next(b + 2);
+        asm volatile("" ::: "memory");
         const char *d = lds + (b & 1) * C::STAGE;
-        const int t = ws * 32 + r;
-        zz_i8 wv[RO][2], xv[2];
+        zz_i8 xv[2][2];
+        auto operand = [&](int j) {
+            const char *q = d + (j * 32 + r) * 128;
 #pragma unroll
-        for (int k = 0; k < 2; k++) {
-            const char *q = d + C::WB + t * 128;
-            xv[k] = zz_f8_pair(q + 16 * ((4 * k + h) ^ ((r >> 1) & 7)), q + 16 * ((4 * k + 2 + h) ^ ((r >> 1) & 7)));
+            for (int k = 0; k < 2; k++)
+                xv[j & 1][k] = zz_f8_pair(q + 16 * ((4 * k + h) ^ ((r >> 1) & 7)), q + 16 * ((4 * k + 2 + h) ^ ((r >> 1) & 7)));
+        };
+        operand(0);
+        float sc[RS], sc2[RS];
+        const float wsc = wsl.of(b), wsc2 = G == 2 ? wul.of(b) : wsc;
 #pragma unroll
-            for (int i = 0; i < RO; i++) {
-                const char *c = d + ((wo * RO + i) * 4 + 2 * k) * 1024 + l * 16;
-                wv[i][k] = zz_f8_pair(c, c + 1024);
-            }
+        for (int j = 0; j < RS; j++) {
+            const float xsc = *(const float *)(d + C::XB + 4 * (j * 32 + r));
+            sc[j] = xsc * wsc;
+            sc2[j] = G == 2 ? xsc * wsc2 : sc[j];
         }
-        const float xsc = *(const float *)(d + C::WB + C::XB + 4 * t);
-        const float sc = xsc * wsl.of(b), sc2 = G == 2 ? xsc * wul.of(b) : sc;
 #pragma unroll
-        for (int i = 0; i < RO; i++) {
+        for (int j = 0; j < RS; j++) {
+            if (j + 1 < RS) operand(j + 1);
             __builtin_amdgcn_sched_barrier(0);
-            p[i] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wv[i][0], xv[0], zz_f8_zero(), 0, 0, 0, 0, 0, 0);
-            p[i] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wv[i][1], xv[1], p[i], 0, 0, 0, 0, 0, 0);
+#pragma unroll
+            for (int k = 0; k < 2; k++)
+                p[j & 1] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wv[k], xv[j & 1][k], k ? p[j & 1] : zz_f8_zero(), 0, 0, 0, 0, 0, 0);
             __builtin_amdgcn_sched_barrier(0);
-            if (RO == 1) add(0, sc, sc2);
-            else if (i) add(i - 1, sc, sc2);
-            else add(RO - 1, late, late2);
+            if (j) add(j - 1, sc[j - 1], sc2[j - 1]);
+            else add(RS - 1, late, late2);
         }
-        late = sc;
-        late2 = sc2;
+        late = sc[RS - 1];
+        late2 = sc2[RS - 1];
+    };
+    std::integral_constant<int, 4> four;
+    std::integral_constant<int, 0> none;
+    ask(w0, 0);
+    asm volatile("" ::: "memory");
+    fetch(0);
+    asm volatile("" ::: "memory");
+    ask(w1, 1);
+    asm volatile("" ::: "memory");
+    wsl.ready();
+    wul.ready();
+    // in threes, so that no register is moved before it is there; a round skipped inside the loop
+    // would have the compiler wait for the youngest codes
+    int b = 0;
+    for (; b + 3 <= nb; b += 3) {
+        round(b, w0, four, [&](int n) { ask(w2, n); });
+        round(b + 1, w1, four, [&](int n) { ask(w0, n); });
+        round(b + 2, w2, four, [&](int n) { ask(w1, n); });
     }
-    if constexpr (RO > 1) add(RO - 1, late, late2);
+    if (b < nb) round(b, w0, four, [](int) {});
+    if (b + 1 < nb) round(b + 1, w1, none, [](int) {});
+    add(RS - 1, late, late2);
     // The tile goes through LDS, [row][packed row] in 16-byte pieces (a row's pieces permuted by the
     // row, for the banks), and leaves in whole lines.
     float *tile = (float *)lds;
     auto place = [&](int t, int o) { return tile + t * C::O + 4 * ((((o >> 2) ^ t) & 7) | ((o >> 2) & ~7)); };
     __syncthreads();                                      // the last block is read
 #pragma unroll
-    for (int i = 0; i < RO; i++)
+    for (int j = 0; j < RS; j++)
 #pragma unroll
         for (int k = 0; k < 4; k++)
-            *(float4 *)place(ws * 32 + r, (wo * RO + i) * 32 + 8 * k + 4 * h) =
-                make_float4(acc[i][4 * k], acc[i][4 * k + 1], acc[i][4 * k + 2], acc[i][4 * k + 3]);
+            *(float4 *)place(j * 32 + r, w * 32 + 8 * k + 4 * h) =
+                make_float4(acc[j][4 * k], acc[j][4 * k + 1], acc[j][4 * k + 2], acc[j][4 * k + 3]);
     __syncthreads();
     constexpr int RL = C::O / 32 * GC / 8;                // lanes a row
     for (int q = tid; q < C::S * RL; q += C::NT) {
@@ -172,17 +209,17 @@ __device__ __forceinline__ void zz_fp8_wide(const ZzF8Ep &a, char *lds, int gt, 
     }
 }
 
-// OCC: waves a SIMD, so that three or four tiles, two of the largest, share a CU
-template <int G, int RO, int WO, int WS, int OCC>
-__global__ __launch_bounds__(64 * WO * WS, OCC) void zz_fp8_wide_kernel(ZzF8Ep a) {
+// OCC: waves a SIMD that the registers are to allow
+template <int G, int RS, int WO, int OCC>
+__global__ __launch_bounds__(64 * WO, OCC) void zz_fp8_wide_kernel(ZzF8Ep a) {
     extern __shared__ __attribute__((aligned(1024))) char lds[];
-    typedef ZzF8Wide<RO, WO, WS> C;
+    typedef ZzF8Wide<RS, WO> C;
     int ot, st;
     if (!zz_f8_place<G, zz_bf16, C::O / 32, C::S>(a, &ot, &st)) return;
-    zz_fp8_wide<G, RO, WO, WS>(a, lds, ot * C::O / 32, st * C::S);
+    zz_fp8_wide<G, RS, WO>(a, lds, ot * C::O / 32, st * C::S);
 }
 
-template <int G, int RO, int WO, int WS, int OCC>
+template <int G, int RS, int WO, int OCC>
 static bool launch_wide(const ZzF8EpCall &c, const ZzF8Ep &a, hipStream_t st) {
-    return launch_tiles_ep<ZzF8Wide<RO, WO, WS>, G>(c, a, zz_fp8_wide_kernel<G, RO, WO, WS, OCC>, st);
+    return launch_tiles_ep<ZzF8Wide<RS, WO>, G>(c, a, zz_fp8_wide_kernel<G, RS, WO, OCC>, st);
 }
