@@ -705,6 +705,14 @@ def test_experts(E, P, O, I, gated, kind):
                 c.mat.close()
 
 
+@pytest.mark.parametrize("dtype, gated, E, P, O, I", [
+    (F32, False, 39, 1265, 434, 261), (F32, True, 145, 172, 17, 534), (F32, True, 26, 865, 153, 790), (F32, True, 104, 3766, 65, 300),
+    (F32, True, 91, 3045, 43, 538), (BF16, False, 145, 150, 39, 531), (BF16, False, 46, 3152, 131, 515), (BF16, False, 53, 1699, 149, 848),
+    (BF16, True, 152, 152, 17, 534), (BF16, True, 91, 3296, 35, 872), (BF16, True, 74, 2726, 49, 529), (BF16, True, 13, 400, 700, 259)])
+def test_experts_in_the_smaller_forms(dtype, gated, E, P, O, I):
+    test_experts_in_every_form(dtype, gated, E, P, O, I)
+
+
 @pytest.mark.parametrize("dtype, gated, E, P, O, I, ldy", [
     (F32, False, 3, 20, 70, 300, 1 << 28), (BF16, True, 3, 20, 70, 300, 1 << 28), (F32, True, 2, 700, 130, 260, 1 << 23),
     (BF16, False, 2, 700, 130, 260, 1 << 23), (F32, False, 2, 9000, 140, 130, 1 << 19), (BF16, True, 2, 9000, 140, 130, 1 << 19)])
