@@ -31,6 +31,8 @@
 #define ZZ_EP_NONE      0
 #define ZZ_EP_GELU_TANH 1   /* v / (1 + exp(-sqrt(8/pi) (v + 0.044715 v^3))), gelu in its tanh form */
 #define ZZ_EP_SILU      2   /* v / (1 + exp(-v)) */
+/* or'ed to the activation: the caller takes sums of fewer bits for speed (zz_fp8_matmul_ep_dev) */
+#define ZZ_EP_8BIT      16
 
 #ifdef __cplusplus
 extern "C" {
@@ -97,14 +99,18 @@ int zz_fp8_upload_expert_dev(int mat, int e, int part, const uint8_t *d_codes, c
  *   y = act(v) + res                                        a plain matrix
  *   y = act(min(v_gate, clamp)) * clip(v_up, -clamp, clamp) + res       a gated pair
  * in f32, rounded once to `dtype`. bias f32 [O], a gated pair's [2][O], gate's first (NULL:
- * none); act ZZ_EP_*; clamp > 0, or 0 for none (a plain matrix takes none); res [S, O] of `dtype`,
+ * none); act ZZ_EP_*, with or without ZZ_EP_8BIT; clamp > 0, or 0 for none (a plain matrix takes none); res [S, O] of `dtype`,
  * rows ldr apart (0: O; NULL: none), may be y itself, rows as far apart. The activations are of
  * one hardware exponential and one reciprocal: off by up to (6 + 10 |a|) 2^-24 of the value, a
  * the exponent, beside what v is off. A NaN stays one; act(-infinity) is NaN, infinity times
- * 0. Results in bf16 of more than some dozens of rows are of the 8-bit matrix instructions: within
- * each 8 columns a product is cut to 13 bits behind the leading one of the largest, before they are
- * added up in f32. That is 1.4e-5 of the 2-norm for normally distributed codes and less than 8.6e-4 of
- * the terms' magnitudes at worst, beside the 2^-8 of a result's rounding. Other limits and promises as
+ * 0. The order in which the blocks of 128 columns are added up follows from the sizes, S among them:
+ * a row's result can differ in its last bits between calls of different S.
+ * With ZZ_EP_8BIT in act, results in bf16 of more than some dozens of rows come from the 8-bit matrix
+ * instructions, at up to twice the rate: within each 8 columns a product is cut, towards zero, to 13
+ * bits behind the leading one of the largest, before they are added up in f32. That is 1.4e-5 of the
+ * 2-norm for normally distributed codes and less than 8.6e-4 of the terms' magnitudes at worst, beside
+ * the 2^-8 of a result's rounding; where terms cancel, of the result it can be any part. Results in
+ * f32 and of few rows are the same with it and without. Other limits and promises as
  * zz_fp8_matmul_dev's, S <= 2^20. y overlaps no other argument. */
 int zz_fp8_matmul_ep_dev(int mat, const uint8_t *d_q, const float *d_s, int S, const float *d_bias, int act,
                          float clamp, const void *d_res, int64_t ldr, int dtype, void *d_y, int64_t ldy,

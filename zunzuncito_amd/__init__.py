@@ -21,7 +21,7 @@ GPU_FMT_Q40, GPU_FMT_Q80, GPU_FMT_TQ2, GPU_FMT_Q4A = 1, 2, 3, 4
 ZZ_GATE_SOFTMAX_PES, ZZ_GATE_SIGMOID_BIAS, ZZ_GATE_SOFTMAX_TOPK, ZZ_GATE_DENSE = 0, 1, 2, 3
 ZZ_GATE_GROUPED = 4
 ZZ_F32, ZZ_BF16 = 0, 1
-ZZ_EP_NONE, ZZ_EP_GELU_TANH, ZZ_EP_SILU = 0, 1, 2
+ZZ_EP_NONE, ZZ_EP_GELU_TANH, ZZ_EP_SILU, ZZ_EP_8BIT = 0, 1, 2, 16
 ZZ_BEAM_MAXW, ZZ_BEAM_MAXV = 16, 524288
 ZZ_EXPERTS_MAXE, ZZ_EXPERTS_MAXK = 512, 16
 ZZ_ACT_GEGLU_TANH, ZZ_ACT_SWIGLU, ZZ_ACT_SWIGLU_CLAMP = 0, 1, 2
@@ -554,7 +554,8 @@ class Fp8Matrix:
 
     def matmul_ep_dev(self, d_q, d_s, S, d_y, d_bias=0, act=ZZ_EP_NONE, clamp=0.0, d_res=0, dtype=ZZ_F32, ldr=0, ldy=0,
                       stream=0):
-        """act(product + bias) + res, for a gated pair act(gate) * up + res (zz_fp8_matmul_ep_dev)."""
+        """act(product + bias) + res, for a gated pair act(gate) * up + res (zz_fp8_matmul_ep_dev);
+        act | ZZ_EP_8BIT: results in bf16 of many rows from the 8-bit matrix instructions."""
         if not lib().zz_fp8_matmul_ep_dev(self.id, d_q or None, d_s or None, S, d_bias or None, act, clamp, d_res or None,
                                           ldr, dtype, d_y or None, ldy, stream or None):
             raise RuntimeError(f"zz_fp8_matmul_ep_dev declined: {last_error()}")

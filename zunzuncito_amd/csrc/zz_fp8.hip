@@ -315,7 +315,8 @@ extern "C" int zz_fp8_matmul(int id, const float *x, float *y, int S) {
 // what both calls check without a device
 static int ep_common(const char *who, const ZzF8EpCall &c) {
     if (c.dtype != ZZ_F32 && c.dtype != ZZ_BF16) ZZ_FAIL("%s: dtype %d declined", who, c.dtype);
-    if (c.act < ZZ_EP_NONE || c.act > ZZ_EP_SILU) ZZ_FAIL("%s: activation %d declined", who, c.act);
+    const int act = c.act & ~ZZ_EP_8BIT;
+    if (act < ZZ_EP_NONE || act > ZZ_EP_SILU) ZZ_FAIL("%s: activation %d declined", who, c.act);
     if (!(c.clamp >= 0.0f) || isinf(c.clamp)) ZZ_FAIL("%s: clamp has to be finite and not negative", who);
     const int64_t far = (int64_t)1 << 36;                 // P rows' bytes stay under 2^62
     if (!c.q || !c.s || !c.y || c.ldy < 0 || c.ldy > far || c.ldr < 0 || c.ldr > far) ZZ_FAIL("%s: bad arguments", who);
@@ -347,6 +348,8 @@ static int ep_run(const char *who, Fp8Mat *m, ZzF8EpCall &c, void *stream) {
     c.we = (int64_t)wbytes(m);
     c.wsu = (int)scale_count(m);
     c.wse = m->parts * c.wsu;
+    c.eight = c.act & ZZ_EP_8BIT;
+    c.act &= ~ZZ_EP_8BIT;
     hipStream_t st = stream ? (hipStream_t)stream : zz_lib_stream();
     if (!(m->parts == 2 ? zz_launch_fp8_gated(c, st) : zz_launch_fp8_ep(c, st))) ZZ_FAIL("%s: launch failed", who);
     return 1;

@@ -131,7 +131,7 @@ struct ZzF8EpCall {
     const float *bias;
     const void *res;
     int64_t ldr;
-    int act;
+    int act, eight;             // ZZ_EP_*; whether the 8-bit instructions may be taken
     float clamp;
     int dtype;
     void *y;

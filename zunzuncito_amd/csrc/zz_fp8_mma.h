@@ -7,8 +7,7 @@
 // the matrix core adds them up in f32. The 8-bit instructions do not (zz_fp8_wide.h): they are
 // 1.4e-5 off in the 2-norm over normally distributed codes and up to 8.5e-4 of the terms' magnitudes,
 // where the f16 form is 1e-8 and 2e-7 off, at twice the rate (8192^3 in a library 2.7 PFLOP/s, in
-// f16 1.35). Results in bf16, whose own rounding is a hundred times as large, bear them: those with
-// an epilogue of many rows take them, the product without one has this form for both types. bf16
+// f16 1.35). A product with an epilogue takes them where its caller allows it. bf16
 // holds every code too, and its library product is faster (1.48): not tried.
 //
 // A block of 128 columns is eight v_mfma_f32_32x32x16_f16 of 32 matrix rows times 32
@@ -525,8 +524,9 @@ __device__ __forceinline__ void zz_fp8_at(int id, int OT, int ST, int *ot, int *
 }
 
 // The form that is expected to take the shortest for `tables` products of S rows each
-// (zz_fp8_mma.hip), of all plain ones, or of those with an epilogue and results in f32 or bf16
+// (zz_fp8_mma.hip), of all plain ones, or of those with an epilogue, or of those and the 8-bit
+// instructions' tiles
 #define ZZ_F8_FORMS_PLAIN 0
-#define ZZ_F8_FORMS_F32   1
-#define ZZ_F8_FORMS_BF16  2
+#define ZZ_F8_FORMS_EP    1
+#define ZZ_F8_FORMS_8BIT  2
 int zz_fp8_form(int O, int S, int tables, int nb, int of);

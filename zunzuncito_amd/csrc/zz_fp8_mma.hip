@@ -148,9 +148,9 @@ int zz_fp8_form(int O, int S, int tables, int nb, int of) {
     int best = 0;
     float least = INFINITY;
     // up to 32 rows the first three: the others' tiles are half empty
-    for (int v = 0; v < (S <= 32 ? 3 : of == ZZ_F8_FORMS_BF16 ? 14 : 11); v++) {
+    for (int v = 0; v < (S <= 32 ? 3 : of == ZZ_F8_FORMS_8BIT ? 14 : 11); v++) {
         const ZzF8Form &f = mm_forms[v];
-        if ((of == ZZ_F8_FORMS_BF16 && v >= 6 && v < 11) || (of && f.parts)) continue;
+        if ((of == ZZ_F8_FORMS_8BIT && v >= 6 && v < 11) || (of && f.parts)) continue;
         int64_t n = (int64_t)((O + f.o - 1) / f.o) * ((S + f.s - 1) / f.s) * tables;
         const int r = (nb + f.ks - 1) / f.ks, cap = 256 * f.per;
         float t = 0.0f;

@@ -1,14 +1,17 @@
-// zz_fp8_wide.h -- tiles of the fp8 product with an epilogue whose results are bf16: the codes go
-// into v_mfma_f32_32x32x64_f8f6f4 as they are.
+// zz_fp8_wide.h -- tiles of the fp8 product with an epilogue whose results are bf16, where the
+// caller takes sums of fewer bits (ZZ_EP_8BIT): the codes go into v_mfma_f32_32x32x64_f8f6f4 as
+// they are.
 //
 // That instruction adds products up in f32, but first cuts the eight of each 8 columns to 13 bits
 // behind the leading one of their largest, towards zero (measured: beside 2^14, 3.5 counts as 2 in
 // the same eight and as itself in another). A product has 8 bits, so that it loses something only
 // below 2^-5 of the largest, and less than 2^-13 of it: 7 x 2^-13 = 8.5e-4 of the terms' magnitudes
 // at worst, 1.4e-5 of the 2-norm over normally distributed codes and 5e-5 over all codes alike. A
-// result's own rounding to bf16 is 1.7e-3 in the 2-norm and up to 2^-8, so that it hides this; f32
-// results, which would show it, and few rows, whose time is the matrix's bytes, keep
-// zz_fp8_mma.h's f16 products.
+// result's own rounding to bf16 is 1.7e-3 in the 2-norm and up to 2^-8, which hides this unless
+// the terms cancel: then nothing may be left (2^14 - 2^14 + 36, the 36 from four products beside
+// the first, comes out as 0). So no call has these tiles that does not ask for them; f32
+// results, which would show the cut, and few rows, whose time is the matrix's bytes, keep
+// zz_fp8_mma.h's f16 products all the same.
 //
 // Without the conversions and at twice the rate: 8192 x 2816 x 2112 65 us (1.50 PFLOP/s) where the
 // f16 tiles take 115; 2048 x 4224 x 2816 gated 36.4 for 71; 32768 rows of 128 experts, 1408 x 2816,
