@@ -2,6 +2,7 @@
 // zz_fp8_mma.hip) and their launchers.
 #pragma once
 #include "zz_common.h"
+#include "zz_fp8_form.h"
 
 #define ZZ_F8B 128                  // elements under one scale
 #define ZZ_F8MAX 448.0f             // largest e4m3 value
@@ -80,11 +81,6 @@ __device__ __forceinline__ void zz_put8(T *p, const float (&v)[8], int n) {
     for (int j = 0; j < 8; j++)
         if (j < n) zz_put(p + j, v[j]);
 }
-
-// An output of at least this many bytes, a quarter of the 256 MB cache in front of memory, is
-// stored past it: who reads it next finds little of it there, and its dirty lines would be
-// written back under the next kernels' reads.
-#define ZZ_NT_BYTES ((int64_t)64 << 20)
 
 struct ZzF8RowsArgs {
     const void *x, *res;        // res, sum, w may be null

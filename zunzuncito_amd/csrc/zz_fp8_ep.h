@@ -159,26 +159,6 @@ static bool launch_async_ep(const ZzF8EpCall &c, const ZzF8Ep &a, hipStream_t st
 
 #include "zz_fp8_wide.h"
 
-// The form for P rows of m matrices, `per` each, O packed rows, nb blocks: zz_fp8_form's choice, but for
-// tables. How the rows are spread is not known here, and a router's choice is skewed: some experts
-// have many times the average, and with tiles of 32 rows their matrices are read that many times,
-// while tiles that are nearly empty cost little (their rows are one, read from the caches). Over a
-// Zipf spread:
-// on the 8-bit instructions from 2^19 packed results on, 128 x 64 tiles at least: 512 pairs of 128 experts, 1408 x 2816 gated,
-// 14.5 us and few-row form 19; 360 of 16, 2800 x 2048, 13.3 and 19.6; 1200 of 32, 3584 x 2048, 19.9 and in
-// 64 x 64 24.0; but 1400 of 8, 500 x 3000, 16.6 and in f16 tiles 14.4. Below: 256 pairs of the first
-// 14.1 and 14.2, 192 14.0 and 12.8; 120 of 8, 4096 x 1024, 8.9 and 7.2.
-// Many matrices of few rows else, from 2048 workgroups of the few-row form on: that form (128 pairs of the
-// first 12.1, two groups a wave 14.9), on the f16 ones from 5 rows an expert on 64 x 128 tiles: 1024 pairs of
-// 128, 2816 x 704 in f32, 16 and in 32 x 32 29, 4096 34 and 78; 1136 of 47, 1044 x 1664 (1551), 16.1 and few rows 13.8.
-static int ep_form(int O, int P, int per, int m, int nb, bool eight) {
-    const int v = zz_fp8_form(O, per, m, nb, eight ? ZZ_F8_FORMS_8BIT : ZZ_F8_FORMS_EP);
-    if (m == 1) return v;
-    if (eight && (int64_t)P * O >= 1 << 19) return v > 12 ? v : 12;
-    if (per > 32 || (int64_t)m * ((O + 31) / 32) <= 2048) return v;
-    return eight || per <= 4 ? 1 : 7;
-}
-
 template <typename T, int G>
 static bool launch_ep(const ZzF8EpCall &c, hipStream_t st) {
     ZzF8Ep a;
@@ -187,29 +167,23 @@ static bool launch_ep(const ZzF8EpCall &c, hipStream_t st) {
     a.offs = c.offs; a.E = c.E; a.P = c.P; a.we = c.we; a.wse = c.wse; a.wsu = c.wsu;
     // large results past the caches where tiles write whole lines, as zz_fp8_mma.hip's
     a.nt = c.P * a.ldy * (int64_t)sizeof(T) >= ZZ_NT_BYTES && (uintptr_t)a.y % 64 == 0 && a.ldy * sizeof(T) % 64 == 0;
-    // the experts that can have rows, and each one's rows, were they spread evenly
-    const int m = c.offs ? (c.E < c.P ? c.E : c.P) : 1, per = (c.P + m - 1) / m;
-    const int O = G * c.m.O;                              // packed rows
-    const int v = ep_form(O, c.P, per, m, a.nb, sizeof(T) == 2 && c.eight);
-    // matrices past the caches are read past them too, as zz_fp8_mma.hip's; several of them by four
-    // waves a workgroup (128 pairs of 128 experts, 1408 x 2816: 11.9 us, by eight 17.5)
-    const bool nt = per <= 32 && (int64_t)m * O * c.m.I >= ZZ_NT_BYTES;
+    const int v = zz_f8_ep_kernel(G * c.m.O, c.m.I, c.P, c.E, c.offs != nullptr, sizeof(T) == 2 && c.eight);
     bool ok = false;
     if (v == 0) ok = launch_few_ep<T, G, 1, 1, 16, false, false>(c, a, st);
-    else if (v == 1 && nt && m > 1) ok = launch_few_ep<T, G, 1, 1, 4, true, true>(c, a, st);
-    else if (v == 1 && nt && per <= 8) ok = launch_few_ep<T, G, 1, 1, 8, true, true>(c, a, st);
-    else if (v == 1 && nt) ok = launch_few_ep<T, G, 2, 1, 4, true, true>(c, a, st);
     else if (v == 1) ok = launch_few_ep<T, G, 1, 1, 4, true, false>(c, a, st);
     else if (v == 2) ok = launch_few_ep<T, G, 2, 1, 8, false, false>(c, a, st);
     else if (v == 3) ok = launch_async_ep<T, G, 1, 1, 2, 1, 2, 2, false>(c, a, st);
     else if (v == 4) ok = launch_async_ep<T, G, 1, 2, 2, 1, 4, 2, false>(c, a, st);
     else if (v == 5) ok = launch_async_ep<T, G, 1, 2, 2, 1, 2, 2, false>(c, a, st);
+    else if (v == 14) ok = launch_few_ep<T, G, 1, 1, 4, true, true>(c, a, st);
+    else if (v == 15) ok = launch_few_ep<T, G, 1, 1, 8, true, true>(c, a, st);
+    else if (v == 16) ok = launch_few_ep<T, G, 2, 1, 4, true, true>(c, a, st);
     if (ok) return true;
     // the largest tiles also where smaller ones are more than a launch holds
     if constexpr (sizeof(T) == 2) {
         if (v == 11 && launch_wide<G, 2, 2, 2>(c, a, st)) return true;
         if (v == 12 && launch_wide<G, 2, 4, 3>(c, a, st)) return true;
-        if (v >= 11) return launch_wide<G, 4, 4, 2>(c, a, st);
+        if (v >= 11 && v <= 13) return launch_wide<G, 4, 4, 2>(c, a, st);
     }
     if (v == 6 && launch_async_ep<T, G, 1, 1, 2, 2, 1, 3, false>(c, a, st)) return true;
     if (v == 7 && launch_async_ep<T, G, 1, 2, 2, 2, 1, 2, true>(c, a, st)) return true;

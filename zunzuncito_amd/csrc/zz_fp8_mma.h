@@ -522,11 +522,3 @@ __device__ __forceinline__ void zz_fp8_at(int id, int OT, int ST, int *ot, int *
     *ot = in / pw;
     *st = pan * PW + in % pw;
 }
-
-// The form that is expected to take the shortest for `tables` products of S rows each
-// (zz_fp8_mma.hip), of all plain ones, or of those with an epilogue, or of those and the 8-bit
-// instructions' tiles
-#define ZZ_F8_FORMS_PLAIN 0
-#define ZZ_F8_FORMS_EP    1
-#define ZZ_F8_FORMS_8BIT  2
-int zz_fp8_form(int O, int S, int tables, int nb, int of);

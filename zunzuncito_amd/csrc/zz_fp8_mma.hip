@@ -111,66 +111,6 @@ static bool launch_few(const ZzF8Mm &a, hipStream_t st) {
     return true;
 }
 
-// Which form: the one that is expected to take the shortest. A form's workgroups go round by
-// round through the 256 CUs, `per` of them on a CU at once; a round with k workgroups on the
-// busiest CU takes fix[k-1] + slope[k-1] * (blocks that a K group runs) microseconds. A form with
-// `parts` runs what is over a multiple of 256 tiles in that many parts each, if these are at most
-// one a CU: 2.9 + 0.49 * blocks after a full round, or less beside workgroups that are there
-// (`busy`: fixed, a block, a block with a part on each CU). Fitted to 114 shapes (O 704 to 65536,
-// I 256 to 8192, S 1 to 8192) with an rms error of 6 to 17 %. Over them the choice lies 2 % behind
-// the best form of each, and up to 17 %. Any one form for all loses far more: the first and the
-// last but one take 4.8 and 25.6 us for 1 x 4224 x 2816, 295 and 109 for 4096 rows; without the
-// parts 4096 x 4224 x 2816 takes 107 us where it takes 95, 1000 x 4224 x 2816 36 for 30.
-// The model has no bandwidth in it and holds for what it was fitted to. For few rows of matrices
-// past the caches its times lie below what their bytes take (262144 x 4096: 131 us, where a read at
-// 7.1 TB/s takes 151), and from about 3700 columns on it prefers the third form, whose loads go
-// through the caches: 1 row of 262144 x 4096 180 us (6.0 TB/s), of 128256 x 7168 152 (6.1), of 18432
-// x 7168 30 (4.4), where the second form's past the caches reaches 6.9 at 262144 x 2816.
-struct ZzF8Form { int o, s, ks, per; float fix[4], slope[4]; int parts; float busy[3]; };
-static const ZzF8Form mm_forms[] = {
-    {32, 32, 16, 1, {1.9f}, {2.0f}},
-    {32, 32, 4, 4, {2.9f, 2.3f, 2.6f, 0.7f}, {0.52f, 1.14f, 1.64f, 2.11f}},
-    {64, 32, 8, 1, {2.6f}, {1.4f}},
-    {64, 32, 2, 4, {2.8f, 3.2f, 2.9f, 2.5f}, {0.64f, 0.80f, 1.16f, 1.43f}},
-    {64, 64, 4, 1, {3.4f}, {1.14f}},
-    {64, 64, 2, 2, {3.0f, 2.8f}, {0.82f, 1.14f}},
-    {64, 64, 1, 3, {2.8f, 3.9f, 2.1f}, {0.49f, 0.66f, 0.95f}},
-    {64, 128, 1, 3, {3.4f, 6.0f, 4.0f}, {0.74f, 0.96f, 1.49f}},
-    {64, 128, 1, 3, {3.4f, 6.0f, 4.0f}, {0.74f, 0.96f, 1.49f}, 2, {0.2f, 0.05f, 0.10f}},
-    {128, 128, 1, 2, {4.5f, 7.8f}, {1.04f, 1.59f}},
-    {128, 128, 1, 2, {4.5f, 7.8f}, {1.04f, 1.59f}, 4, {1.6f, 0.03f, 0.13f}},
-    // zz_fp8_wide.h's, from 512 and 2816 columns with one to `per` workgroups on each CU
-    {64, 64, 1, 4, {4.6f, 5.6f, 6.5f, 6.9f}, {0.41f, 0.45f, 0.48f, 0.62f}},
-    {128, 64, 1, 3, {5.1f, 6.6f, 7.6f}, {0.46f, 0.58f, 0.81f}},
-    {128, 128, 1, 2, {7.8f, 9.2f}, {0.63f, 0.93f}},
-};
-int zz_fp8_form(int O, int S, int tables, int nb, int of) {
-    int best = 0;
-    float least = INFINITY;
-    // up to 32 rows the first three: the others' tiles are half empty
-    for (int v = 0; v < (S <= 32 ? 3 : of == ZZ_F8_FORMS_8BIT ? 14 : 11); v++) {
-        const ZzF8Form &f = mm_forms[v];
-        if ((of == ZZ_F8_FORMS_8BIT && v >= 6 && v < 11) || (of && f.parts)) continue;
-        int64_t n = (int64_t)((O + f.o - 1) / f.o) * ((S + f.s - 1) / f.s) * tables;
-        const int r = (nb + f.ks - 1) / f.ks, cap = 256 * f.per;
-        float t = 0.0f;
-        if (f.parts) {
-            const int parts = (int)(n % 256) * f.parts;
-            if (!parts || parts > 256) continue;
-            n -= n % 256;
-            t = n % cap ? f.busy[0] + (f.busy[1] + f.busy[2] * parts / 256.0f) * r : 2.9f + 0.49f * r;
-        }
-        const int rem = (int)(n % cap);
-        t += (float)(n / cap) * (f.fix[f.per - 1] + f.slope[f.per - 1] * r);
-        if (rem) t += f.fix[(rem - 1) / 256] + f.slope[(rem - 1) / 256] * r;
-        if (t < least) {
-            least = t;
-            best = v;
-        }
-    }
-    return best;
-}
-
 template <typename T>
 static bool launch_mm(const ZzF8Mm &a, hipStream_t st) {
     const int v = zz_fp8_form(a.m.O, a.S, 1, a.nb, ZZ_F8_FORMS_PLAIN);
