@@ -33,3 +33,19 @@ def test_8bit_tiles_are_asked_for(forms):
              for p in (1, 7, 60, 300, 2000, 30000)]
     assert all(v <= 9 or v >= 14 for v in forms([(*s, 0) for s in sizes]))
     assert {11, 12, 13} <= set(forms([(*s, 1) for s in sizes]))
+
+
+def test_tables(forms):
+    """1 to 32 rows an expert, spread by no rule that is known: small tiles, not those of 64 x 128, which
+    took 1.6 times as long over even and skewed spreads; many rows: large ones."""
+    for o, i, e in ((1408, 2816, 128), (2816, 704, 128), (3584, 2048, 32), (1536, 2048, 256), (4096, 1024, 128)):
+        assert {v % 13 for v in forms([(o, i, e * per, e, 1, 0) for per in (1, 2)])} == {1}
+        assert set(forms([(o, i, e * per, e, 1, 0) for per in (3, 5, 8, 17, 32)])) == {3}
+        assert set(forms([(o, i, e * 512, e, 1, 0)])) <= {7, 9}
+        assert set(forms([(o, i, e * per, e, 1, 1) for per in (8, 17, 32)])) == {12}
+
+
+def test_small_tables(forms):
+    """Up to 1024 workgroups of the few-row form a table takes what one matrix of its rows does."""
+    for o, i, e, per in ((512, 512, 64, 9), (200, 300, 40, 30), (4096, 1024, 8, 20)):
+        assert forms([(o, i, e * per, e, 1, 0)])[0] in (0, 1, 2, 14)

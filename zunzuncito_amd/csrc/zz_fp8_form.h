@@ -77,30 +77,30 @@ static inline int zz_fp8_form(int O, int S, int tables, int nb, int of) {
     return best;
 }
 
-// The form for P rows of m matrices, `per` each, O packed rows, nb blocks: zz_fp8_form's choice, but for
-// tables of several. How the rows are spread is not known here, and a router's choice is skewed: some experts
-// have many times the average, and with tiles of 32 rows their matrices are read that many times,
-// while tiles that are nearly empty cost little (their rows are one, read from the caches). Over a
-// Zipf spread:
-// on the 8-bit instructions from 2^19 packed results on, 128 x 64 tiles at least: 512 pairs of 128 experts, 1408 x 2816 gated,
-// 14.5 us and few-row form 19; 360 of 16, 2800 x 2048, 13.3 and 19.6; 1200 of 32, 3584 x 2048, 19.9 and in
-// 64 x 64 24.0; but 1400 of 8, 500 x 3000, 16.6 and in f16 tiles 14.4. Below: 256 pairs of the first
-// 14.1 and 14.2, 192 14.0 and 12.8; 120 of 8, 4096 x 1024, 8.9 and 7.2.
-// Many matrices of few rows else, from 2048 workgroups of the few-row form on: that form (128 pairs of the
-// first 12.1, two groups a wave 14.9), on the f16 ones from 5 rows an expert on 64 x 128 tiles: 1024 pairs of
-// 128, 2816 x 704 in f32, 16 and in 32 x 32 29, 4096 34 and 78; 1136 of 47, 1044 x 1664 (1551), 16.1 and few rows 13.8.
+// The form for P rows of m matrices, `per` each on average, O packed rows, nb blocks: zz_fp8_form's
+// choice, but for tables of several from 1024 workgroups of the few-row form on. How the rows are spread
+// is not known here; even, mildly uneven, by Zipf's law (1.1) and over 8 experts alone were measured, 32
+// tables of 2 to 512 experts, 1 to 512 rows an expert. Figures are of bf16 results, f32's within 3 %.
+// On the f16 instructions up to 2 rows an expert the second form (128 experts of 2 x 704 x 2816, 2 rows
+// each: 77 us, the fourth 92), up to 32 the fourth, 64 x 32 tiles (8 rows each, and by Zipf's law: 93 and 90 us,
+// the second 85 and 89; 32 rows: 108 and 128, the second 136 and 175, 64 x 128 tiles 148 and 166): 1.5 to 3 %
+// behind the best form of each, 11 % where 8 experts have all rows, and up to 1.9 times as long there
+// (of 256, 2048 x 768, 32 rows each on average: 76 us, 128 x 128 tiles 44).
+// On the 8-bit ones from 2^19 packed results on 128 x 64 tiles at least, whatever an expert's rows (128
+// experts of 4096 x 1024, by Zipf's law 1, 8, 32 rows each: 39, 91, 110 us, the second form 49, 112, 204; of
+// 2 x 704 x 2816, 4 rows each, 91 and 79), below that the second: 3 to 4 % behind the best of each.
 static inline int zz_f8_ep_form(int O, int P, int per, int m, int nb, bool eight) {
     const int v = zz_fp8_form(O, per, m, nb, eight ? ZZ_F8_FORMS_8BIT : ZZ_F8_FORMS_EP);
     if (m == 1) return v;
     if (eight && (int64_t)P * O >= 1 << 19) return v > 12 ? v : 12;
-    if (per > 32 || (int64_t)m * ((O + 31) / 32) <= 2048) return v;
-    return eight || per <= 4 ? 1 : 7;
+    if (per > 32 || (int64_t)m * ((O + 31) / 32) <= 1024) return v;
+    return eight || per <= 2 ? 1 : 3;
 }
 
 // The kernel of a product with an epilogue: P rows of a table of E matrices (`table`; else one), O packed
 // rows and I columns each. A form, but 14 to 16 the second form's for matrices past the caches, which
-// are read past them too, as zz_fp8_mma.hip's: of several matrices by four waves a workgroup (128
-// pairs of 128 experts, 1408 x 2816: 11.9 us, by eight 17.5), of one for up to 8 rows, and for more.
+// are read past them too, as zz_fp8_mma.hip's: of several matrices by four waves a workgroup, as the second
+// form's (128 pairs to 8 of 128 experts, 1408 x 2816: 11.9 us, by eight 17.5), of one for up to 8 rows, and for more.
 static inline int zz_f8_ep_kernel(int O, int I, int P, int E, bool table, bool eight) {
     // the matrices that can have rows, and each one's rows, were they spread evenly
     const int m = table ? (E < P ? E : P) : 1, per = (P + m - 1) / m;
