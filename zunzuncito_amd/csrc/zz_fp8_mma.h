@@ -325,8 +325,9 @@ __device__ __forceinline__ void zz_wait_vm() {
 
 // A matrix's scales, one of 64 blocks in each lane: a round takes its own from there by a readlane,
 // where a load just before the round's wait for its codes would be waited for with them (512 x 4224 x
-// 2816 took 26.4 us with that and takes 25.1). The first is waited for in ready(), so that others can be
-// requested with it, the later ones where they are made, so that nothing waits for them elsewhere.
+// 2816 took 26.4 us with that and takes 25.1). The first is waited for in ready(), behind the first
+// blocks' requests (before them 512 x 4224 x 2816 without an epilogue took 20.1 us, behind them 19.7, 512 x
+// 65536 x 704 62.3 and 60.8), the later ones where they are made, so that nothing waits for them elsewhere.
 struct ZzF8Scales {
     const float *p;
     int nb, base = 0;
@@ -403,8 +404,6 @@ __device__ __forceinline__ void zz_fp8_tile(const A &a, char *lds, int gt, int t
 #pragma unroll
     for (int i = 0; i < C::XI; i++)
         xo[i] = xo[i] * nb * ZZ_F8B + 16 * ((l & 7) ^ ((((w * C::XI + i) & 1) << 2) | (l >> 4)));
-    wsl.ready();
-    wul.ready();
     auto fetch = [&](int it, int slot) {
         const int b = min(it * KS + kg, nb - 1);          // behind the last block: its data, not used
         const unsigned d = lb + slot * C::STAGE;
@@ -423,6 +422,8 @@ __device__ __forceinline__ void zz_fp8_tile(const A &a, char *lds, int gt, int t
 #pragma unroll
     for (int i = 0; i < NS - 1; i++)
         if (i < rounds) fetch(i, i);
+    wsl.ready();
+    wul.ready();
     int slot = 0, into = NS - 1;
     for (int it = 0; it < rounds; it++) {
         const int b = it * KS + kg;
