@@ -1,0 +1,55 @@
+"""The fp8 product's far limits: the largest gated pairs."""
+import pytest
+import torch
+
+import zunzuncito_amd as zz
+from test_gpu_experts import ptr, stream
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True, scope="module")
+def _up():
+    zz.init()
+
+
+def free(gb):
+    torch.cuda.empty_cache()
+    return torch.cuda.mem_get_info()[0] >= gb << 30
+
+
+# 2^35 packed codes and more are laid out by more threads than one launch holds
+@pytest.mark.parametrize("O, I", [((1 << 19) - 1, 1 << 16), (1 << 24, 2047)])
+def test_largest_gated_pair(O, I):
+    if not free(130):
+        pytest.skip("needs 130 GiB of device memory")
+    nb, no = -(-I // 128), -(-O // 128)
+    codes = torch.zeros(O, I, dtype=torch.uint8, device="cuda")
+    rows = [0, 15, 16, 12345, O // 2, O - 2, O - 1]
+    codes[rows] = 0x38                                    # 1.0
+    ws = torch.full((no, nb), 1.0 / I, device="cuda")
+    mat = zz.Fp8Experts(1, O, I, gated=True)
+    try:
+        torch.cuda.synchronize()
+        mat.upload_dev(0, ptr(codes), ptr(ws))
+        codes[rows[3]] = 0
+        ws *= 2.0
+        torch.cuda.synchronize()
+        mat.upload_dev(0, ptr(codes), ptr(ws), part=1)
+        del codes
+        q = torch.zeros(2, nb * 128, dtype=torch.uint8, device="cuda")
+        q[:, :I] = 0x38
+        s = torch.tensor([1.0, 4.0], device="cuda").expand(nb, 2).contiguous()
+        bias = torch.zeros(2, O, device="cuda")
+        bias[1] = 0.5                                     # up's: a column without codes is gate's 0 times a half
+        y = torch.full((3, O), 9.0, device="cuda")
+        mat.matmul_ep_dev(ptr(q), ptr(s), 2, ptr(y), d_bias=ptr(bias), stream=stream())
+        want = torch.zeros(2, O, device="cuda")
+        want[0, rows], want[1, rows] = 2.5, 4.0 * 8.5
+        want[0, rows[3]], want[1, rows[3]] = 0.5, 2.0
+        assert (y[2] == 9.0).all()
+        assert (y[:2] - want).abs().max() <= 34.0 * 2 * (I + nb) * 2.0 ** -24
+        assert ((y[:2] != 0) == (want != 0)).all()
+    finally:
+        mat.close()
+        torch.cuda.empty_cache()

@@ -43,38 +43,39 @@ __global__ __launch_bounds__(256, 2) void zz_fp8_tiles_kernel(ZzF8Mm a, int whol
 
 // one 16-byte piece of the packed layout per thread; part 0, 1: gate's, up's rows of a gated pair
 // (-1: a plain matrix), the other's left as they are. The first threads copy the scales, of which
-// there are fewer than pieces.
+// there are fewer than pieces. Pieces can be more than a launch's threads.
 __global__ __launch_bounds__(256) void zz_fp8_pack_kernel(const uint8_t *src, int O, int I, int nb, uint8_t *dst,
                                                           int64_t n, int part, const float *scales, float *ws, int ns) {
-    const int64_t p = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (p < ns) ws[p] = scales[p];
-    if (p >= n) return;
-    const int l = (int)(p & 63), pc = (int)(p >> 6) & 3;
-    const int64_t gb = p >> 8, g = gb / nb;
-    const int b = (int)(gb - g * nb), k = b * ZZ_F8B + 32 * pc + 16 * (l >> 5);
-    int64_t row = g * 32 + (l & 31);
-    if (part >= 0) {
-        if (((l >> 4) & 1) != part) return;
-        row = g * 16 + (l & 15);
-    }
-    unsigned w[4] = {0, 0, 0, 0};
-    if (row < O) {
-        const uint8_t *s = src + row * I + k;
-        if (k + 16 <= I) {
-            __builtin_memcpy(w, s, 16);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 16; j++)
-                if (k + j < I) w[j >> 2] |= (unsigned)s[j] << (8 * (j & 3));
+    for (int64_t p = (int64_t)blockIdx.x * 256 + threadIdx.x; p < n; p += (int64_t)gridDim.x * 256) {
+        if (p < ns) ws[p] = scales[p];
+        const int l = (int)(p & 63), pc = (int)(p >> 6) & 3;
+        const int64_t gb = p >> 8, g = gb / nb;
+        const int b = (int)(gb - g * nb), k = b * ZZ_F8B + 32 * pc + 16 * (l >> 5);
+        int64_t row = g * 32 + (l & 31);
+        if (part >= 0) {
+            if (((l >> 4) & 1) != part) continue;
+            row = g * 16 + (l & 15);
         }
+        unsigned w[4] = {0, 0, 0, 0};
+        if (row < O) {
+            const uint8_t *s = src + row * I + k;
+            if (k + 16 <= I) {
+                __builtin_memcpy(w, s, 16);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 16; j++)
+                    if (k + j < I) w[j >> 2] |= (unsigned)s[j] << (8 * (j & 3));
+            }
+        }
+        *(uint4 *)(dst + 16 * p) = make_uint4(w[0], w[1], w[2], w[3]);
     }
-    *(uint4 *)(dst + 16 * p) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 int zz_launch_fp8_pack(const uint8_t *codes, int O, int I, int part, uint8_t *dst, const float *scales, float *ws, hipStream_t st) {
     const int nb = zz_f8_nb(I), gc = part < 0 ? 32 : 16;
     const int64_t n = (int64_t)((O + gc - 1) / gc) * nb * 256;
-    hipLaunchKernelGGL(zz_fp8_pack_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, codes, O, I, nb, dst, n, part,
+    const int64_t g = (n + 255) / 256, most = 1 << 23;    // 2^31 threads
+    hipLaunchKernelGGL(zz_fp8_pack_kernel, dim3((unsigned)(g < most ? g : most)), dim3(256), 0, st, codes, O, I, nb, dst, n, part,
                        scales, ws, scales ? zz_f8_nb(O) * nb : 0);
     return hipGetLastError() == hipSuccess;
 }
