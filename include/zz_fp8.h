@@ -111,7 +111,8 @@ int zz_fp8_upload_expert_dev(int mat, int e, int part, const uint8_t *d_codes, c
  * 2-norm for normally distributed codes and less than 8.6e-4 of the terms' magnitudes at worst, beside
  * the 2^-8 of a result's rounding; where terms cancel, of the result it can be any part. Results in
  * f32 and of few rows are the same with it and without. Other limits and promises as
- * zz_fp8_matmul_dev's, S <= 2^20. y overlaps no other argument. */
+ * zz_fp8_matmul_dev's, S <= 2^20, and results are of less than 2^24 tiles of 128 rows and 128 columns (a
+ * gated pair's: 64). y overlaps no other argument. */
 int zz_fp8_matmul_ep_dev(int mat, const uint8_t *d_q, const float *d_s, int S, const float *d_bias, int act,
                          float clamp, const void *d_res, int64_t ldr, int dtype, void *d_y, int64_t ldy,
                          void *stream);
@@ -121,7 +122,7 @@ int zz_fp8_matmul_ep_dev(int mat, const uint8_t *d_q, const float *d_s, int S, c
  * offs [E + 1] and row [P] are device memory (zz_experts_dispatch_dev makes them): offs ascends from
  * 0 or more to P or less, rows of y outside it are left as they were; with an index outside 0 ..
  * R-1 row 0 is taken. bias [E][O], gated [E][2][O]; res [P, O]. P, R <= 2^24; with d_row, R *
- * zz_fp8_row_bytes(I) < 2^32. The form is chosen by the table's size and P: rows' results do not depend
+ * zz_fp8_row_bytes(I) < 2^32. The tiles count as (P + 127 min(E, P)) / 128 tiles of rows. The form is chosen by the table's size and P: rows' results do not depend
  * on how many rows other experts have. With ZZ_EP_8BIT a table's results in bf16 can come from the
  * 8-bit instructions however few rows an expert has. */
 int zz_fp8_matmul_experts_dev(int mat, const uint8_t *d_q, const float *d_s, int R, const int *d_row,

@@ -9,17 +9,22 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 
 
 @pytest.fixture(scope="module")
-def forms(tmp_path_factory):
-    """forms(cases): each one's kernel; a case is (packed rows, columns, rows, matrices, table, 8-bit)."""
+def both(tmp_path_factory):
+    """both(cases): each one's kernel, and whether a launch holds it; a case is (packed rows, columns, rows, matrices, table, 8-bit)."""
     exe = tmp_path_factory.mktemp("form") / "fp8_form"
     subprocess.run(["g++", "-O1", "-std=c++17", "-Wall", "-Werror", os.path.join(HERE, "fp8_form.cpp"), "-o", str(exe)], check=True)
 
     def run(cases):
         text = "\n".join(" ".join(str(int(v)) for v in c) for c in cases)
-        out = subprocess.run([str(exe)], input=text, capture_output=True, text=True, check=True).stdout.split()
+        out = subprocess.run([str(exe)], input=text, capture_output=True, text=True, check=True).stdout.splitlines()
         assert len(out) == len(cases)
-        return [int(v) for v in out]
+        return [tuple(int(v) for v in line.split()) for line in out]
     return run
+
+
+@pytest.fixture(scope="module")
+def forms(both):
+    return lambda cases: [v for v, _ in both(cases)]
 
 
 def test_one_matrix(forms):
@@ -49,3 +54,11 @@ def test_small_tables(forms):
     """Up to 1024 workgroups of the few-row form a table takes what one matrix of its rows does."""
     for o, i, e, per in ((512, 512, 64, 9), (200, 300, 40, 30), (4096, 1024, 8, 20)):
         assert forms([(o, i, e * per, e, 1, 0)])[0] in (0, 1, 2, 14)
+
+
+def test_most_tiles(both):
+    """2^24 tiles of 128 x 128 are 2^32 threads, which no launch holds."""
+    fits = lambda *c: both([(*c, 0)])[0][1]  # noqa: E731
+    assert fits(2 * 8064, 5, 1 << 24, 1, 1) and fits(2 * 8128, 5, (1 << 24) - 1024, 1, 1)
+    assert not fits(2 * 8191, 5, 1 << 24, 1, 1) and not fits(2 * 8191, 5, 1 << 24, 512, 1)
+    assert fits(1 << 24, 128, 120, 120, 1) and not fits(1 << 24, 128, 300, 127, 1)

@@ -53,3 +53,18 @@ def test_largest_gated_pair(O, I):
     finally:
         mat.close()
         torch.cuda.empty_cache()
+
+
+def test_most_tiles():
+    """Results of 2^24 tiles are declined, and why, before anything is launched."""
+    mat = zz.Fp8Experts(1, 8191, 5, gated=True)
+    try:
+        for part in range(2):
+            codes, ws = torch.zeros(8191, 5, dtype=torch.uint8, device="cuda"), torch.ones(64, 1, device="cuda")
+            torch.cuda.synchronize()
+            mat.upload_dev(0, ptr(codes), ptr(ws), part=part)
+        far = [1 << 40, 1 << 41, 1 << 42, 1 << 43]        # pretended addresses
+        with pytest.raises(RuntimeError, match="2\\^24 tiles"):
+            mat.matmul_dev(far[0], far[1], 1 << 24, 0, far[2], 1 << 24, far[3], dtype=zz.ZZ_BF16, stream=stream())
+    finally:
+        mat.close()

@@ -334,6 +334,8 @@ static int ep_run(const char *who, Fp8Mat *m, ZzF8EpCall &c, void *stream) {
     if (!c.ldr) c.ldr = m->O;
     if (c.ldy < m->O || (c.res && c.ldr < m->O)) ZZ_FAIL("%s: rows closer than their width", who);
     if ((int64_t)c.P * m->O >= (int64_t)1 << 37) ZZ_FAIL("%s: results of 2^37 elements or more", who);
+    if (!zz_f8_ep_fits(m->parts * m->O, c.P, c.E, c.offs != nullptr))
+        ZZ_FAIL("%s: results of 2^24 tiles or more (128 rows, %d columns)", who, 128 / m->parts);
     if (c.row && (uint64_t)c.R * zz_fp8_row_bytes(m->I) >= (uint64_t)1 << 32)
         ZZ_FAIL("%s: rows by index within 2^32 bytes", who);
     const int64_t ny = span(c.ldy, c.P, m->O, esz);

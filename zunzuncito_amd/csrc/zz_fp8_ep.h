@@ -123,20 +123,11 @@ __global__ __launch_bounds__(64 * WO * WS * KS, 2) void zz_fp8_tiles_ep_kernel(Z
     zz_fp8_tile<T, G, RO, RS, WO, WS, KS, NS, NT>(a, lds, ot * C::O / 32, st * C::S);
 }
 
-// the most row tiles of `ts` rows that P rows of m experts can make
-static inline int64_t ep_tiles(const ZzF8EpCall &c, int ts) {
-    const int64_t m = c.offs ? (c.E < c.P ? c.E : c.P) : 1;
-    return (c.P + m * (ts - 1)) / ts;
-}
-
-// whether a launch in one dimension holds n workgroups of `threads`
-static inline bool ep_fits(int64_t n, int threads) { return n * threads <= 0xffffffffll; }
-
 template <typename T, int G, int RG, int RS, int NW, bool PF, bool NT>
 static bool launch_few_ep(const ZzF8EpCall &c, const ZzF8Ep &a, hipStream_t st) {
     constexpr int OC = RG * zz_f8_gw<G>;
-    const int64_t n = ep_tiles(c, 32 * RS) * ((a.m.O + OC - 1) / OC);
-    if (!ep_fits(n, 64 * NW)) return false;
+    const int64_t n = zz_f8_ep_tiles(c.P, c.E, c.offs, 32 * RS) * ((a.m.O + OC - 1) / OC);
+    if (!zz_f8_fits(n, 64 * NW)) return false;
     hipLaunchKernelGGL((zz_fp8_few_ep_kernel<T, G, RG, RS, NW, PF, NT>), dim3((unsigned)n), dim3(64 * NW), NW * RG * RS * 4096, st, a);
     return true;
 }
@@ -144,8 +135,8 @@ static bool launch_few_ep(const ZzF8EpCall &c, const ZzF8Ep &a, hipStream_t st) 
 template <typename C, int G>
 static bool launch_tiles_ep(const ZzF8EpCall &c, const ZzF8Ep &a, void (*kernel)(ZzF8Ep), hipStream_t st) {
     constexpr int OC = C::O / 32 * zz_f8_gw<G>;
-    const int64_t n = (ep_tiles(c, C::S) * ((a.m.O + OC - 1) / OC) + 7) / 8 * 8;
-    if (!ep_fits(n, C::NT)) return false;
+    const int64_t n = (zz_f8_ep_tiles(c.P, c.E, c.offs, C::S) * ((a.m.O + OC - 1) / OC) + 7) / 8 * 8;
+    if (!zz_f8_fits(n, C::NT)) return false;
     hipLaunchKernelGGL(kernel, dim3((unsigned)n), dim3(C::NT), C::LDS, st, a);
     return true;
 }

@@ -97,6 +97,20 @@ static inline int zz_f8_ep_form(int O, int P, int per, int m, int nb, bool eight
     return eight || per <= 2 ? 1 : 3;
 }
 
+// The most row tiles of `ts` rows that P rows of E matrices can make; one matrix without a table
+static inline int64_t zz_f8_ep_tiles(int P, int E, bool table, int ts) {
+    const int64_t m = table ? (E < P ? E : P) : 1;
+    return (P + m * (ts - 1)) / ts;
+}
+
+// whether a launch in one dimension holds n workgroups of `threads`
+static inline bool zz_f8_fits(int64_t n, int threads) { return n * threads <= 0xffffffffll; }
+
+// whether there is a form whose launch holds P rows of O packed rows: the largest tiles, 128 x 128 by 256
+static inline bool zz_f8_ep_fits(int O, int P, int E, bool table) {
+    return zz_f8_fits((zz_f8_ep_tiles(P, E, table, 128) * ((O + 127) / 128) + 7) / 8 * 8, 256);
+}
+
 // The kernel of a product with an epilogue: P rows of a table of E matrices (`table`; else one), O packed
 // rows and I columns each. A form, but 14 to 16 the second form's for matrices past the caches, which
 // are read past them too, as zz_fp8_mma.hip's: of several matrices by four waves a workgroup, as the second
