@@ -57,7 +57,8 @@ int zz_add_norm_fp8_dev(int dtype, const void *d_x, int64_t ldx, const void *d_r
                         uint8_t *d_q, float *d_s, void *stream);
 
 /* The same rounding of x itself, without sum and norm: scales and codes are those of f32's
- * quotients to the last bit. Any D up to 2^20, S <= 2^20 (S * ceil(D/128) <= 2^27). */
+ * quotients to the last bit. Any D up to 2^20, S <= 2^24 (S * ceil(D/128) <= 2^27): the
+ * rows that a table's product takes, too. */
 int zz_rows_fp8_dev(int dtype, const void *d_x, int64_t ldx, int S, int D, uint8_t *d_q, float *d_s,
                     void *stream);
 

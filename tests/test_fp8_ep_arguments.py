@@ -25,3 +25,14 @@ def test_activations_pass(act):
     for a in (act, act | zz.ZZ_EP_8BIT):
         for ok in calls(a):       # declined for what comes after: no library, or no such matrix
             assert ok == 0 and any(w in zz.last_error() for w in ("gpu_init", "no such"))
+
+
+@pytest.mark.parametrize("bad, why", [
+    (dict(S=(1 << 24) + 1), "bad arguments"), (dict(S=1 << 24, D=128 * 9), "2\\^27"), (dict(S=1 << 24, ldx=(1 << 36) + 1), "closer"),
+    (dict(S=4, ldx=(1 << 40) + 1), "closer"), (dict(S=1 << 24), "overlaps"), (dict(S=1 << 24, ldx=1 << 36), "overlaps"),
+])
+def test_rows_of_a_table(bad, why):
+    """As many rows are rounded as a table's product takes; what is too many, too far apart or overlaps
+    (here: the codes and x's rows) is declined."""
+    with pytest.raises(RuntimeError, match=why):
+        zz.rows_fp8_dev(**{**dict(d_x=Q, S=4, D=1024, d_q=Q + (1 << 30), d_s=1 << 50), **bad})

@@ -68,3 +68,40 @@ def test_most_tiles():
             mat.matmul_dev(far[0], far[1], 1 << 24, 0, far[2], 1 << 24, far[3], dtype=zz.ZZ_BF16, stream=stream())
     finally:
         mat.close()
+
+
+@pytest.mark.parametrize("dtype, S, D", [(torch.bfloat16, (1 << 20) + 77, 130), (torch.float32, (1 << 20) + 1, 1000),
+                                         (torch.bfloat16, 1 << 24, 96)])
+def test_rows_past_2_20_and_their_product(dtype, S, D):
+    """As many rows as a table's product takes: their codes are those of the rows in two calls, and the
+    product of them with a table is right at both ends."""
+    nb, kind = -(-D // 128), zz.ZZ_BF16 if dtype == torch.bfloat16 else zz.ZZ_F32
+    x = torch.randn(S, D, generator=torch.Generator(device="cuda").manual_seed(3), device="cuda").to(dtype)
+    q, s = torch.full((S + 1, nb * 128), 9, dtype=torch.uint8, device="cuda"), torch.full((nb * S + 1,), 9.0, device="cuda")
+    zz.rows_fp8_dev(ptr(x), S, D, ptr(q), ptr(s), dtype=kind, stream=stream())
+    assert (q[S] == 9).all() and s[nb * S] == 9.0
+    cut = list(range(0, S, 1 << 20)) + [S]
+    for lo, hi in list(zip(cut, cut[1:])):
+        n = hi - lo
+        q1, s1 = torch.empty(n, nb * 128, dtype=torch.uint8, device="cuda"), torch.empty(nb, n, device="cuda")
+        zz.rows_fp8_dev(x[lo:].data_ptr(), n, D, ptr(q1), ptr(s1), dtype=kind, stream=stream())
+        assert torch.equal(q[lo:hi], q1) and torch.equal(s[:nb * S].view(nb, S)[:, lo:hi], s1)
+    E, O = 3, 17
+    w = torch.randint(0, 100, (E, O, D), generator=torch.Generator(device="cuda").manual_seed(4), device="cuda", dtype=torch.uint8)
+    ws = torch.ones(1, nb, device="cuda")
+    mat = zz.Fp8Experts(E, O, D)
+    try:
+        torch.cuda.synchronize()
+        for e in range(E):
+            mat.upload_dev(e, w[e].data_ptr(), ptr(ws))
+        offs = [0, 5, S - 7, S]
+        y, cut = torch.empty(S, O, device="cuda"), torch.tensor(offs, dtype=torch.int32).cuda()
+        mat.matmul_dev(ptr(q), ptr(s), S, 0, ptr(cut), S, ptr(y), stream=stream())
+        f8 = torch.float8_e4m3fn
+        for e, at in ((0, slice(0, 5)), (1, slice(5, 40)), (1, slice(S - 40, S - 7)), (2, slice(S - 7, S))):
+            rows = q[at].view(f8).double() * s[:nb * S].view(nb, S)[:, at].t().repeat_interleave(128, 1).double()
+            v = w[e].view(f8).double()
+            off = (y[at].double() - rows[:, :D] @ v.t()).abs()
+            assert (off <= (2 * 128 + nb + 18) * 2.0 ** -24 * (rows[:, :D].abs() @ v.t().abs())).all()
+    finally:
+        mat.close()

@@ -38,12 +38,13 @@ extern "C" int64_t zz_fp8_row_bytes(int64_t D) {
     return D < 1 ? -1 : (D + ZZ_F8B - 1) / ZZ_F8B * ZZ_F8B;
 }
 
-static int rows_common(const char *who, int dtype, const void *x, int64_t *ldx, int S, int D, const uint8_t *q,
+static int rows_common(const char *who, int dtype, const void *x, int64_t *ldx, int S, int most, int D, const uint8_t *q,
                        const float *s) {
     if (dtype != ZZ_F32 && dtype != ZZ_BF16) ZZ_FAIL("%s: dtype %d declined", who, dtype);
-    if (!x || !q || !s || S < 1 || S > ZZ_F8_MAXS || D < 1) ZZ_FAIL("%s: bad arguments (1 <= S <= 2^20)", who);
+    if (!x || !q || !s || S < 1 || S > most || D < 1) ZZ_FAIL("%s: bad arguments (1 <= S <= %d)", who, most);
     if (!*ldx) *ldx = D;
-    if (*ldx < D || *ldx > (int64_t)1 << 40) ZZ_FAIL("%s: rows closer than their width", who);
+    // S rows' bytes stay under 2^62
+    if (*ldx < D || *ldx > (int64_t)1 << (S > ZZ_F8_MAXS ? 36 : 40)) ZZ_FAIL("%s: rows closer than their width", who);
     const int esz = dtype == ZZ_F32 ? 4 : 2;
     if ((uintptr_t)x % esz || (uintptr_t)q % 16 || (uintptr_t)s % 4) ZZ_FAIL("%s: misaligned pointer", who);
     return 1;
@@ -55,7 +56,7 @@ extern "C" int zz_add_norm_fp8_dev(int dtype, const void *d_x, int64_t ldx, cons
                                    void *d_sum, int64_t lds, const float *d_w, float eps, int S, int D,
                                    uint8_t *d_q, float *d_s, void *stream) {
     const char *who = "zz_add_norm_fp8_dev";
-    if (!rows_common(who, dtype, d_x, &ldx, S, D, d_q, d_s)) return 0;
+    if (!rows_common(who, dtype, d_x, &ldx, S, ZZ_F8_MAXS, D, d_q, d_s)) return 0;
     if (D > ZZ_F8_MAXNORM) ZZ_FAIL("%s: D <= %d", who, ZZ_F8_MAXNORM);
     if (!(eps >= 0.0f) || isinf(eps)) ZZ_FAIL("%s: eps has to be finite and not negative", who);
     const int esz = dtype == ZZ_F32 ? 4 : 2;
@@ -89,7 +90,7 @@ extern "C" int zz_add_norm_fp8_dev(int dtype, const void *d_x, int64_t ldx, cons
 extern "C" int zz_rows_fp8_dev(int dtype, const void *d_x, int64_t ldx, int S, int D, uint8_t *d_q, float *d_s,
                                void *stream) {
     const char *who = "zz_rows_fp8_dev";
-    if (!rows_common(who, dtype, d_x, &ldx, S, D, d_q, d_s)) return 0;
+    if (!rows_common(who, dtype, d_x, &ldx, S, ZZ_F8_MAXP, D, d_q, d_s)) return 0;
     if (D > 1 << 20 || (int64_t)S * zz_f8_nb(D) > 1 << 27) ZZ_FAIL("%s: D <= 2^20, S * ceil(D/128) <= 2^27", who);
     const int esz = dtype == ZZ_F32 ? 4 : 2;
     const int64_t nx = span(ldx, S, D, esz), nq = S * zz_fp8_row_bytes(D), ns = (int64_t)zz_f8_nb(D) * S * 4;
