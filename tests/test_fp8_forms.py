@@ -1,6 +1,7 @@
 """The form that a product with an epilogue takes (zunzuncito_amd/csrc/zz_fp8_form.h, built here for the
 host): rules on sizes."""
 import os
+import random
 import subprocess
 
 import pytest
@@ -62,3 +63,44 @@ def test_most_tiles(both):
     assert fits(2 * 8064, 5, 1 << 24, 1, 1) and fits(2 * 8128, 5, (1 << 24) - 1024, 1, 1)
     assert not fits(2 * 8191, 5, 1 << 24, 1, 1) and not fits(2 * 8191, 5, 1 << 24, 512, 1)
     assert fits(1 << 24, 128, 120, 120, 1) and not fits(1 << 24, 128, 300, 127, 1)
+
+
+def some_sizes(table, eight, n=100000):
+    """(packed rows, columns, rows, matrices, table, 8-bit) over the sizes that calls have"""
+    rng = random.Random(2)
+    size = lambda top: round(2 ** rng.uniform(0, top))  # noqa: E731
+    return [(size(17), size(13), size(14), size(9) if table else 1, table, eight) for _ in range(n)]
+
+
+def sizes_of(test, *names):
+    """What a test is parametrised with, as dicts."""
+    for mark in test.pytestmark:
+        if mark.name == "parametrize":
+            args = [a.strip() for a in mark.args[0].split(",")]
+            if set(names) <= set(args):
+                yield from (dict(zip(args, v)) for v in mark.args[1])
+
+
+@pytest.mark.parametrize("gated", [False, True])
+def test_exact_sums_are_tested_in_every_form(forms, gated):
+    """The sizes of test_gpu_fp8_sums.py, which are run in both types, take every form there is."""
+    import test_gpu_fp8_sums as T
+    G = 2 if gated else 1
+    for table, sizes in ((0, [(G * o, i, s, 1, 0, 0) for s, o, i in T.SINGLE]), (1, [(G * o, i, p, e, 1, 0) for e, p, o, i in T.TABLES])):
+        assert set(forms(sizes)) == set(forms(some_sizes(table, 0)))
+
+
+@pytest.mark.parametrize("gated", [False, True])
+def test_8bit_tiles_are_tested_in_every_form(forms, gated):
+    """test_gpu_fp8_eight.py has each of the three 8-bit tiles, for one matrix and for tables, plain and
+    gated."""
+    import test_gpu_fp8_eight as T
+    G = 2 if gated else 1
+    one, table = [], []
+    for f in (v for k, v in vars(T).items() if k.startswith("test_")):
+        mine = [d for d in sizes_of(f, "O", "I") if d.get("gated", gated) == gated]
+        one += [(G * d["O"], d["I"], d["S"], 1, 0, 1) for d in mine if "S" in d]
+        table += [(G * d["O"], d["I"], d["P"], d["E"], 1, 1) for d in mine if "P" in d]
+    for t, sizes in ((0, one), (1, table)):
+        assert {11, 12, 13} <= set(forms(sizes))
+        assert {11, 12, 13} == {v for v in forms(some_sizes(t, 1)) if 10 < v < 14}

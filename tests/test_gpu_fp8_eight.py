@@ -35,3 +35,10 @@ for _name in ("test_epilogue", "test_epilogue_in_every_form", "test_epilogue_in_
               "test_experts_in_the_smaller_forms", "test_experts_far_rows", "test_experts_far_codes", "test_experts_most_rows",
               "test_layer", "test_streams_and_graphs"):
     globals()[_name] = again(getattr(T, _name))
+
+
+# tables on the 8-bit 64 x 64 tiles too, which only many narrow experts take
+@pytest.mark.parametrize("gated, E, P, O, I", [(False, 130, 15554, 33, 3290), (True, 132, 14468, 17, 2353), (False, 17, 1145, 3035, 319),
+                                               (True, 4, 257, 6359, 279)])
+def test_tables_on_the_8bit_tiles(gated, E, P, O, I):
+    T.test_experts_in_every_form(T.BF16, gated, E, P, O, I)

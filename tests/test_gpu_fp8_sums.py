@@ -5,9 +5,9 @@ import pytest
 import torch
 
 import zzref8 as R
-import zzrefx as X
 import zunzuncito_amd as zz
-from test_gpu_experts import BF16, F32, KIND, Case, near, picked, ptr, spread, stream
+import test_gpu_experts
+from test_gpu_experts import BF16, F32, KIND, ptr, spread, stream
 
 pytestmark = pytest.mark.gpu
 
@@ -58,7 +58,8 @@ class Whole:
 
 SINGLE = [(1, 2816, 2112), (8, 1000, 704), (3, 65600, 1088), (20, 32800, 1088), (33, 4284, 649), (37, 4162, 810), (65, 5447, 796),
           (137, 5631, 392), (361, 1352, 514), (455, 3107, 263), (518, 3466, 260), (1090, 3600, 257), (1239, 5017, 260),
-          (1764, 1194, 263), (1926, 1555, 259), (2048, 2112, 2816), (8300, 4224, 130)]
+          (1764, 1194, 263), (1926, 1555, 259), (2048, 2112, 2816), (8300, 4224, 130), (774, 1236, 1559), (9, 31746, 2273),
+          (292, 426, 521)]
 
 
 @pytest.mark.parametrize("gated", [False, True])
@@ -77,27 +78,38 @@ def test_sums_are_exact(S, O, I, gated):
 
 TABLES = [(137, 195, 34, 609), (8, 36, 4324, 267), (38, 1235, 213, 770), (51, 3492, 143, 667), (128, 512, 704, 300),
           (13, 400, 700, 259), (428, 1965, 139, 280), (6, 395, 4274, 263), (31, 2019, 1774, 267), (8, 4100, 1056, 257),
-          (128, 8192, 704, 512)]
+          (128, 8192, 704, 512), (8, 4, 704, 1024), (32, 4, 704, 2816), (2, 261, 1781, 691), (2, 2, 24578, 1370), (3, 874, 135, 558),
+          (2, 456, 540, 918), (2, 2, 23064, 733), (2, 1, 31431, 2178), (1, 9, 31746, 2273)]
 
 
 @pytest.mark.parametrize("gated", [False, True])
 @pytest.mark.parametrize("E, P, O, I", TABLES)
 def test_sums_of_a_table_are_exact(E, P, O, I, gated):
     for dtype in (BF16, F32):
-        print("case", E, P, O, I, gated, dtype, flush=True)
-        n = max(1, P // 2)
-        c = Whole(E, 2 if gated else 1, O, I, n, E + P)
-        try:
-            offs = spread(P, E, "skew", E + P).cuda()
-            at = torch.randint(0, n, (P,), generator=torch.Generator().manual_seed(P)).cuda()
-            row = at.int()
-            y = torch.full((P + 1, O), 9.0, dtype=dtype, device="cuda")
-            c.mat.matmul_dev(ptr(c.q), ptr(c.s), n, ptr(row), ptr(offs), P, ptr(y), dtype=KIND[dtype], stream=stream())
-            k = int(offs[E])
-            e = torch.searchsorted(offs.long(), torch.arange(k, device="cuda"), right=True) - 1
-            assert torch.equal(y[:k], c.want(at[:k], e, dtype)) and (y[k:] == 9.0).all()
-        finally:
-            c.mat.close()
+        for indexed in (True, False):
+            print("case", E, P, O, I, gated, dtype, indexed, flush=True)
+            n = max(1, P // 2) if indexed else P
+            c = Whole(E, 2 if gated else 1, O, I, n, E + P)
+            try:
+                at = torch.randint(0, n, (P,), generator=torch.Generator().manual_seed(P)).cuda() if indexed else torch.arange(P, device="cuda")
+                row = at.int() if indexed else None
+                for kind in ("skew", "one", "late"):
+                    offs = spread(P, E, kind, E + P).cuda()
+                    y = torch.full((P + 1, O), 9.0, dtype=dtype, device="cuda")
+                    c.mat.matmul_dev(ptr(c.q), ptr(c.s), n, ptr(row), ptr(offs), P, ptr(y), dtype=KIND[dtype], stream=stream())
+                    lo, hi = int(offs[0]), int(offs[E])
+                    e = torch.searchsorted(offs.long(), torch.arange(lo, hi, device="cuda"), right=True) - 1
+                    assert torch.equal(y[lo:hi], c.want(at[lo:hi], e, dtype)) and (y[:lo] == 9.0).all() and (y[hi:] == 9.0).all()
+            finally:
+                c.mat.close()
+
+
+# the same tables with bias, activation and residual, few rows of the sixteen-wave form among them
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("E, P, O, I", [t for t in TABLES if t[0] * t[2] * t[3] < 1 << 24] + [(8, 5, 704, 1024), (32, 7, 704, 1280)])
+def test_tables_in_every_form(E, P, O, I, gated):
+    for dtype in (F32, BF16):
+        test_gpu_experts.test_experts_in_every_form(dtype, gated, E, P, O, I)
 
 
 def normal_codes(n, I, seed, per):
