@@ -1,9 +1,10 @@
-"""The fp8 product's far limits: the largest gated pairs."""
+"""The fp8 product's far limits: the largest gated pairs, results, rows by index and rows."""
 import pytest
 import torch
 
 import zunzuncito_amd as zz
-from test_gpu_experts import ptr, stream
+from test_gpu_experts import BF16, F32, KIND, ptr, stream
+from test_gpu_fp8_sums import Whole
 
 pytestmark = pytest.mark.gpu
 
@@ -105,3 +106,27 @@ def test_rows_past_2_20_and_their_product(dtype, S, D):
             assert (off <= (2 * 128 + nb + 18) * 2.0 ** -24 * (rows[:, :D].abs() @ v.t().abs())).all()
     finally:
         mat.close()
+
+
+@pytest.mark.parametrize("dtype, eight, P, O", [(F32, 0, 9, 33), (BF16, 0, 9, 33), (F32, 0, 300, 200), (BF16, 0, 300, 200), (F32, 0, 4000, 1030),
+                                                (BF16, 0, 4000, 1030), (BF16, zz.ZZ_EP_8BIT, 4000, 1030), (BF16, zz.ZZ_EP_8BIT, 9000, 2050)])
+def test_rows_by_index_up_to_2_32_bytes(dtype, eight, P, O):
+    """Codes of just under 2^32 bytes, of which only the first rows, the last and those on both sides of
+    2^31 are named; every other row's are NaN."""
+    E, I, n = 2, 1 << 16, (1 << 16) - 1
+    c = Whole(E, 1, O, I, n, 3, big=not eight)
+    try:
+        assert (1 << 32) - (1 << 16) == c.q.numel()
+        named = torch.tensor([0, 1, 32766, 32767, 32768, 32769, n - 2, n - 1], device="cuda")
+        keep = c.q[named].clone()
+        c.q.fill_(0x7F)
+        c.q[named] = keep
+        at = named[torch.randint(0, 8, (P,), generator=torch.Generator().manual_seed(1)).cuda()]
+        at[:8], at[P - 8:] = named, named
+        row, offs = at.int(), torch.tensor([0, P // 3, P], dtype=torch.int32).cuda()
+        y = torch.full((P + 1, O), 9.0, dtype=dtype, device="cuda")
+        c.mat.matmul_dev(ptr(c.q), ptr(c.s), n, ptr(row), ptr(offs), P, ptr(y), act=eight, dtype=KIND[dtype], stream=stream())
+        e = (torch.arange(P, device="cuda") >= P // 3).long()
+        assert torch.equal(y[:P], c.want(at, e, dtype)) and (y[P] == 9.0).all()
+    finally:
+        c.mat.close()

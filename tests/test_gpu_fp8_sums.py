@@ -24,9 +24,10 @@ def e4m3(v):
 class Whole:
     """Codes whose sums are whole in every order of addition, and which 13 bits do not hold: of 16 columns
     in a row's somewhere, the first of each eight have products of 2^14 and -2^14, four beside the first
-    x w with x a power of two, w of 4 bits. A result, 4 x w (gated: 16 x^2 w), is one of bf16."""
+    x w with x a power of two, w of 4 bits. A result, 4 x w (gated: 16 x^2 w), is one of bf16. big False:
+    without the large products, so that 13 bits do hold them."""
 
-    def __init__(self, E, G, O, I, n, seed):
+    def __init__(self, E, G, O, I, n, seed, big=True):
         g = torch.Generator(device="cuda").manual_seed(seed)
         pick = lambda lo, hi, *k: torch.randint(lo, hi, k, generator=g, device="cuda")  # noqa: E731
         self.E, self.G, self.O, self.I, self.n = E, G, O, I, n
@@ -34,7 +35,7 @@ class Whole:
         self.w = pick(8, 16, E, O).float() / 8 * 2.0 ** pick(-1, 2, E, O).float()
         self.x, self.size = 2.0 ** pick(-1, 3, n).float(), 2.0 ** pick(-2, 3, n).float()
         w = torch.zeros(G, O, I, device="cuda")
-        w[:, :, at], w[:, :, at + 8] = 64.0, -64.0
+        w[:, :, at], w[:, :, at + 8] = (64.0, -64.0) if big else (0.0, 0.0)
         nb = R.blocks(I)
         x = torch.zeros(n, nb * 128, dtype=torch.uint8, device="cuda")
         x[:, at] = x[:, at + 8] = e4m3(torch.tensor(256.0))
@@ -110,6 +111,21 @@ def test_sums_of_a_table_are_exact(E, P, O, I, gated):
 def test_tables_in_every_form(E, P, O, I, gated):
     for dtype in (F32, BF16):
         test_gpu_experts.test_experts_in_every_form(dtype, gated, E, P, O, I)
+
+
+@pytest.mark.parametrize("gated", [False, True])
+def test_what_the_8bit_choice_leaves_alone(gated):
+    """f32 results, and few rows of one matrix: bit for bit the same with ZZ_EP_8BIT and without."""
+    for dtype, S, O, I in ((F32, 1, 300, 200), (F32, 700, 2000, 513), (F32, 2048, 2112, 300), (BF16, 1, 2816, 512), (BF16, 32, 4224, 700)):
+        c = Whole(1, 2 if gated else 1, O, I, S, 4)
+        try:
+            q = torch.randint(0, 120, c.q.shape, generator=torch.Generator().manual_seed(2), dtype=torch.uint8).cuda()
+            y, z = (torch.empty(S, O, dtype=dtype, device="cuda") for _ in range(2))
+            c.mat.matmul_ep_dev(ptr(q), ptr(c.s), S, ptr(y), act=2, dtype=KIND[dtype], stream=stream())
+            c.mat.matmul_ep_dev(ptr(q), ptr(c.s), S, ptr(z), act=2 | zz.ZZ_EP_8BIT, dtype=KIND[dtype], stream=stream())
+            assert torch.equal(y, z) and y.isfinite().all()
+        finally:
+            c.mat.close()
 
 
 def normal_codes(n, I, seed, per):
