@@ -100,11 +100,12 @@ int zz_fp8_upload_expert_dev(int mat, int e, int part, const uint8_t *d_codes, c
  *   y = act(v) + res                                        a plain matrix
  *   y = act(min(v_gate, clamp)) * clip(v_up, -clamp, clamp) + res       a gated pair
  * in f32, rounded once to `dtype`. bias f32 [O], a gated pair's [2][O], gate's first (NULL:
- * none); act ZZ_EP_*, with or without ZZ_EP_8BIT; clamp > 0, or 0 for none (a plain matrix takes none); res [S, O] of `dtype`,
- * rows ldr apart (0: O; NULL: none), may be y itself, rows as far apart. The activations are of
- * one hardware exponential and one reciprocal: off by up to (6 + 10 |a|) 2^-24 of the value, a
- * the exponent, beside what v is off. A NaN stays one; act(-infinity) is NaN, infinity times
- * 0. The order in which the blocks of 128 columns are added up follows from the sizes, S among them:
+ * none); act ZZ_EP_*, with or without ZZ_EP_8BIT; clamp > 0, or 0 for none (a plain matrix takes
+ * none); res [S, O] of `dtype`, rows ldr apart (0: O; NULL: none), may be y itself, rows as far apart. The
+ * activations are of one hardware exponential and one reciprocal: off by up to (6 + 10 |a|) 2^-24 of
+ * the value, a the exponent, beside what v is off; where a is above 87.3, so that 1 / (1 + exp(a)) is less than
+ * 2^-126, they may be 0 for less than |v| 2^-126. A NaN stays one; act(-infinity) is NaN, infinity
+ * times 0. The order in which the blocks of 128 columns are added up follows from the sizes, S among them:
  * a row's result can differ in its last bits between calls of different S.
  * With ZZ_EP_8BIT in act, results in bf16 of more than some dozens of rows come from the 8-bit matrix
  * instructions, at up to twice the rate: within each 8 columns a product is cut, towards zero, to 13

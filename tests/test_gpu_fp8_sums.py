@@ -128,6 +128,30 @@ def test_what_the_8bit_choice_leaves_alone(gated):
             c.mat.close()
 
 
+def test_activations_over_their_range():
+    """silu and gelu of v alone (the bias, behind sums of zero) as near as zz_fp8.h says, on both sides of
+    where the reciprocal leaves f32's normal numbers."""
+    v = np.concatenate([np.linspace(-120, 120, 6001), np.linspace(-87.2, -88.9, 2001), np.linspace(-10.2, -10.0, 2001),
+                        np.linspace(-1, 1, 2001), [-1e30, -1e5, 1e5, 1e30, 1e-30, -1e-30, 0.0]]).astype(np.float32)
+    O = v.size
+    bias = torch.from_numpy(v).cuda()
+    mat = zz.Fp8Experts(1, O, 128)
+    try:
+        mat.upload(0, np.zeros((O, 128), np.uint8), np.ones((R.blocks(O), 1), np.float32))
+        q, s = torch.zeros(1, 128, dtype=torch.uint8, device="cuda"), torch.ones(1, 1, device="cuda")
+        x = v.astype(np.float64)
+        for act, a in ((zz.ZZ_EP_SILU, -x), (zz.ZZ_EP_GELU_TANH, -np.sqrt(8.0 / np.pi) * (x + 0.044715 * x ** 3))):
+            y = torch.empty(1, O, device="cuda")
+            mat.matmul_ep_dev(ptr(q), ptr(s), 1, ptr(y), d_bias=ptr(bias), act=act, stream=stream())
+            with np.errstate(over="ignore"):
+                want = x / (1.0 + np.exp(a))
+            bound = (6 + 10 * np.minimum(np.abs(a), 1e4)) * 2.0 ** -24 * np.abs(want) + np.where(a > 87.3, np.abs(x) * 2.0 ** -126, 0.0) + 2.0 ** -149
+            off = np.abs(y[0].double().cpu().numpy() - want)
+            assert np.all(off <= bound), (act, v[~(off <= bound)][:5], off[~(off <= bound)][:5])
+    finally:
+        mat.close()
+
+
 def normal_codes(n, I, seed, per):
     """e4m3 codes and scales of normal values, the largest of each `per` x 128 block at 448."""
     v = torch.randn(-(-n // per) * per, R.blocks(I) * 128, generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda")

@@ -142,7 +142,7 @@ __global__ __launch_bounds__(1024) void zz_xp_count_kernel(XpArgs a) {
 // The positions of a chunk's pairs. Each of 16 waves has a run of them: how many of an expert lie
 // in the waves before is added up in LDS; within a wave's 64 pairs, the lanes with the same expert
 // are found by a ballot for each bit of the id. Nothing depends on the order of atomics. A wave's
-// pairs are requested 256 at a time, and the first 256 kept for the second pass.
+// pairs are requested 256 at a time; up to 256 it keeps for the second pass, more it requests again.
 template <bool ONE>
 __global__ __launch_bounds__(1024) void zz_xp_place_kernel(XpArgs a) {
     __shared__ int wcnt[16][ZZ_EXPERTS_MAXE], total[ZZ_EXPERTS_MAXE], pre[ZZ_EXPERTS_MAXE], base[ZZ_EXPERTS_MAXE + 1];
