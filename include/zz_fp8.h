@@ -124,9 +124,10 @@ int zz_fp8_matmul_ep_dev(int mat, const uint8_t *d_q, const float *d_s, int S, c
  * offs [E + 1] and row [P] are device memory (zz_experts_dispatch_dev makes them): offs ascends from
  * 0 or more to P or less, rows of y outside it are left as they were; with an index outside 0 ..
  * R-1 row 0 is taken. bias [E][O], gated [E][2][O]; res [P, O]. P, R <= 2^24; with d_row, R *
- * zz_fp8_row_bytes(I) < 2^32. The tiles count as (P + 127 min(E, P)) / 128 tiles of rows. The form is chosen by the table's size and P: rows' results do not depend
- * on how many rows other experts have. With ZZ_EP_8BIT a table's results in bf16 can come from the
- * 8-bit instructions however few rows an expert has. */
+ * zz_fp8_row_bytes(I) < 2^32. Tiles count as (P + 127 min(E, P)) / 128 of rows times those of columns. The
+ * form is chosen by the table's size and P: rows' results do not depend on how many rows other experts
+ * have. With ZZ_EP_8BIT a table's results in bf16 can come from the 8-bit instructions however few rows
+ * an expert has. */
 int zz_fp8_matmul_experts_dev(int mat, const uint8_t *d_q, const float *d_s, int R, const int *d_row,
                               const int *d_offs, int P, const float *d_bias, int act, float clamp,
                               const void *d_res, int64_t ldr, int dtype, void *d_y, int64_t ldy, void *stream);

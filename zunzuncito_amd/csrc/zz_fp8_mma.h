@@ -125,7 +125,7 @@ __device__ __forceinline__ int zz_f8_row(const A &a, int t) {
 }
 
 // The same for N rows t0 + t[k] of a tile, their indexes requested together (one after the other, a
-// tile began two microseconds later: 32768 rows of 128 experts, 1408 x 2816 gated, took 172 us for 160);
+// tile began two microseconds later: 32768 rows to 8 of 128 experts, 1408 x 2816 gated, took 172 us for 160);
 // without an index t stays as it is, from the tile's first row.
 template <int G, int N, typename A>
 __device__ __forceinline__ void zz_f8_rows(const A &a, int t0, unsigned (&t)[N]) {

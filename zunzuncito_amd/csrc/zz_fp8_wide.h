@@ -14,14 +14,15 @@
 // zz_fp8_mma.h's f16 products all the same.
 //
 // Without the conversions and at twice the rate: 8192 x 2816 x 2112 65 us (1.50 PFLOP/s) where the
-// f16 tiles take 115; 2048 x 4224 x 2816 gated 36.4 for 71; 32768 rows of 128 experts, 1408 x 2816,
-// 153 for 263. What bounds them is the way of the codes to the matrix cores, which are 40 % busy at
-// 1.9 GHz: 32 KB a block for 128 x 128, and 128 bytes a cycle of LDS. So a wave keeps 32 packed
-// rows times all rows of the tile: its part of the matrix lies in operand order, no other wave wants
-// it, and it comes straight into registers, past LDS, which then holds more blocks. With the matrix
-// through LDS and waves of 64 x 32 the same three took 63.5, 37.6 and 153, but 128 experts of 256
-// rows each 224 for 197, 64 of 512 188 for 169, 64 rows each 125 for 120. Measured and not better,
-// 128 x 128 at 164: 256 x 256 (166) and 256 x 128 (184), 64 x 64 a wave (170), a third workgroup on a
+// f16 tiles take 115; 2048 x 4224 x 2816 gated 36.8 for 66; 32768 rows of 128 experts, 1408 x 2816, 256
+// each 204 for 298, all of 8 experts 161 for 295. Nothing is full (in the order of the last three): the
+// matrix cores are 25, 31 and 40 % busy, LDS's index path 16, 20 and 26 % with conflicts below 1 %, of
+// memory 1.4 TB/s are asked. Two waves a SIMD wait for each other's round, and at a tile's start and end.
+// A wave keeps 32 packed rows times all rows of the tile: its part of the matrix lies in operand order, no
+// other wave wants it, and it comes straight into registers, past LDS, which then holds more blocks. With the matrix
+// through LDS and waves of 64 x 32 128 experts of 256 rows each took 224 for 197, 64 of 512 188 for 169, 64
+// rows each 125 for 120. Measured and not better (8 experts of 4096 rows, 128 x 128 at 164): 256 x 256 (166)
+// and 256 x 128 (184), 64 x 64 a wave (170), a third workgroup on a
 // CU (spills), the row operands' next block read over the barrier (170), later lines touched for the
 // L2 (199 and more), the XCDs' parts cut by the matrices they read (171: more workgroups without a tile).
 #pragma once
